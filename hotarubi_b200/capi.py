@@ -108,6 +108,113 @@ class Rows(ctypes.Structure):
     ]
 
 
+DT_F32, DT_BF16, DT_E5M2 = 0, 1, 2
+
+
+class KvCache(ctypes.Structure):
+    """hrb_kv_cache: a 4-bit key/value cache in pages."""
+    _fields_ = [
+        ("data", ctypes.c_void_p), ("page_stride", ctypes.c_uint64), ("pages", ctypes.c_uint32),
+        ("page", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("hd", ctypes.c_uint32),
+    ]
+
+
+class BlocksDesc(ctypes.Structure):
+    """hrb_blocks_desc."""
+    _fields_ = [
+        ("seqs", ctypes.c_uint32), ("page", ctypes.c_uint32),
+        ("cached", ctypes.c_void_p), ("fresh", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+        ("nfree", ctypes.c_uint32), ("head_in", ctypes.c_void_p), ("head_out", ctypes.c_void_p),
+        ("table", ctypes.c_void_p), ("table_ld", ctypes.c_uint32), ("q_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("pos", ctypes.c_void_p),
+        ("max_tokens", ctypes.c_uint32),
+    ]
+
+
+class QkvDesc(ctypes.Structure):
+    """hrb_qkv_desc."""
+    _fields_ = [
+        ("cache", KvCache), ("tokens", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+        ("dtype", ctypes.c_uint32), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p), ("ldq", ctypes.c_uint64), ("ldk", ctypes.c_uint64),
+        ("ldv", ctypes.c_uint64), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
+        ("eps", ctypes.c_float), ("rope", ctypes.c_void_p), ("max_pos", ctypes.c_uint32),
+        ("rot", ctypes.c_uint32), ("interleaved", ctypes.c_uint32), ("pos", ctypes.c_void_p),
+        ("axes", ctypes.c_uint32), ("sections", ctypes.c_uint32 * 3), ("slots", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p), ("ldqo", ctypes.c_uint64),
+    ]
+
+
+class AttnDesc(ctypes.Structure):
+    """hrb_attn_desc."""
+    _fields_ = [
+        ("cache", KvCache), ("seqs", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+        ("q", ctypes.c_void_p), ("ldq", ctypes.c_uint64), ("q_start", ctypes.c_void_p),
+        ("total_q", ctypes.c_uint32), ("max_q", ctypes.c_uint32), ("kv_len", ctypes.c_void_p),
+        ("max_kv", ctypes.c_uint32), ("total_kv", ctypes.c_uint64), ("table", ctypes.c_void_p),
+        ("table_ld", ctypes.c_uint32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+        ("causal", ctypes.c_uint32), ("window", ctypes.c_uint32), ("prefix", ctypes.c_void_p),
+        ("slopes", ctypes.c_void_p), ("out", ctypes.c_void_p), ("ldo", ctypes.c_uint64),
+        ("oq", ctypes.c_void_p), ("oscale", ctypes.c_void_p), ("ldoq", ctypes.c_uint64),
+        ("oquant", ctypes.c_uint32), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+def kv_record_bytes(page: int, hd: int) -> int:
+    """hrb_kv_record_bytes: bytes of one (page, head) record."""
+    return page * (hd + hd // 16)
+
+
+def kv_cache(data, pages: int, page: int, kv_heads: int, hd: int, page_stride: int = 0) -> KvCache:
+    """A cache over the device bytes `data`, [pages][kv_heads][record] unless
+    page_stride (bytes) says otherwise."""
+    return KvCache(_ptr(data), page_stride, pages, page, kv_heads, hd)
+
+
+def blocks_desc(seqs: int, page: int, *, cached, fresh, free_pages, nfree, table, table_ld, q_start,
+                kv_len, slots, max_tokens, pos=None, head_in=None, head_out=None) -> BlocksDesc:
+    return BlocksDesc(seqs, page, _ptr(cached), _ptr(fresh), _ptr(free_pages), nfree,
+                      _ptr(head_in), _ptr(head_out), _ptr(table), table_ld, _ptr(q_start),
+                      _ptr(kv_len), _ptr(slots), _ptr(pos), max_tokens)
+
+
+def qkv_desc(cache: KvCache, tokens: int, heads: int, *, q, k, v, slots, q_out, dtype=DT_F32,
+             ldq=None, ldk=None, ldv=None, q_norm=None, k_norm=None, eps=1e-6, rope=None,
+             max_pos=0, rot=0, interleaved=False, pos=None, axes=1, sections=(),
+             ldqo=None) -> QkvDesc:
+    """hrb_qkv_desc.  Row strides default to packed rows; `rope` is the
+    [max_pos][rot / 2][2] table of (cos, sin)."""
+    w, kw = heads * cache.hd, cache.kv_heads * cache.hd
+    cuts = tuple(sections) + (0,) * (3 - len(sections))
+    return QkvDesc(cache, tokens, heads, dtype, _ptr(q), _ptr(k), _ptr(v),
+                   w if ldq is None else ldq, kw if ldk is None else ldk,
+                   kw if ldv is None else ldv, _ptr(q_norm), _ptr(k_norm), eps, _ptr(rope),
+                   max_pos, rot, 1 if interleaved else 0, _ptr(pos), axes,
+                   (ctypes.c_uint32 * 3)(*cuts), _ptr(slots), _ptr(q_out),
+                   w if ldqo is None else ldqo)
+
+
+def attn_desc(cache: KvCache, seqs: int, heads: int, *, q, q_start, total_q, max_q, kv_len, max_kv,
+              table, table_ld, scale, total_kv=0, ldq=None, softcap=0.0, causal=True, window=0,
+              prefix=None, slopes=None, out=None, ldo=None, oq=None, oscale=None, ldoq=0,
+              oquant=QUANT_VEC, workspace=None, workspace_bytes=0) -> AttnDesc:
+    """hrb_attn_desc; q and out rows are packed unless ldq and ldo say otherwise."""
+    w = heads * cache.hd
+    return AttnDesc(cache, seqs, heads, _ptr(q), w if ldq is None else ldq, _ptr(q_start), total_q,
+                    max_q, _ptr(kv_len), max_kv, total_kv, _ptr(table), table_ld, scale, softcap,
+                    1 if causal else 0, window, _ptr(prefix), _ptr(slopes), _ptr(out),
+                    w if ldo is None else ldo, _ptr(oq), _ptr(oscale), ldoq, oquant,
+                    _ptr(workspace), workspace_bytes)
+
+
+def rope_table(max_pos: int, rot: int, theta: float = 10000.0) -> np.ndarray:
+    """The [max_pos][rot / 2][2] FP32 table of (cos, sin) of pos / theta^(2p / rot)."""
+    inv = theta ** (-np.arange(rot // 2, dtype=np.float64) * 2 / rot)
+    angle = np.arange(max_pos, dtype=np.float64)[:, None] * inv
+    return np.stack((np.cos(angle), np.sin(angle)), -1).astype(np.float32)
+
+
 NULL_ENTRY = 0xFFFFFFFF
 
 
@@ -215,6 +322,13 @@ def load() -> ctypes.CDLL:
             "hrb_image_data": (P, [P]),
             "hrb_image_weights": (ctypes.c_int, [P, P, u32, ctypes.c_uint64, ctypes.c_uint64,
                                                  u32, u32, P, P, P]),
+            "hrb_kv_record_bytes": (ctypes.c_uint64, [u32, u32]),
+            "hrb_block_tables": (ctypes.c_int, [P, ctypes.POINTER(BlocksDesc), P]),
+            "hrb_qkv_append": (ctypes.c_int, [P, ctypes.POINTER(QkvDesc), P]),
+            "hrb_kv_read": (ctypes.c_int, [P, ctypes.POINTER(KvCache), P, u32, u32, P, P, P]),
+            "hrb_attention": (ctypes.c_int, [P, ctypes.POINTER(AttnDesc), P]),
+            "hrb_attention_workspace": (ctypes.c_int, [P, ctypes.POINTER(AttnDesc),
+                                                       ctypes.POINTER(ctypes.c_uint64)]),
             "hrb_gemm_image": (ctypes.c_int, [P, P, ctypes.POINTER(GemmDesc), ctypes.c_uint64,
                                               ctypes.c_uint64, P]),
         }
@@ -522,6 +636,28 @@ class Library:
         d = GaccDesc(tokens, slots, corners, blocks, _ptr(entries), _ptr(w), _ptr(rows),
                      row_stride, nrows, _ptr(out), 1 if accumulate else 0)
         self._check(self.lib.hrb_gacc_dense(self.ctx, ctypes.byref(d), stream or None))
+
+    # -- serving ----------------------------------------------------------
+    def block_tables(self, d: BlocksDesc, stream: int = 0) -> None:
+        self._check(self.lib.hrb_block_tables(self.ctx, ctypes.byref(d), stream or None))
+
+    def qkv_append(self, d: QkvDesc, stream: int = 0) -> None:
+        self._check(self.lib.hrb_qkv_append(self.ctx, ctypes.byref(d), stream or None))
+
+    def kv_read(self, cache: KvCache, slots, tokens: int, k=None, v=None, dtype=DT_F32,
+                stream: int = 0) -> None:
+        """hrb_kv_read: the cached rows at `slots` as values."""
+        self._check(self.lib.hrb_kv_read(self.ctx, ctypes.byref(cache), _ptr(slots), tokens, dtype,
+                                         _ptr(k), _ptr(v), stream or None))
+
+    def attention(self, d: AttnDesc, stream: int = 0) -> None:
+        self._check(self.lib.hrb_attention(self.ctx, ctypes.byref(d), stream or None))
+
+    def attention_workspace(self, d: AttnDesc) -> int:
+        """Scratch bytes an hrb_attention call with this descriptor needs."""
+        n = ctypes.c_uint64()
+        self._check(self.lib.hrb_attention_workspace(self.ctx, ctypes.byref(d), ctypes.byref(n)))
+        return int(n.value)
 
     def conv(self, d: ConvDesc, stream: int = 0) -> None:
         self._check(self.lib.hrb_conv_dense(self.ctx, ctypes.byref(d), stream or None))

@@ -20,6 +20,7 @@
 
 #include "hrb_gemm.h"
 #include "hrb_kernels.cuh"
+#include "hrb_serve.cuh"
 #include "hrb_tc.cuh"
 
 struct hrb_ctx {
@@ -42,6 +43,9 @@ struct hrb_ctx {
   // The int8 weight chunks of the tensor-core exact GEMM (launch_x_translate).
   void* xscratch = nullptr;
   size_t xscratch_bytes = 0;
+  // Scratch of the serving calls (serve.cu).
+  void* serve = nullptr;
+  size_t serve_bytes = 0;
   // Bit 0: the encoder met Inf/NaN; bit 1: a tensor-core kernel gave up
   // waiting (it then leaves its outputs unwritten).
   uint32_t* d_error = nullptr;
@@ -792,6 +796,17 @@ QuantJob make_quant_job_for_noalloc(const hrb_gemm_desc* d, int8_t* q, uint8_t* 
 QuantJob make_post_quant_job_for_noalloc(const hrb_gemm_desc* d) { return post_quant_job(d); }
 
 int ctx_device(const hrb_ctx* ctx) { return ctx->device; }
+cudaStream_t ctx_stream(const hrb_ctx* ctx, void* stream) {
+  return stream != nullptr ? static_cast<cudaStream_t>(stream) : ctx->stream;
+}
+uint32_t* ctx_error_word(const hrb_ctx* ctx) { return ctx->d_error; }
+int ctx_sm_count(const hrb_ctx* ctx) { return ctx->sm_count; }
+void ctx_count_launches(hrb_ctx* ctx, uint32_t n) { ctx->launches += n; }
+hrb_status ctx_serve_scratch(hrb_ctx* ctx, size_t bytes, void** out) {
+  const hrb_status st = grow(ctx, &ctx->serve, &ctx->serve_bytes, bytes);
+  *out = ctx->serve;
+  return st;
+}
 
 hrb_status ctx_fail(hrb_ctx* ctx, hrb_status status, const char* message) {
   return fail(ctx, status, "%s", message);
@@ -861,6 +876,7 @@ hrb_status hrb_destroy(hrb_ctx* ctx) {
   cudaFree(ctx->scratch);
   cudaFree(ctx->staging);
   cudaFree(ctx->xscratch);
+  cudaFree(ctx->serve);
   cudaFree(ctx->d_error);
   if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
   delete ctx;
@@ -883,6 +899,16 @@ hrb_status hrb_sync(hrb_ctx* ctx) {
     if (flag & hrb::kErrScaleRange) {
       return fail(ctx, HRB_EDATA, "an activation scale byte of 255 has no tensor-core encoding "
                                   "(use HRB_MODE_EXACT)");
+    }
+    if (flag & hrb::kErrKvSlot) {
+      return fail(ctx, HRB_EDATA, "a slot, position or block table entry is out of range");
+    }
+    if (flag & hrb::kErrKvNonFinite) {
+      return fail(ctx, HRB_EDATA, "a key or value to cache is infinite or NaN");
+    }
+    if (flag & hrb::kErrKvPages) {
+      return fail(ctx, HRB_EDATA, "block tables: a token without a page or past max_tokens, or a "
+                                  "negative length");
     }
     return fail(ctx, HRB_EDATA, "MXINT8 input is infinite or NaN");
   }

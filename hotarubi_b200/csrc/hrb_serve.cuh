@@ -1,0 +1,99 @@
+// Job descriptors and launchers of the serving kernels (section 11 of
+// hrb_gemm.h), and what their entry points (serve.cu) use of a context.
+// Internal to libhrb_gemm.so.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "hrb_gemm.h"
+#include "hrb_kv.cuh"
+
+namespace hrb {
+
+// Context fields for serve.cu (defined in capi.cu).
+cudaStream_t ctx_stream(const hrb_ctx* ctx, void* stream);
+uint32_t* ctx_error_word(const hrb_ctx* ctx);
+int ctx_sm_count(const hrb_ctx* ctx);
+void ctx_count_launches(hrb_ctx* ctx, uint32_t n);
+// The context's scratch of the serving calls, grown to `bytes`.
+hrb_status ctx_serve_scratch(hrb_ctx* ctx, size_t bytes, void** out);
+
+struct BlocksJob {
+  const int32_t *cached, *fresh, *free_pages, *head_in;
+  int32_t *head_out, *table, *q_start, *kv_len, *slots, *pos;
+  uint32_t seqs, page_log2, nfree, table_ld, max_tokens;
+};
+void launch_block_tables(const BlocksJob& job, uint32_t* error_flag, cudaStream_t stream);
+
+struct QkvJob {
+  KvCache cache;
+  const void* x[3];       // q, k, v
+  uint64_t ld[3];         // elements
+  const float* norm[2];   // of q and k, or null
+  const float2* rope;     // [max_pos][half], or null
+  const int32_t* pos;     // [axes][tokens]
+  const int32_t* slots;
+  void* q_out;
+  uint64_t ldqo;
+  float eps;
+  uint32_t tokens, heads, max_pos, half, interleaved;
+  uint32_t cut[2];        // first pairs of axes 1 and 2 (half where there is none)
+};
+// vec: every row starts at a multiple of four elements' bytes.
+void launch_qkv_append(const QkvJob& job, bool bf16, bool vec, uint32_t* error_flag, int sm_count,
+                       cudaStream_t stream);
+void launch_kv_read(const KvCache& cache, const int32_t* slots, uint32_t tokens, uint32_t dtype,
+                    void* k, void* v, uint32_t* error_flag, int sm_count, cudaStream_t stream);
+
+struct AttnJob {
+  KvCache cache;
+  const uint16_t* q;      // BF16 bits
+  uint64_t ldq;
+  const int32_t *q_start, *kv_len, *table, *prefix;
+  const float* slopes;
+  uint16_t* out;          // BF16 bits, or null
+  uint64_t ldo;
+  int8_t* oq;             // or null
+  uint8_t* oscale;
+  uint64_t ldoq;
+  uint32_t vec_rule;
+  uint32_t seqs, heads, group, total_q, max_q, max_kv, table_ld;
+  uint32_t causal, window;
+  float scale, softcap;
+};
+
+// The keys row position i of request n may see: [lo, hi) and [0, pre), both
+// held to the request's keys.
+struct Seen {
+  int32_t lo, hi, pre;
+};
+__device__ __forceinline__ Seen attn_seen(const AttnJob& j, int32_t i, int32_t kv, int32_t pre) {
+  Seen s;
+  if (!j.causal) {
+    s.lo = 0;
+    s.hi = kv;
+    s.pre = 0;
+  } else {
+    s.hi = min(max(i + 1, 0), kv);
+    s.lo = j.window != 0 && i >= static_cast<int32_t>(j.window)
+               ? i + 1 - static_cast<int32_t>(j.window) : 0;
+    s.pre = min(pre, kv);
+  }
+  return s;
+}
+__device__ __forceinline__ bool attn_sees(const Seen& s, int32_t k) {
+  return (k >= s.lo && k < s.hi) || k < s.pre;
+}
+
+// FP32 to BF16 bits, to nearest even.
+__device__ __forceinline__ uint16_t attn_bf16(float x) {
+  uint16_t r;
+  asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(x));
+  return r;
+}
+
+void launch_attn_simple(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
+
+}  // namespace hrb

@@ -46,7 +46,8 @@ typedef enum hrb_status {
   HRB_ENOMEM = 3,   /* device or pinned host allocation failed */
   HRB_ENOTSUP = 4,  /* valid request this build does not serve */
   HRB_EDATA = 5     /* non-finite activation given to the MXINT8 encoder
-                       (formats.cpp:37 Require) */
+                       (formats.cpp:37 Require), or data of the serving calls
+                       (section 11) outside what they name */
 } hrb_status;
 
 typedef struct hrb_ctx hrb_ctx;
@@ -640,6 +641,178 @@ typedef struct hrb_rows {
  * and MXFP4) a scale byte of 255, is reported by hrb_sync (HRB_EDATA). */
 HRB_API hrb_status hrb_gemm_rows(hrb_ctx* ctx, const hrb_gemm_desc* desc, const hrb_rows* rows,
                                  void* stream);
+
+/* ---------------------------------------------------------------------
+ * 11. Serving attention over a 4-bit cache.  No counterpart in the
+ *    reference, whose NPU attends over at most 256 MXINT8 keys with two GEMM
+ *    instructions and VEC programs (tools/compiler/kernels.cpp:155-244); here
+ *    a server of many requests gets the steps between its QKV and output
+ *    Linears:
+ *      hrb_block_tables  pages and slots of this step's tokens;
+ *      hrb_qkv_append    norms and rotation of q and k, k and v encoded into
+ *                        the cache;
+ *      hrb_attention     attention of the new tokens over the cache.
+ *    All pointers are device pointers unless said otherwise; every call is
+ *    asynchronous on `stream` and reads request lengths, tables and slots on
+ *    the device, so a step can be captured into a CUDA graph (with a
+ *    workspace of the caller's, or after one call of the same size).
+ * ------------------------------------------------------------------- */
+
+/* Keys and values in MXFP4 (E2M1 codes, one E8M0 scale byte per 32 dims, the
+ * weight format HRB_WFMT_MXFP4), in pages of `page` tokens.  The record of
+ * (page p, head h) starts at data + p * page_stride + h * record bytes and
+ * holds, in this order:
+ *   K codes [page][hd / 2], K scales [page][hd / 32],
+ *   V codes [page][hd / 2], V scales [page][hd / 32]
+ * (hrb_kv_record_bytes in all), dim 2j in the low nibble of byte j.  Scale
+ * byte b is 2^(b - 127); hrb_qkv_append writes bytes 104..140 (2^-23..2^13)
+ * and readers take a byte outside as the nearest of these, so that every
+ * cached value is an FP16 number.  Token t of a page table row is at slot
+ * table[t / page] * page + t % page. */
+typedef struct hrb_kv_cache {
+  uint8_t* data;         /* 16-byte aligned */
+  uint64_t page_stride;  /* bytes, a multiple of 16, at least kv_heads *
+                            hrb_kv_record_bytes(page, hd); 0: that */
+  uint32_t pages;
+  uint32_t page;         /* tokens a page: 16, 32, 64, 128 or 256 */
+  uint32_t kv_heads;
+  uint32_t hd;           /* dims a head: 32, 64, 96 or 128 */
+} hrb_kv_cache;
+
+/* page * (hd + hd / 16): 136 bytes a token at hd = 128. */
+HRB_API uint64_t hrb_kv_record_bytes(uint32_t page, uint32_t hd);
+
+/* Element types of the serving calls' rows. */
+typedef enum hrb_dtype {
+  HRB_DT_F32 = 0,
+  HRB_DT_BF16 = 1,
+  HRB_DT_E5M2 = 2   /* FP8: holds every cached value of 2^-16 and above exactly */
+} hrb_dtype;
+
+/* Block tables and slot maps of one step.  Request i has cached[i] tokens in
+ * the cache and adds fresh[i]:
+ *   have_i = ceil(cached[i] / page)    need_i = ceil((cached[i] + fresh[i]) / page) - have_i
+ *   table[i][have_i + n] = free_pages[head + sum_{j<i} need_j + n],  n < need_i
+ *   q_start[i] = sum_{j<i} fresh[j]    kv_len[i] = cached[i] + fresh[i]
+ * and new token r of request i, token q_start[i] + r of the step, is at
+ * position pos = cached[i] + r and slot table[i][pos / page] * page + pos %
+ * page.  Table entries other than those are left alone; slots and pos of
+ * tokens from q_start[seqs] up to max_tokens become -1 and 0 (a step padded
+ * to a fixed size).  Tokens whose page is missing (the free list has run out,
+ * the row is full, or the table's own entry is negative) get slot -1, a table
+ * entry without a page becomes -1, tokens past max_tokens are dropped, a
+ * negative length counts as 0: hrb_sync then reports HRB_EDATA. */
+typedef struct hrb_blocks_desc {
+  uint32_t seqs;               /* at most 65536 */
+  uint32_t page;               /* tokens a page, as hrb_kv_cache's */
+  const int32_t* cached;       /* [seqs] */
+  const int32_t* fresh;        /* [seqs] */
+  const int32_t* free_pages;   /* [nfree] */
+  uint32_t nfree;
+  const int32_t* head_in;      /* [1] first unused entry of free_pages, or NULL: 0 */
+  int32_t* head_out;           /* [1] head + pages asked for, or NULL.  Another
+                                  address than head_in */
+  int32_t* table;              /* [seqs][table_ld], in and out */
+  uint32_t table_ld;
+  int32_t* q_start;            /* [seqs + 1] */
+  int32_t* kv_len;             /* [seqs] */
+  int32_t* slots;              /* [max_tokens] */
+  int32_t* pos;                /* [max_tokens], or NULL */
+  uint32_t max_tokens;
+} hrb_blocks_desc;
+HRB_API hrb_status hrb_block_tables(hrb_ctx* ctx, const hrb_blocks_desc* desc, void* stream);
+
+/* The rows of the QKV Linear to the query operand and the cache, one pass:
+ *   q, k:  x = x / sqrt(mean(x^2) + eps) * norm       (per head; NULL: x as it is)
+ *          (x_a, x_b) = (x_a c - x_b s, x_b c + x_a s) over the pairs of the
+ *          first `rot` dims: pair p is dims (p, p + rot / 2), or (2p, 2p + 1)
+ *          with `interleaved`; (c, s) = rope[pos][p]
+ *   q_out = BF16(q);  k and v encoded into the cache at the token's slot.
+ * With several axes (time, height, width) pair p takes the position of the
+ * axis whose section holds p: the first sections[0] pairs axis 0, the next
+ * sections[1] axis 1, and so on.
+ * Encoding, per 32 dims: e = floor(log2 max|x|) - 2 held to -23..13, code =
+ * E2M1 nearest x / 2^e, ties to even, saturating at 6; a block of zeros has
+ * e = -23.  Arithmetic is FP32, each of the two roundings once.
+ * A negative slot caches nothing (q_out is still written).  hrb_sync reports
+ * HRB_EDATA for a slot or position outside the cache or the table (nothing is
+ * cached; the row is not rotated) and for Inf or NaN in k or v (NaN is cached
+ * as 0, Inf saturates).  Two tokens of one call must not share a slot. */
+typedef struct hrb_qkv_desc {
+  hrb_kv_cache cache;
+  uint32_t tokens, heads;
+  uint32_t dtype;                  /* HRB_DT_F32 or HRB_DT_BF16: q, k and v */
+  const void *q, *k, *v;           /* [tokens][heads * hd], [tokens][kv_heads * hd] twice */
+  uint64_t ldq, ldk, ldv;          /* elements between rows */
+  const float *q_norm, *k_norm;    /* [hd], or NULL */
+  float eps;
+  const float* rope;               /* [max_pos][rot / 2][2] (cos, sin), or NULL: no rotation */
+  uint32_t max_pos, rot;           /* rot even, at most hd */
+  uint32_t interleaved;
+  const int32_t* pos;              /* [axes][tokens] */
+  uint32_t axes, sections[3];      /* 1..3; sections sum to rot / 2 (ignored for one axis) */
+  const int32_t* slots;            /* [tokens] */
+  void* q_out;                     /* BF16 [tokens][ldqo] */
+  uint64_t ldqo;
+} hrb_qkv_desc;
+HRB_API hrb_status hrb_qkv_append(hrb_ctx* ctx, const hrb_qkv_desc* desc, void* stream);
+
+/* The cached keys and values of `tokens` slots as the values they stand for:
+ * k, v [tokens][kv_heads * hd] of `dtype` (FP32 and BF16 hold them exactly);
+ * either may be NULL.  A negative slot reads as zeros, one outside the cache
+ * too, with HRB_EDATA from hrb_sync. */
+HRB_API hrb_status hrb_kv_read(hrb_ctx* ctx, const hrb_kv_cache* cache, const int32_t* slots,
+                               uint32_t tokens, uint32_t dtype, void* k, void* v, void* stream);
+
+/* Attention of the step's tokens over the cache.  Request n has the rows
+ * q_start[n] .. q_start[n + 1] - 1 of q, its last tokens, and kv_len[n] keys;
+ * row r of it is at position i = kv_len[n] - (its rows) + r.  Query head h
+ * reads key/value head h / (heads / kv_heads).
+ *   s_j = scale * q . k_j;  softcap: s_j = softcap * tanh(s_j / softcap);
+ *   slopes: s_j -= slopes[h] * |i - j|;  out = sum_j softmax_j(s) v_j
+ * over the keys 0 <= j < kv_len[n] that row sees: all of them, or with
+ * `causal` those with j <= i (and j > i - window, when window is not 0) and
+ * those with j < prefix[n].  A row that sees none gives zeros.  Scores,
+ * softmax statistics and sums are FP32; q and the softmax weights enter the
+ * tensor cores as FP16 (q after a power-of-two scaling of its row).
+ * A table entry outside the cache reads as a page of zeros, with HRB_EDATA
+ * from hrb_sync. */
+typedef struct hrb_attn_desc {
+  hrb_kv_cache cache;
+  uint32_t seqs, heads;
+  const void* q;             /* BF16 [total_q][ldq], 16-byte aligned rows */
+  uint64_t ldq;
+  const int32_t* q_start;    /* [seqs + 1] */
+  uint32_t total_q, max_q;   /* rows of q and out; most rows of one request */
+  const int32_t* kv_len;     /* [seqs] */
+  uint32_t max_kv;           /* most keys of one request */
+  uint64_t total_kv;         /* keys of all requests together, or more; 0: seqs * max_kv */
+  const int32_t* table;      /* [seqs][table_ld] */
+  uint32_t table_ld;         /* at least ceil(max_kv / page) */
+  float scale, softcap;      /* softcap 0: none */
+  uint32_t causal, window;
+  const int32_t* prefix;     /* [seqs], or NULL */
+  const float* slopes;       /* [heads], or NULL */
+  void* out;                 /* BF16 [total_q][ldo], or NULL with oq */
+  uint64_t ldo;
+  /* Optional MXINT8 copy of the output for the output Linear, as
+   * hrb_gemm_desc's cq: codes [total_q][ldoq] and scales [total_q][ldoq / 32]
+   * (ldoq a multiple of 32, at least heads * hd; 0: heads * hd) of the FP32
+   * result, by the rule `oquant` (hrb_quant). */
+  int8_t* oq;
+  uint8_t* oscale;
+  uint64_t ldoq;
+  uint32_t oquant;
+  /* Scratch, 256-byte aligned, of at least hrb_attention_workspace bytes for
+   * this descriptor; NULL: the context's own (grown by the call when it is
+   * too small, and shared by the context's calls). */
+  void* workspace;
+  uint64_t workspace_bytes;
+} hrb_attn_desc;
+HRB_API hrb_status hrb_attention(hrb_ctx* ctx, const hrb_attn_desc* desc, void* stream);
+/* Host only: the scratch bytes a call with this descriptor needs. */
+HRB_API hrb_status hrb_attention_workspace(hrb_ctx* ctx, const hrb_attn_desc* desc,
+                                           uint64_t* bytes);
 
 #ifdef __cplusplus
 }
