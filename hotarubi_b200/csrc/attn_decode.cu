@@ -1,0 +1,719 @@
+// hrb_attention for few rows a request (single tokens, a few speculated
+// ones): the cache is streamed once and everything else hides behind it.
+//
+// A block serves one request, one key/value head and a chunk of its keys;
+// all rows that read that head (rows of q times query heads a key/value head,
+// at most 8 NT) are one operand.  Each of its warps takes tiles of 32 keys
+// on its own: bulk copies bring a tile's codes and scales into the warp's
+// ring in shared memory, the lanes turn them into FP16 in registers
+// (cvt.e2m1x2, times the block scale: both exact) straight in the layout of
+// an mma.sync operand, and with the running maximum m and sum l of a row
+//   S^T = K Q^T           (keys x rows; m16n8k16, the keys as the 16)
+//   p = 2^(s - m)         (FP16 for the product, FP32 for l)
+//   O^T += V^T P^T        (dims x rows; the dims as the 16)
+// Keys and dims, not rows, fill the 16 of the instruction, so 8 rows or
+// fewer waste nothing; tcgen05 would need the decoded keys written to shared
+// memory first (2 bytes a code against half a byte read).  The order of the
+// reduced index is free, so a lane reads consecutive dims of a key: its 32
+// nibbles are one 16-byte load at hd = 128.
+// m only moves when a score passes it by 2^8 (a vote, no shuffles), which
+// FP16 weights allow.
+//
+// Chunks of one request are joined by k_attn_join from the rows' (m, l, O)
+// in FP32.
+//
+// Bound by HBM for long histories: hd + hd / 16 bytes a key and head.
+#include <cuda_fp16.h>
+
+#include <atomic>
+#include <cstdint>
+
+#include "hrb_quant.cuh"
+#include "hrb_serve.cuh"
+#include "sm100.cuh"
+
+namespace hrb {
+namespace {
+
+using namespace sm100;
+
+constexpr uint32_t kTile = 32;   // keys a stage
+constexpr uint32_t kWarps = 4;
+constexpr uint32_t kStages = 3;
+constexpr float kLazy = 8.0f;    // log2 of the most a weight may pass 1 before m moves
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) {
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  return half2_bits(__hmul2(*reinterpret_cast<const __half2*>(&a),
+                            *reinterpret_cast<const __half2*>(&b)));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                    uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Where a tile's parts lie in a stage: pages of 16 tokens bring two records,
+// larger pages 32 tokens of one.
+struct TileGeom {
+  uint32_t ks, v, vs;          // K scales, V codes, V scales (K codes at 0)
+  uint32_t code_half, scale_half;  // from tokens 0..15 to 16..31
+};
+template <uint32_t HD>
+__device__ __forceinline__ TileGeom tile_geom(uint32_t page) {
+  const uint32_t n = min(page, kTile);
+  TileGeom g;
+  g.ks = n * (HD / 2u);
+  g.v = n * (HD / 2u + HD / 32u);
+  g.vs = g.v + n * (HD / 2u);
+  g.code_half = page == 16u ? 16u * (HD + HD / 16u) : 16u * (HD / 2u);
+  g.scale_half = page == 16u ? 16u * (HD + HD / 16u) : 16u * (HD / 32u);
+  return g;
+}
+
+// Two scale bytes as FP16 powers of two, `lo` in the low half.
+__device__ __forceinline__ uint32_t scale2(uint32_t lo, uint32_t hi) {
+  return half2_bits(__floats2half2_rn(kv_scale(lo), kv_scale(hi)));
+}
+
+// FP32 value of dim 32 b + lane of one output row and head, to BF16 and to
+// the MXINT8 copy.
+__device__ __forceinline__ void write_block(const AttnJob& j, uint64_t row, uint32_t head,
+                                            uint32_t b, uint32_t lane, float x,
+                                            uint32_t* error_flag) {
+  const uint32_t col = head * j.cache.hd + 32u * b + lane;
+  if (j.out != nullptr) j.out[row * j.ldo + col] = attn_bf16(x);
+  if (j.oq == nullptr) return;
+  const uint32_t bits = __float_as_uint(x), mag = bits & 0x7FFFFFFFu;
+  const uint32_t key = __reduce_max_sync(0xFFFFFFFFu, j.vec_rule ? mag >> 23 : mag);
+  uint32_t scale;
+  const int32_t code = mxint8_code(bits, key, j.vec_rule != 0, scale);
+  j.oq[row * j.ldoq + col] = static_cast<int8_t>(code);
+  if (lane == 0u) j.oscale[row * (j.ldoq / 32u) + col / 32u] = static_cast<uint8_t>(scale);
+  if (mag >= 0x7F800000u && !j.vec_rule) atomicOr(error_flag, 1u);
+}
+
+template <uint32_t HD, uint32_t NT>
+struct Smem {
+  static constexpr uint32_t kStageBytes = kTile * (HD + HD / 16u);
+  static constexpr uint32_t kRing = kWarps * kStages * kStageBytes;
+  static constexpr uint32_t kJoin = kWarps * 8u * NT * (HD + 4u) * 4u;
+  static constexpr uint32_t kBuf = kRing > kJoin ? kRing : kJoin;
+  static constexpr uint32_t kQ = NT > 2u ? 8u * NT * HD * 2u : 0u;  // Q fragments, see below
+  static constexpr uint32_t kBytes = kBuf + kQ + kWarps * kStages * 8u;
+};
+
+template <uint32_t HD, uint32_t NT>
+__global__ void __launch_bounds__(kWarps * 32)
+    k_attn_decode(const AttnJob j, uint32_t* __restrict__ error_flag) {
+  using S = Smem<HD, NT>;
+  constexpr uint32_t kSteps = HD / 16u;           // MMAs along dims; m16 tiles of dims
+  constexpr uint32_t kRows = 8u * NT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+  const uint32_t g = lane >> 2, t = lane & 3u;
+  uint8_t* ring = smem + warp * kStages * S::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBuf + S::kQ) + warp * kStages;
+
+  const uint32_t n = blockIdx.z, head = blockIdx.y;
+  int32_t q0, q_len, kv;
+  if (!attn_request(j, n, &q0, &q_len, &kv)) {
+    if (blockIdx.x == 0u && threadIdx.x == 0u) atomicOr(error_flag, kErrKvSlot);
+    return;
+  }
+  const int32_t rows = q_len * static_cast<int32_t>(j.group);
+  const int32_t c0 = static_cast<int32_t>(blockIdx.x * j.chunk);
+  if (rows == 0 || (c0 >= kv && c0 > 0)) return;
+  const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
+  const bool whole = kv <= static_cast<int32_t>(j.chunk);  // no other chunk of this request
+
+  if (lane < kStages) mbar_init(full + lane, 1);
+  fence_barrier_init();
+  __syncwarp();
+
+  // The keys that the rows see, and the tiles of this warp among them.
+  const int32_t pre = j.prefix != nullptr ? __ldg(j.prefix + n) : 0;
+  const Seen first = attn_seen(j, kv - q_len, kv, pre), last = attn_seen(j, kv - 1, kv, pre);
+  const int32_t tiles = (c1 - c0 + static_cast<int32_t>(kTile) - 1) / static_cast<int32_t>(kTile);
+  auto tile_seen = [&](int32_t i) {
+    const int32_t a = c0 + i * static_cast<int32_t>(kTile), b = a + static_cast<int32_t>(kTile);
+    return (b > first.lo && a < last.hi) || a < first.pre;
+  };
+
+  const TileGeom geo = tile_geom<HD>(j.cache.page);
+  const int32_t* table = j.table + static_cast<uint64_t>(n) * j.table_ld;
+  const uint32_t copies = j.cache.page == 16u ? 2u : j.cache.page == 32u ? 1u : 4u;
+  // Lane l holds the pages of the warp's tile number base + l.
+  int32_t page_a = -1, page_b = -1, base = 0;
+  auto load_pages = [&](int32_t at) {  // tiles number at .. at + 31 of this warp
+    base = at;
+    const int32_t i = static_cast<int32_t>(warp) + (at + static_cast<int32_t>(lane)) * static_cast<int32_t>(kWarps);
+    const int32_t k = c0 + i * static_cast<int32_t>(kTile);
+    page_a = k < kv ? __ldg(table + (k >> j.cache.page_log2)) : -2;
+    page_b = page_a;
+    if (j.cache.page == 16u) page_b = k + 16 < kv ? __ldg(table + ((k + 16) >> 4)) : -2;
+  };
+  // -2: no keys there; other values outside the cache read as zeros.
+  auto issue = [&](int32_t number, uint32_t stage) {
+    const int32_t i = static_cast<int32_t>(warp) + number * static_cast<int32_t>(kWarps);
+    const uint32_t k = static_cast<uint32_t>(c0 + i * static_cast<int32_t>(kTile));
+    const int32_t pa = __shfl_sync(0xFFFFFFFFu, page_a, number - base);
+    const int32_t pb = __shfl_sync(0xFFFFFFFFu, page_b, number - base);
+    const int32_t page = lane == 1u && j.cache.page == 16u ? pb : pa;
+    const bool there = page >= 0 && static_cast<uint32_t>(page) < j.cache.pages;
+    uint8_t* dst = ring + stage * S::kStageBytes;
+    uint32_t bytes, from;
+    if (j.cache.page <= 32u) {
+      bytes = j.cache.record;
+      from = 0;
+      dst += lane * j.cache.record;
+    } else {
+      const uint32_t in = k & (j.cache.page - 1u);
+      const bool scales = (lane & 1u) != 0u;
+      bytes = scales ? kTile * (HD / 32u) : kTile * (HD / 2u);
+      from = (lane >= 2u ? kv_vcodes(j.cache) : 0u) +
+             (scales ? kv_kscales(j.cache) + in * (HD / 32u) : in * (HD / 2u));
+      dst += (lane >= 2u ? geo.v : 0u) + (scales ? geo.ks : 0u);
+    }
+    const bool copy = lane < copies && there;
+    const uint32_t total = __reduce_add_sync(0xFFFFFFFFu, copy ? bytes : 0u);
+    if (lane == 0u) mbar_arrive_expect_tx(full + stage, total);
+    __syncwarp();
+    if (copy) {
+      bulk_g2s(dst, kv_record(j.cache, static_cast<uint32_t>(page), head) + from, bytes,
+               full + stage);
+    }
+  };
+
+  // Q: row r of the operand is row r / group of q, head r % group of this
+  // key/value head's.  Lane (g, t) holds dims [t HD / 4, (t + 1) HD / 4) of
+  // row 8 nt + g as FP16 pairs, its row scaled so that its largest value is
+  // in [2^13, 2^14): bf16's 8 bits fit in 11, and what falls under FP16's
+  // range is 2^-37 of the row's largest.
+  uint32_t qf[NT <= 2u ? NT : 1u][kSteps][2];
+  uint32_t* q_smem = reinterpret_cast<uint32_t*>(smem + S::kBuf);
+  float row_scale[NT];  // of row 8 nt + g
+#pragma unroll
+  for (uint32_t nt = 0; nt < NT; ++nt) {
+    const int32_t r = static_cast<int32_t>(8u * nt + g);
+    uint32_t w[HD / 8u];
+#pragma unroll
+    for (uint32_t i = 0; i < HD / 8u; ++i) w[i] = 0;
+    if (r < rows) {
+      const uint64_t row = static_cast<uint64_t>(q0 + r / static_cast<int32_t>(j.group));
+      const uint32_t h = head * j.group + static_cast<uint32_t>(r) % j.group;
+      const uint4* src = reinterpret_cast<const uint4*>(j.q + row * j.ldq + h * HD + t * (HD / 4u));
+#pragma unroll
+      for (uint32_t i = 0; i < HD / 32u; ++i) {
+        const uint4 v = __ldg(src + i);
+        w[4u * i] = v.x;
+        w[4u * i + 1u] = v.y;
+        w[4u * i + 2u] = v.z;
+        w[4u * i + 3u] = v.w;
+      }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < HD / 8u; ++i) {
+      top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+    }
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    const int32_t e = min(max(static_cast<int32_t>(top >> 7), 27), 254) - 127;
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
+    row_scale[nt] = __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
+#pragma unroll
+    for (uint32_t i = 0; i < HD / 8u; ++i) {
+      const uint32_t h2 = half2_bits(__floats2half2_rn(__uint_as_float(w[i] << 16) * up,
+                                                       __uint_as_float(w[i] & 0xFFFF0000u) * up));
+      if constexpr (NT <= 2u) {
+        qf[nt][i / 2u][i & 1u] = h2;
+      } else if (warp == 0u) {
+        q_smem[((nt * kSteps + i / 2u) * 32u + lane) * 2u + (i & 1u)] = h2;
+      }
+    }
+  }
+  if constexpr (NT > 2u) __syncthreads();
+  // The lane's two rows of each n tile in S^T and O^T: 8 nt + 2 t + {0, 1}.
+  float factor[NT][2], m[NT][2], l[NT][2], slope[NT][2];
+  Seen seen[NT][2];
+  int32_t pos[NT][2];
+  const bool capped = j.softcap != 0.f;
+#pragma unroll
+  for (uint32_t nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (uint32_t c = 0; c < 2u; ++c) {
+      const int32_t r = static_cast<int32_t>(8u * nt + 2u * t + c);
+      const float sc = __shfl_sync(0xFFFFFFFFu, row_scale[nt], (2u * t + c) * 4u);
+      factor[nt][c] = j.scale * sc * (capped ? 1.0f : kLog2e);
+      m[nt][c] = -INFINITY;
+      l[nt][c] = 0.f;
+      pos[nt][c] = kv - q_len + r / static_cast<int32_t>(j.group);
+      seen[nt][c] = attn_seen(j, pos[nt][c], kv, pre);
+      if (r >= rows) seen[nt][c].lo = seen[nt][c].hi = seen[nt][c].pre = 0;
+      slope[nt][c] = j.slopes != nullptr && r < rows
+                         ? __ldg(j.slopes + head * j.group + static_cast<uint32_t>(r) % j.group) * kLog2e
+                         : 0.f;
+    }
+  }
+  float o[NT][kSteps][4];
+#pragma unroll
+  for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (uint32_t i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (uint32_t c = 0; c < 4u; ++c) o[nt][i][c] = 0.f;
+
+  // The warp's tiles: number x is tile warp + x kWarps of the chunk.
+  const int32_t mine = (tiles - static_cast<int32_t>(warp) + static_cast<int32_t>(kWarps) - 1) /
+                       static_cast<int32_t>(kWarps);
+  auto next = [&](int32_t x) {  // the next number from x on whose tile is seen
+    while (x < mine && !tile_seen(static_cast<int32_t>(warp) + x * static_cast<int32_t>(kWarps))) ++x;
+    return x;
+  };
+  load_pages(0);
+  int32_t ahead = next(0);  // next to issue
+  int32_t at = ahead;       // next to use
+  uint32_t in_flight = 0;
+  // Pages of the tile in use are read again from lane registers: keep the
+  // numbers in use and in flight within the 32 that are loaded.
+  for (uint32_t s = 0; s < kStages; ++s) {
+    if (ahead < mine && ahead < base + 32) {
+      issue(ahead, s);
+      ++in_flight;
+      ahead = next(ahead + 1);
+    }
+  }
+  uint32_t stage = 0, parity = 0;
+  bool ok = true, bad_page = false;
+  while (at < mine) {
+    if (in_flight == 0u) {  // the loaded pages are used up
+      load_pages(at);
+      for (uint32_t s = 0, st = stage; s < kStages; ++s) {
+        if (ahead < mine && ahead < base + 32) {
+          issue(ahead, st);
+          ++in_flight;
+          ahead = next(ahead + 1);
+        }
+        st = st + 1u == kStages ? 0u : st + 1u;
+      }
+    }
+    const int32_t pa = __shfl_sync(0xFFFFFFFFu, page_a, at - base);
+    const int32_t pb = __shfl_sync(0xFFFFFFFFu, page_b, at - base);
+    const bool bad_a = pa != -2 && static_cast<uint32_t>(pa) >= j.cache.pages;
+    const bool bad_b = pb != -2 && static_cast<uint32_t>(pb) >= j.cache.pages;
+    const int32_t k0 = c0 + (static_cast<int32_t>(warp) + at * static_cast<int32_t>(kWarps)) *
+                                static_cast<int32_t>(kTile);
+    ok = mbar_wait(full + stage, parity, error_flag);
+    if (!__all_sync(0xFFFFFFFFu, ok)) break;
+    const uint8_t* tile = ring + stage * S::kStageBytes;
+
+    // S^T: keys k0 + 16 hf + {g, g + 8}, rows {2t, 2t + 1} of each n tile.
+    float s[NT][2][4];
+#pragma unroll
+    for (uint32_t hf = 0; hf < 2u; ++hf) {
+      const uint8_t* kc = tile + hf * geo.code_half;
+      const uint8_t* ks = tile + geo.ks + hf * geo.scale_half;
+      uint32_t w[2][HD / 32u];
+      uint32_t sc[2][2];  // the lane's block scales (two blocks at hd 96)
+#pragma unroll
+      for (uint32_t r = 0; r < 2u; ++r) {
+        const uint8_t* p = kc + (g + 8u * r) * (HD / 2u) + t * (HD / 8u);
+        if constexpr (HD == 128u) {
+          const uint4 v = *reinterpret_cast<const uint4*>(p);
+          w[r][0] = v.x;
+          w[r][1] = v.y;
+          w[r][2] = v.z;
+          w[r][3] = v.w;
+        } else if constexpr (HD == 64u) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p);
+          w[r][0] = v.x;
+          w[r][1] = v.y;
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < HD / 32u; ++i) w[r][i] = *reinterpret_cast<const uint32_t*>(p + 4u * i);
+        }
+        const uint8_t* q = ks + (g + 8u * r) * (HD / 32u);
+        const uint32_t b0 = q[t * (HD / 4u) / 32u];
+        sc[r][0] = scale2(b0, b0);
+        if constexpr (HD == 96u) {
+          const uint32_t b1 = q[(t * 24u + 23u) / 32u];
+          sc[r][1] = scale2(b1, b1);
+        } else {
+          sc[r][1] = sc[r][0];
+        }
+      }
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (uint32_t c = 0; c < 4u; ++c) s[nt][hf][c] = 0.f;
+#pragma unroll
+      for (uint32_t i = 0; i < HD / 32u; ++i) {
+        uint32_t a[2][4];
+#pragma unroll
+        for (uint32_t r = 0; r < 2u; ++r) {
+          e2m1x8_to_f16x2(w[r][i], a[r]);
+#pragma unroll
+          for (uint32_t d = 0; d < 4u; ++d) {
+            // Dims 24 t + 8 i + 2 d of hd 96 pass a block's end inside the lane.
+            const uint32_t x = HD == 96u && t * 24u + 8u * i + 2u * d >= 32u * (t * 24u / 32u + 1u)
+                                   ? sc[r][1] : sc[r][0];
+            a[r][d] = mul2(a[r][d], x);
+          }
+        }
+#pragma unroll
+        for (uint32_t st = 0; st < 2u; ++st) {
+#pragma unroll
+          for (uint32_t nt = 0; nt < NT; ++nt) {
+            uint32_t b0, b1;
+            if constexpr (NT <= 2u) {
+              b0 = qf[nt][2u * i + st][0];
+              b1 = qf[nt][2u * i + st][1];
+            } else {
+              const uint2 b = *reinterpret_cast<const uint2*>(
+                  q_smem + ((nt * kSteps + 2u * i + st) * 32u + lane) * 2u);
+              b0 = b.x;
+              b1 = b.y;
+            }
+            mma(s[nt][hf], a[0][2u * st], a[1][2u * st], a[0][2u * st + 1u], a[1][2u * st + 1u],
+                b0, b1);
+          }
+        }
+      }
+    }
+    if (bad_a || bad_b) {
+      bad_page = true;
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c)
+          if (c < 4u ? bad_a : bad_b) s[nt][c / 4u][c & 3u] = 0.f;
+    }
+    // Scores to the exponent of two, masked.
+#pragma unroll
+    for (uint32_t nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (uint32_t c = 0; c < 8u; ++c) {
+        const uint32_t rr = c & 1u;
+        float x = s[nt][c / 4u][c & 3u] * factor[nt][rr];
+        if (capped) {
+          // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2x / cap)))
+          const float y = ex2(x * j.cap_in);
+          x = j.cap_out * (1.0f - __fdividef(2.0f, 1.0f + y));
+        }
+        const int32_t k = k0 + static_cast<int32_t>(16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g);
+        if (j.slopes != nullptr) x -= slope[nt][rr] * fabsf(static_cast<float>(pos[nt][rr] - k));
+        s[nt][c / 4u][c & 3u] = attn_sees(seen[nt][rr], k) ? x : -INFINITY;
+      }
+    }
+    // m moves where a score passes it by more than kLazy.
+    bool moves = false;
+    float top[NT][2];
+#pragma unroll
+    for (uint32_t nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (uint32_t c = 0; c < 2u; ++c) {
+        top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][c + 2u]), fmaxf(s[nt][1][c], s[nt][1][c + 2u]));
+        moves |= top[nt][c] > m[nt][c] + kLazy;
+      }
+    }
+    if (__any_sync(0xFFFFFFFFu, moves)) {
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (uint32_t c = 0; c < 2u; ++c) {
+          float x = top[nt][c];
+          x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
+          const float to = fmaxf(m[nt][c], x);
+          const float keep = to == -INFINITY ? 1.0f : ex2(m[nt][c] - to);
+          m[nt][c] = to;
+          l[nt][c] *= keep;
+#pragma unroll
+          for (uint32_t i = 0; i < kSteps; ++i) {
+            o[nt][i][c] *= keep;
+            o[nt][i][c + 2u] *= keep;
+          }
+        }
+      }
+    }
+    // P^T as the B operand: pairs of keys in a lane, rows across lanes.
+    uint32_t p[NT][2][2];
+#pragma unroll
+    for (uint32_t nt = 0; nt < NT; ++nt) {
+      const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
+      const float m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+      for (uint32_t hf = 0; hf < 2u; ++hf) {
+#pragma unroll
+        for (uint32_t r = 0; r < 2u; ++r) {
+          const float x = ex2(s[nt][hf][2u * r] - m0), y = ex2(s[nt][hf][2u * r + 1u] - m1);
+          l[nt][0] += x;
+          l[nt][1] += y;
+          p[nt][hf][r] = transpose8x8(half2_bits(__floats2half2_rn(x, y)));
+        }
+      }
+    }
+    if (bad_a || bad_b) {
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (uint32_t hf = 0; hf < 2u; ++hf)
+          if (hf == 0u ? bad_a : bad_b) p[nt][hf][0] = p[nt][hf][1] = 0u;
+    }
+    // O^T: m16 tile i holds dims D(i, g, 0) as its rows g and D(i, g, 1) as
+    // its rows g + 8, two dims of one byte.
+#pragma unroll
+    for (uint32_t hf = 0; hf < 2u; ++hf) {
+      const uint8_t* vc = tile + geo.v + hf * geo.code_half;
+      const uint8_t* vs = tile + geo.vs + hf * geo.scale_half;
+      constexpr uint32_t kWords = (HD + 63u) / 64u;  // words of codes a lane and key (the last half used at hd 96 and 32)
+      uint32_t w[4][kWords], sc[2][2];
+#pragma unroll
+      for (uint32_t r = 0; r < 4u; ++r) {  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+        const uint32_t key = 2u * t + (r & 1u) + 8u * (r >> 1);
+        const uint8_t* p8 = vc + key * (HD / 2u);
+        if constexpr (HD == 128u) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p8 + 8u * g);
+          w[r][0] = v.x;
+          w[r][1] = v.y;
+        } else if constexpr (HD == 96u) {
+          w[r][0] = *reinterpret_cast<const uint32_t*>(p8 + 4u * g);
+          w[r][1] = *reinterpret_cast<const uint16_t*>(p8 + 32u + 2u * g);
+        } else if constexpr (HD == 64u) {
+          w[r][0] = *reinterpret_cast<const uint32_t*>(p8 + 4u * g);
+        } else {
+          w[r][0] = *reinterpret_cast<const uint16_t*>(p8 + 2u * g);
+        }
+      }
+#pragma unroll
+      for (uint32_t r = 0; r < 2u; ++r) {
+        const uint8_t* q = vs + (2u * t + 8u * r) * (HD / 32u);
+        const uint32_t b = HD == 128u ? g >> 1 : HD == 32u ? 0u : g >> 2;
+        sc[r][0] = scale2(q[b], q[b + HD / 32u]);
+        sc[r][1] = HD == 96u ? scale2(q[2], q[2u + HD / 32u]) : sc[r][0];
+      }
+#pragma unroll
+      for (uint32_t x = 0; x < kWords; ++x) {
+        uint32_t lo[2][4], hi[2][4];  // of the key pairs (2t, 2t + 1) and 8 further
+#pragma unroll
+        for (uint32_t r = 0; r < 2u; ++r) {
+          const uint32_t a = w[2u * r][x], b = w[2u * r + 1u][x];
+          e2m1x8_to_f16x2((a & 0x0F0F0F0Fu) | ((b << 4) & 0xF0F0F0F0u), lo[r]);
+          e2m1x8_to_f16x2(((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u), hi[r]);
+        }
+#pragma unroll
+        for (uint32_t d = 0; d < 4u; ++d) {
+          const uint32_t i = 4u * x + d;
+          if (i < kSteps) {
+            const uint32_t which = HD == 96u && x == 1u ? 1u : 0u;
+            const uint32_t a0 = mul2(lo[0][d], sc[0][which]), a1 = mul2(hi[0][d], sc[0][which]);
+            const uint32_t a2 = mul2(lo[1][d], sc[1][which]), a3 = mul2(hi[1][d], sc[1][which]);
+#pragma unroll
+            for (uint32_t nt = 0; nt < NT; ++nt) {
+              mma(o[nt][i], a0, a1, a2, a3, p[nt][hf][0], p[nt][hf][1]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();  // all lanes have read the stage
+    --in_flight;
+    at = next(at + 1);
+    if (ahead < mine && ahead < base + 32) {
+      issue(ahead, stage);
+      ++in_flight;
+      ahead = next(ahead + 1);
+    }
+    if (++stage == kStages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+  if (!ok) {  // timed out: wait (bounded) for the copies in flight
+    while (in_flight-- > 0u) {
+      mbar_wait(full + stage, parity, error_flag);
+      if (++stage == kStages) {
+        stage = 0;
+        parity ^= 1u;
+      }
+    }
+  }
+  if (bad_page && lane == 0u) atomicOr(error_flag, kErrKvSlot);
+
+  // Join the warps: rows of (m, l, O) in shared memory over the rings.
+  __syncthreads();
+  constexpr uint32_t kLd = HD + 4u;
+  float* mine_o = reinterpret_cast<float*>(smem) + warp * kRows * kLd;
+#pragma unroll
+  for (uint32_t nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (uint32_t c = 0; c < 2u; ++c) {
+      float x = l[nt][c];
+      x += __shfl_xor_sync(0xFFFFFFFFu, x, 4);
+      x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
+      x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
+      float* to = mine_o + (8u * nt + 2u * t + c) * kLd;
+      if (g == 0u) {
+        to[HD] = m[nt][c];
+        to[HD + 1u] = x;
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < kSteps; ++i) {
+        uint32_t d;
+        if constexpr (HD == 128u) {
+          d = 16u * g + 2u * i;
+        } else if constexpr (HD == 32u) {
+          d = 4u * g + 2u * i;
+        } else {
+          d = i < 4u ? 8u * g + 2u * i : 64u + 4u * g + 2u * (i - 4u);
+        }
+        to[d] = o[nt][i][c];
+        to[d + 1u] = o[nt][i][c + 2u];
+      }
+    }
+  }
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(smem);
+  for (int32_t r = static_cast<int32_t>(warp); r < rows; r += static_cast<int32_t>(kWarps)) {
+    float top = -INFINITY;
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) top = fmaxf(top, all[(w * kRows + r) * kLd + HD]);
+    float part[kWarps], sum = 0.f;
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) {
+      const float mw = all[(w * kRows + r) * kLd + HD];
+      part[w] = mw == -INFINITY ? 0.f : ex2(mw - top);
+      // A row of NaNs alone has m = -inf and l = NaN.
+      const float lw = all[(w * kRows + r) * kLd + HD + 1u];
+      sum += mw == -INFINITY ? lw : lw * part[w];
+      if (mw == -INFINITY && lw != 0.f) part[w] = 1.f;
+    }
+    const uint64_t row = static_cast<uint64_t>(q0 + r / static_cast<int32_t>(j.group));
+    const uint32_t h = head * j.group + static_cast<uint32_t>(r) % j.group;
+    const uint64_t cell = (static_cast<uint64_t>(blockIdx.x) * j.total_q + row) * j.heads + h;
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+#pragma unroll
+    for (uint32_t b = 0; b < HD / 32u; ++b) {
+      float x = 0.f;
+#pragma unroll
+      for (uint32_t w = 0; w < kWarps; ++w) {
+        x += part[w] * all[(w * kRows + r) * kLd + 32u * b + lane];
+      }
+      if (whole) {
+        write_block(j, row, h, b, lane, x * inv, error_flag);
+      } else {
+        j.part_o[cell * HD + 32u * b + lane] = x;
+      }
+    }
+    if (!whole && lane == 0u) j.part_ml[cell] = make_float2(top, sum);
+  }
+}
+
+// Joins the chunks of a request's rows: a warp a row and head.
+__global__ void __launch_bounds__(128)
+    k_attn_join(const AttnJob j, uint32_t* __restrict__ error_flag) {
+  const uint32_t lane = threadIdx.x & 31u, hd = j.cache.hd;
+  const uint32_t r = (blockIdx.x * 4u + (threadIdx.x >> 5)) / j.heads;
+  const uint32_t h = (blockIdx.x * 4u + (threadIdx.x >> 5)) % j.heads;
+  int32_t q0, q_len, kv;
+  attn_request(j, blockIdx.y, &q0, &q_len, &kv);
+  if (static_cast<int32_t>(r) >= q_len) return;
+  const uint64_t row = static_cast<uint64_t>(q0) + r, unit = row * j.heads + h;
+  const uint32_t chunks = (static_cast<uint32_t>(kv) + j.chunk - 1u) / j.chunk;
+  if (chunks <= 1u) return;
+  const uint64_t stride = static_cast<uint64_t>(j.total_q) * j.heads;
+  float top = -INFINITY;
+  for (uint32_t c = lane; c < chunks; c += 32u) top = fmaxf(top, j.part_ml[c * stride + unit].x);
+#pragma unroll
+  for (uint32_t d = 16; d > 0; d /= 2u) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (uint32_t c = 0; c < chunks; ++c) {
+    const float2 ml = j.part_ml[c * stride + unit];
+    const float w = ml.x == -INFINITY ? (ml.y != 0.f ? 1.f : 0.f) : ex2(ml.x - top);
+    if (w == 0.f) continue;
+    sum += ml.y * w;
+    for (uint32_t b = 0; b < hd / 32u; ++b) {
+      x[b] += w * j.part_o[(c * stride + unit) * hd + 32u * b + lane];
+    }
+  }
+  const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+  for (uint32_t b = 0; b < hd / 32u; ++b) {
+    write_block(j, row, h, b, lane, x[b] * inv, error_flag);
+  }
+}
+
+template <uint32_t HD, uint32_t NT>
+cudaError_t launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stream) {
+  static std::atomic<uint64_t> set{0};  // devices whose limit is raised
+  if (((set.load(std::memory_order_relaxed) >> (job.device & 63u)) & 1u) == 0u || job.device > 63u) {
+    const cudaError_t st = cudaFuncSetAttribute(
+        k_attn_decode<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, NT>::kBytes);
+    if (st != cudaSuccess) return st;
+    set.fetch_or(uint64_t{1} << (job.device & 63u), std::memory_order_relaxed);
+  }
+  k_attn_decode<HD, NT><<<dim3(chunks, job.cache.kv_heads, job.seqs), kWarps * 32,
+                          Smem<HD, NT>::kBytes, stream>>>(job, err);
+  return cudaSuccess;
+}
+
+template <uint32_t HD>
+cudaError_t launch_rows(const AttnJob& job, uint32_t rows, uint32_t chunks, uint32_t* err,
+                        cudaStream_t stream) {
+  if (rows <= 8u) return launch<HD, 1>(job, chunks, err, stream);
+  if (rows <= 16u) return launch<HD, 2>(job, chunks, err, stream);
+  return launch<HD, 4>(job, chunks, err, stream);
+}
+
+}  // namespace
+
+uint32_t attn_decode_chunk(const AttnJob& job, uint64_t total_kv, int sm_count) {
+  // Enough chunks to fill the GPU about four times over with the requests'
+  // keys, of 256 keys at least and 128 chunks a request at most.
+  const uint64_t blocks = static_cast<uint64_t>(sm_count) * 16u;
+  uint64_t chunk = total_kv * job.cache.kv_heads / blocks;
+  const uint64_t least = (static_cast<uint64_t>(job.max_kv) + 127u) / 128u;
+  if (chunk < least) chunk = least;
+  if (chunk < 256u) chunk = 256u;
+  chunk = (chunk + kWarps * kTile - 1u) / (kWarps * kTile) * (kWarps * kTile);
+  return static_cast<uint32_t>(chunk < 0x40000000u ? chunk : 0x40000000u);
+}
+
+int launch_attn_decode(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream) {
+  const uint32_t rows = job.max_q * job.group;
+  const uint32_t chunks = job.max_kv == 0u ? 1u : (job.max_kv + job.chunk - 1u) / job.chunk;
+  cudaError_t st;
+  switch (job.cache.hd) {
+    case 32: st = launch_rows<32>(job, rows, chunks, error_flag, stream); break;
+    case 64: st = launch_rows<64>(job, rows, chunks, error_flag, stream); break;
+    case 96: st = launch_rows<96>(job, rows, chunks, error_flag, stream); break;
+    default: st = launch_rows<128>(job, rows, chunks, error_flag, stream); break;
+  }
+  if (st != cudaSuccess) return -1;
+  if (chunks == 1u) return 1;
+  k_attn_join<<<dim3((job.max_q * job.heads + 3u) / 4u, job.seqs), 128, 0, stream>>>(job,
+                                                                                  error_flag);
+  return 2;
+}
+
+}  // namespace hrb

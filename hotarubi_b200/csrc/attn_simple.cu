@@ -28,10 +28,13 @@ __global__ void __launch_bounds__(kThreads)
     if (static_cast<uint32_t>(j.q_start[mid]) <= row) lo = mid; else hi = mid;
   }
   while (lo + 1u < j.seqs && static_cast<uint32_t>(j.q_start[lo + 1u]) <= row) ++lo;
-  const int32_t first = j.q_start[lo], last = j.q_start[lo + 1u];
-  if (static_cast<int32_t>(row) < first || static_cast<int32_t>(row) >= last) return;
-  const int32_t kv = min(max(j.kv_len[lo], 0), static_cast<int32_t>(j.max_kv));
-  const int32_t i = j.kv_len[lo] - (last - first) + (static_cast<int32_t>(row) - first);
+  int32_t q0, q_len, kv;
+  if (!attn_request(j, lo, &q0, &q_len, &kv)) {
+    if (h == 0u && t == 0u) atomicOr(error_flag, kErrKvSlot);
+    return;
+  }
+  if (static_cast<int32_t>(row) < q0 || static_cast<int32_t>(row) >= q0 + q_len) return;
+  const int32_t i = kv - q_len + (static_cast<int32_t>(row) - q0);
   const Seen seen = attn_seen(j, i, kv, j.prefix != nullptr ? j.prefix[lo] : 0);
   const float slope = j.slopes != nullptr ? j.slopes[h] : 0.f;
   if (t < hd) {

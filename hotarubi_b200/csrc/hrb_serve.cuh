@@ -61,8 +61,31 @@ struct AttnJob {
   uint32_t vec_rule;
   uint32_t seqs, heads, group, total_q, max_q, max_kv, table_ld;
   uint32_t causal, window;
+  uint32_t device;
   float scale, softcap;
+  float cap_in, cap_out;  // 2 log2(e) / softcap, softcap * log2(e)
+  // Keys a block of the split kernels takes, and the chunks' results: rows
+  // of (m, l) and O, [chunk][total_q][heads] and the same by [hd].
+  uint32_t chunk;
+  float2* part_ml;
+  float* part_o;
 };
+
+// Rows [q0, q0 + q_len) and keys of request n, held to what the descriptor
+// says there are; false (and no rows) where the lists contradict it.
+__device__ __forceinline__ bool attn_request(const AttnJob& j, uint32_t n, int32_t* q0,
+                                             int32_t* q_len, int32_t* kv) {
+  *q0 = __ldg(j.q_start + n);
+  *q_len = __ldg(j.q_start + n + 1u) - *q0;
+  const int32_t len = __ldg(j.kv_len + n);
+  *kv = min(max(len, 0), static_cast<int32_t>(j.max_kv));
+  if (*q0 >= 0 && *q_len >= 0 && *q_len <= static_cast<int32_t>(j.max_q) &&
+      *q0 <= static_cast<int32_t>(j.total_q) - *q_len && len <= static_cast<int32_t>(j.max_kv)) {
+    return true;
+  }
+  *q_len = 0;
+  return false;
+}
 
 // The keys row position i of request n may see: [lo, hi) and [0, pre), both
 // held to the request's keys.
@@ -93,6 +116,12 @@ __device__ __forceinline__ uint16_t attn_bf16(float x) {
   asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(x));
   return r;
 }
+
+// Requests of at most kDecodeRows rows of q times query heads a key/value
+// head.  Returns the launches, or -1.
+constexpr uint32_t kDecodeRows = 32u;
+uint32_t attn_decode_chunk(const AttnJob& job, uint64_t total_kv, int sm_count);
+int launch_attn_decode(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
 
 void launch_attn_simple(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
 

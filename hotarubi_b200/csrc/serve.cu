@@ -124,8 +124,9 @@ hrb_status check_attn(hrb_ctx* ctx, const hrb_attn_desc* d) {
   return HRB_OK;
 }
 
-hrb::AttnJob attn_job(const hrb_attn_desc* d) {
+hrb::AttnJob attn_job(const hrb_ctx* ctx, const hrb_attn_desc* d) {
   hrb::AttnJob j{};
+  j.device = static_cast<uint32_t>(hrb::ctx_device(ctx));
   j.cache = hrb::make_kv_cache(d->cache);
   j.q = static_cast<const uint16_t*>(d->q);
   j.ldq = d->ldq;
@@ -151,7 +152,24 @@ hrb::AttnJob attn_job(const hrb_attn_desc* d) {
   j.window = d->window;
   j.scale = d->scale;
   j.softcap = d->softcap;
+  j.cap_in = d->softcap != 0.f ? 2.885390081777927f / d->softcap : 0.f;
+  j.cap_out = d->softcap * 1.4426950408889634f;
   return j;
+}
+
+uint64_t up256(uint64_t x) { return (x + 255u) / 256u * 256u; }
+
+// Fills in how the call is split and where its scratch lies from `base`
+// (null: to learn the size).  Returns the scratch bytes.
+uint64_t attn_plan(const hrb_ctx* ctx, const hrb_attn_desc* d, hrb::AttnJob* j, uint8_t* base) {
+  const uint64_t total_kv = d->total_kv != 0u ? d->total_kv : uint64_t{d->seqs} * d->max_kv;
+  if (j->max_q * j->group > hrb::kDecodeRows) return 0;
+  j->chunk = hrb::attn_decode_chunk(*j, total_kv, hrb::ctx_sm_count(ctx));
+  if (j->max_kv <= j->chunk) return 0;
+  const uint64_t cells = (uint64_t{j->max_kv} + j->chunk - 1u) / j->chunk * j->total_q * j->heads;
+  j->part_ml = reinterpret_cast<float2*>(base);
+  j->part_o = reinterpret_cast<float*>(base + up256(cells * 8u));
+  return up256(cells * 8u) + cells * j->cache.hd * 4u;
 }
 
 }  // namespace
@@ -306,18 +324,42 @@ hrb_status hrb_kv_read(hrb_ctx* ctx, const hrb_kv_cache* cache, const int32_t* s
 hrb_status hrb_attention_workspace(hrb_ctx* ctx, const hrb_attn_desc* d, uint64_t* bytes) {
   if (ctx == nullptr || bytes == nullptr) return HRB_EINVAL;
   *bytes = 0;
-  return check_attn(ctx, d);
+  const hrb_status st = check_attn(ctx, d);
+  if (st != HRB_OK || d->total_q == 0u) return st;
+  hrb::AttnJob j = attn_job(ctx, d);
+  *bytes = attn_plan(ctx, d, &j, nullptr);
+  return HRB_OK;
 }
 
 hrb_status hrb_attention(hrb_ctx* ctx, const hrb_attn_desc* d, void* stream) {
   if (ctx == nullptr) return HRB_EINVAL;
-  const hrb_status st = check_attn(ctx, d);
+  hrb_status st = check_attn(ctx, d);
   if (st != HRB_OK) return st;
   if (d->total_q == 0u) return HRB_OK;
   if (cudaSetDevice(hrb::ctx_device(ctx)) != cudaSuccess) {
     return refuse(ctx, HRB_ECUDA, "cudaSetDevice");
   }
-  hrb::launch_attn_simple(attn_job(d), hrb::ctx_error_word(ctx), hrb::ctx_stream(ctx, stream));
+  hrb::AttnJob j = attn_job(ctx, d);
+  const uint64_t need = attn_plan(ctx, d, &j, nullptr);
+  if (need != 0u) {
+    void* base = d->workspace;
+    if (base == nullptr) {
+      st = hrb::ctx_serve_scratch(ctx, need, &base);
+      if (st != HRB_OK) return st;
+    } else if (d->workspace_bytes < need) {
+      return refuse(ctx, HRB_EINVAL, "workspace of %llu bytes, %llu needed",
+                    static_cast<unsigned long long>(d->workspace_bytes),
+                    static_cast<unsigned long long>(need));
+    }
+    attn_plan(ctx, d, &j, static_cast<uint8_t*>(base));
+  }
+  cudaStream_t s = hrb::ctx_stream(ctx, stream);
+  if (j.max_q * j.group <= hrb::kDecodeRows) {
+    const int n = hrb::launch_attn_decode(j, hrb::ctx_error_word(ctx), s);
+    if (n < 0) return refuse(ctx, HRB_ECUDA, "k_attn_decode: %s", cudaGetErrorString(cudaGetLastError()));
+    return launched(ctx, static_cast<uint32_t>(n), "hrb_attention");
+  }
+  hrb::launch_attn_simple(j, hrb::ctx_error_word(ctx), s);
   return launched(ctx, 1, "hrb_attention");
 }
 

@@ -321,7 +321,7 @@ class Step:
                              self.values, self.scale, **kw)
 
     def run(self, hrb, prefix=None, slopes=None, oq=False, oquant=capi.QUANT_VEC, out=True, stream=0,
-            total_kv=0, workspace=False, sync=True, table=None, **kw):
+            total_kv=0, workspace=False, sync=True, table=None, max_q=None, max_kv=None, **kw):
         w = self.heads * self.hd
         self.dq, self.dd = self.q.cuda(), dev(self.cache.data)
         lists = [dev(np.asarray(x, np.int32)) for x in
@@ -334,8 +334,10 @@ class Step:
         d = capi.attn_desc(
             capi.kv_cache(self.dd, self.pages, self.page, self.kvh, self.hd,
                           page_stride=self.cache.stride), len(self.lens), self.heads, q=self.dq,
-            ldq=self.ldq, q_start=lists[0], total_q=self.rows, max_q=max(q for q, _ in self.lens),
-            kv_len=lists[1], max_kv=max(max(kv, 0) for _, kv in self.lens), total_kv=total_kv,
+            ldq=self.ldq, q_start=lists[0], total_q=self.rows,
+            max_q=max(q for q, _ in self.lens) if max_q is None else max_q, kv_len=lists[1],
+            max_kv=max(max(kv, 0) for _, kv in self.lens) if max_kv is None else max_kv,
+            total_kv=total_kv,
             table=lists[2], table_ld=self.ld, scale=self.scale, prefix=pre, slopes=slo,
             out=o if out else None, ldo=w + 8, oq=codes if oq else None,
             oscale=scales if oq else None, ldoq=w + 32 if oq else 0, oquant=oquant, **kw)
@@ -344,6 +346,7 @@ class Step:
             self.ws = torch.full((max(n, 256) + 256,), 0xFF, dtype=torch.uint8, device="cuda")
             d.workspace, d.workspace_bytes = self.ws.data_ptr(), n
         self.keep = (lists, pre, slo)
+        self.out, self.codes, self.scales = o[:, :w], codes, scales
         ready()
         hrb.attention(d, stream=stream)
         if sync:
@@ -352,7 +355,6 @@ class Step:
         if workspace:
             assert (self.ws[max(n, 256):] == 0xFF).all()
         assert not out or (o[:, w:] == 5.0).all()
-        self.out, self.codes, self.scales = o[:, :w], codes, scales
         return o[:, :w].double().cpu().numpy().reshape(self.rows, self.heads, self.hd)
 
 
@@ -432,11 +434,41 @@ def test_attention_rows_that_see_nothing_are_zero(hrb, lens):
     assert empty.any() and not got[empty].any()
 
 
-def test_attention_negative_and_long_lengths_are_held(hrb):
+@pytest.mark.parametrize("q", [1, 90])
+def test_attention_a_negative_length_is_no_keys(hrb, q):
     rng = np.random.default_rng(4)
-    s = Step(rng, [(1, 30), (1, 0), (1, 50)], 4, 2, 64, 16)
-    s.lens = [(1, 30), (1, -3), (1, 50)]
+    s = Step(rng, [(q, 130), (q, 0), (q, 150)], 4, 2, 64, 16)
+    s.lens = [(q, 130), (q, -3), (q, 150)]
     close(s.run(hrb), *s.want())
+
+
+@pytest.mark.parametrize("what", ["kv", "rows", "order"])
+@pytest.mark.parametrize("q", [1, 90])
+def test_attention_leaves_out_requests_past_its_bounds(hrb, what, q):
+    rng = np.random.default_rng(5)
+    s = Step(rng, [(q, 130), (q, 120), (q, 150)], 4, 2, 64, 16)
+    want, mass = s.want()
+    if what == "kv":
+        s.lens[1] = (q, 1 << 20)
+        kw = dict(max_kv=150)
+    elif what == "rows":
+        s.start[3] += 5
+        kw = dict(max_q=q)
+    else:
+        s.start[1] = -4
+        kw = {}
+    with pytest.raises(capi.HrbError) as e:
+        s.run(hrb, **kw)
+    assert e.value.status == capi.HRB_EDATA
+    torch.cuda.synchronize()
+    out = {"kv": [1], "rows": [2], "order": [0, 1]}[what]
+    got = s.out.double().cpu().numpy().reshape(s.rows, s.heads, s.hd)
+    for n in range(3):
+        a, b = n * q, (n + 1) * q
+        if n in out:
+            assert (got[a:b] == 5.0).all()
+        else:
+            close(got[a:b], want[a:b], mass[a:b])
 
 
 @pytest.mark.parametrize("lens", [[(1, 3000), (1, 2049), (1, 5)], [(5, 4100)], [(140, 2500)]])
@@ -525,17 +557,8 @@ def test_attention_reports_a_page_outside_the_cache(hrb, lens):
         s.run(hrb, table=table)
     assert e.value.status == capi.HRB_EDATA
     torch.cuda.synchronize()
-    got = s.run(hrb, table=table, sync=False)
-    torch.cuda.synchronize()
-    with pytest.raises(capi.HrbError):
-        hrb.sync()
-    torch.cuda.synchronize()
-    del got
-    want, mass = s.want()
-    w = s.heads * s.hd
-    # The rows were written all the same: read them again from the device.
-    close(s.out.double().cpu().numpy().reshape(s.rows, s.heads, s.hd), want, mass)
-    assert s.out.shape == (s.rows, w)
+    # The rows are written all the same.
+    close(s.out.double().cpu().numpy().reshape(s.rows, s.heads, s.hd), *s.want())
 
 
 def test_attention_cache_beyond_32_bit_offsets(hrb):
