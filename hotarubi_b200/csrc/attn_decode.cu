@@ -90,9 +90,14 @@ __device__ __forceinline__ TileGeom tile_geom(uint32_t page) {
   return g;
 }
 
-// Two scale bytes as FP16 powers of two, `lo` in the low half.
+// Two scale bytes as FP16 powers of two, `lo` in the low half.  Bytes
+// outside the cache's range (stale keys) become its ends after the
+// conversion, which takes two fewer instructions than before it.
 __device__ __forceinline__ uint32_t scale2(uint32_t lo, uint32_t hi) {
-  return half2_bits(__floats2half2_rn(kv_scale(lo), kv_scale(hi)));
+  const __half2 h = __floats2half2_rn(__uint_as_float(lo << 23), __uint_as_float(hi << 23));
+  const __half2 most = __half2half2(__ushort_as_half(0x7000));   // 2^13
+  const __half2 least = __half2half2(__ushort_as_half(0x0002));  // 2^-23
+  return half2_bits(__hmax2(__hmin2(h, most), least));
 }
 
 // FP32 value of dim 32 b + lane of one output row and head, to BF16 and to
@@ -153,11 +158,6 @@ __global__ void __launch_bounds__(kWarps * 32)
   // The keys that the rows see, and the tiles of this warp among them.
   const int32_t pre = j.prefix != nullptr ? __ldg(j.prefix + n) : 0;
   const Seen first = attn_seen(j, kv - q_len, kv, pre), last = attn_seen(j, kv - 1, kv, pre);
-  const int32_t tiles = (c1 - c0 + static_cast<int32_t>(kTile) - 1) / static_cast<int32_t>(kTile);
-  auto tile_seen = [&](int32_t i) {
-    const int32_t a = c0 + i * static_cast<int32_t>(kTile), b = a + static_cast<int32_t>(kTile);
-    return (b > first.lo && a < last.hi) || a < first.pre;
-  };
 
   const TileGeom geo = tile_geom<HD>(j.cache.page);
   const int32_t* table = j.table + static_cast<uint64_t>(n) * j.table_ld;
@@ -283,15 +283,20 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
       for (uint32_t c = 0; c < 4u; ++c) o[nt][i][c] = 0.f;
 
-  // The warp's tiles: number x is tile warp + x kWarps of the chunk.
-  const int32_t mine = (tiles - static_cast<int32_t>(warp) + static_cast<int32_t>(kWarps) - 1) /
-                       static_cast<int32_t>(kWarps);
-  auto next = [&](int32_t x) {  // the next number from x on whose tile is seen
-    while (x < mine && !tile_seen(static_cast<int32_t>(warp) + x * static_cast<int32_t>(kWarps))) ++x;
-    return x;
+  // The warp's tiles: number x is tile warp + x kWarps of the chunk, those
+  // below `gap` or from `resume` to `mine` hold keys that a row sees (the
+  // prefix, and the window or all).
+  auto numbers_to = [&](int32_t k) {  // numbers whose tiles start before key k
+    const int32_t tiles = (min(max(k, c0), c1) - c0 + static_cast<int32_t>(kTile) - 1) /
+                          static_cast<int32_t>(kTile);
+    return (tiles - static_cast<int32_t>(warp) + static_cast<int32_t>(kWarps) - 1) /
+           static_cast<int32_t>(kWarps);
   };
-  load_pages(0);
+  const int32_t gap = numbers_to(first.pre), mine = max(gap, numbers_to(last.hi));
+  const int32_t resume = max(gap, min(mine, numbers_to(first.lo + 1 - static_cast<int32_t>(kTile))));
+  auto next = [&](int32_t x) { return x >= gap && x < resume ? resume : x; };
   int32_t ahead = next(0);  // next to issue
+  load_pages(ahead);
   int32_t at = ahead;       // next to use
   uint32_t in_flight = 0;
   // Pages of the tile in use are read again from lane registers: keep the
@@ -408,22 +413,41 @@ __global__ void __launch_bounds__(kWarps * 32)
         for (uint32_t c = 0; c < 8u; ++c)
           if (c < 4u ? bad_a : bad_b) s[nt][c / 4u][c & 3u] = 0.f;
     }
-    // Scores to the exponent of two, masked.
+    // Scores to the exponent of two.  Tiles that all rows see whole (all but
+    // a request's last for single tokens) skip the masks.
+    const int32_t k1 = k0 + static_cast<int32_t>(kTile);
+    const bool clear = (k0 >= last.lo && k1 <= first.hi) || k1 <= first.pre;
 #pragma unroll
-    for (uint32_t nt = 0; nt < NT; ++nt) {
+    for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (uint32_t c = 0; c < 8u; ++c) {
-        const uint32_t rr = c & 1u;
-        float x = s[nt][c / 4u][c & 3u] * factor[nt][rr];
-        if (capped) {
-          // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2x / cap)))
-          const float y = ex2(x * j.cap_in);
-          x = j.cap_out * (1.0f - __fdividef(2.0f, 1.0f + y));
+      for (uint32_t c = 0; c < 8u; ++c) s[nt][c / 4u][c & 3u] *= factor[nt][c & 1u];
+    if (capped) {
+      // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2x / cap)))
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) {
+          const float y = ex2(s[nt][c / 4u][c & 3u] * j.cap_in);
+          s[nt][c / 4u][c & 3u] = j.cap_out * (1.0f - __fdividef(2.0f, 1.0f + y));
         }
-        const int32_t k = k0 + static_cast<int32_t>(16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g);
-        if (j.slopes != nullptr) x -= slope[nt][rr] * fabsf(static_cast<float>(pos[nt][rr] - k));
-        s[nt][c / 4u][c & 3u] = attn_sees(seen[nt][rr], k) ? x : -INFINITY;
-      }
+    }
+    if (j.slopes != nullptr) {
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) {
+          const int32_t k = k0 + static_cast<int32_t>(16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g);
+          s[nt][c / 4u][c & 3u] -= slope[nt][c & 1u] * fabsf(static_cast<float>(pos[nt][c & 1u] - k));
+        }
+    }
+    if (!clear) {
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) {
+          const int32_t k = k0 + static_cast<int32_t>(16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g);
+          if (!attn_sees(seen[nt][c & 1u], k)) s[nt][c / 4u][c & 3u] = -INFINITY;
+        }
     }
     // m moves where a score passes it by more than kLazy.
     bool moves = false;
@@ -630,12 +654,16 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-// Joins the chunks of a request's rows: a warp a row and head.
-__global__ void __launch_bounds__(128)
+// Joins the chunks of a request's rows: a block a row and head, its warps
+// summing every kJoinWarps-th chunk (many chunks have many loads in flight;
+// their order does not depend on anything but their number).
+constexpr uint32_t kJoinWarps = 8;
+
+__global__ void __launch_bounds__(kJoinWarps * 32)
     k_attn_join(const AttnJob j, uint32_t* __restrict__ error_flag) {
-  const uint32_t lane = threadIdx.x & 31u, hd = j.cache.hd;
-  const uint32_t r = (blockIdx.x * 4u + (threadIdx.x >> 5)) / j.heads;
-  const uint32_t h = (blockIdx.x * 4u + (threadIdx.x >> 5)) % j.heads;
+  __shared__ float part[kJoinWarps][128], sums[kJoinWarps];
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, hd = j.cache.hd;
+  const uint32_t r = blockIdx.x / j.heads, h = blockIdx.x % j.heads;
   int32_t q0, q_len, kv;
   attn_request(j, blockIdx.y, &q0, &q_len, &kv);
   if (static_cast<int32_t>(r) >= q_len) return;
@@ -648,19 +676,29 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
   for (uint32_t d = 16; d > 0; d /= 2u) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
   float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t c = 0; c < chunks; ++c) {
+#pragma unroll 4
+  for (uint32_t c = warp; c < chunks; c += kJoinWarps) {
     const float2 ml = j.part_ml[c * stride + unit];
+    const float* o = j.part_o + (c * stride + unit) * hd + lane;
     const float w = ml.x == -INFINITY ? (ml.y != 0.f ? 1.f : 0.f) : ex2(ml.x - top);
-    if (w == 0.f) continue;
     sum += ml.y * w;
-    for (uint32_t b = 0; b < hd / 32u; ++b) {
-      x[b] += w * j.part_o[(c * stride + unit) * hd + 32u * b + lane];
+#pragma unroll
+    for (uint32_t b = 0; b < 4u; ++b) {
+      if (b < hd / 32u) x[b] += w * o[32u * b];
     }
   }
-  const float inv = sum != 0.f ? 1.0f / sum : 0.f;
-  for (uint32_t b = 0; b < hd / 32u; ++b) {
-    write_block(j, row, h, b, lane, x[b] * inv, error_flag);
+#pragma unroll
+  for (uint32_t b = 0; b < 4u; ++b) part[warp][32u * b + lane] = x[b];
+  if (lane == 0u) sums[warp] = sum;
+  __syncthreads();
+  if (warp >= hd / 32u) return;
+  float y = 0.f, all = 0.f;
+#pragma unroll
+  for (uint32_t w = 0; w < kJoinWarps; ++w) {
+    y += part[w][32u * warp + lane];
+    all += sums[w];
   }
+  write_block(j, row, h, warp, lane, y * (all != 0.f ? 1.0f / all : 0.f), error_flag);
 }
 
 template <uint32_t HD, uint32_t NT>
@@ -711,8 +749,8 @@ int launch_attn_decode(const AttnJob& job, uint32_t* error_flag, cudaStream_t st
   }
   if (st != cudaSuccess) return -1;
   if (chunks == 1u) return 1;
-  k_attn_join<<<dim3((job.max_q * job.heads + 3u) / 4u, job.seqs), 128, 0, stream>>>(job,
-                                                                                  error_flag);
+  k_attn_join<<<dim3(job.max_q * job.heads, job.seqs), kJoinWarps * 32, 0, stream>>>(job,
+                                                                                   error_flag);
   return 2;
 }
 
