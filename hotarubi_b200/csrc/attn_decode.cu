@@ -28,8 +28,7 @@
 #include <atomic>
 #include <cstdint>
 
-#include "hrb_quant.cuh"
-#include "hrb_serve.cuh"
+#include "hrb_attn.cuh"
 #include "sm100.cuh"
 
 namespace hrb {
@@ -40,23 +39,6 @@ using namespace sm100;
 constexpr uint32_t kTile = 32;   // keys a stage
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kStages = 3;
-constexpr float kLazy = 8.0f;    // log2 of the most a weight may pass 1 before m moves
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t half2_bits(__half2 h) {
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  return half2_bits(__hmul2(*reinterpret_cast<const __half2*>(&a),
-                            *reinterpret_cast<const __half2*>(&b)));
-}
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
@@ -88,33 +70,6 @@ __device__ __forceinline__ TileGeom tile_geom(uint32_t page) {
   g.code_half = page == 16u ? 16u * (HD + HD / 16u) : 16u * (HD / 2u);
   g.scale_half = page == 16u ? 16u * (HD + HD / 16u) : 16u * (HD / 32u);
   return g;
-}
-
-// Two scale bytes as FP16 powers of two, `lo` in the low half.  Bytes
-// outside the cache's range (stale keys) become its ends after the
-// conversion, which takes two fewer instructions than before it.
-__device__ __forceinline__ uint32_t scale2(uint32_t lo, uint32_t hi) {
-  const __half2 h = __floats2half2_rn(__uint_as_float(lo << 23), __uint_as_float(hi << 23));
-  const __half2 most = __half2half2(__ushort_as_half(0x7000));   // 2^13
-  const __half2 least = __half2half2(__ushort_as_half(0x0002));  // 2^-23
-  return half2_bits(__hmax2(__hmin2(h, most), least));
-}
-
-// FP32 value of dim 32 b + lane of one output row and head, to BF16 and to
-// the MXINT8 copy.
-__device__ __forceinline__ void write_block(const AttnJob& j, uint64_t row, uint32_t head,
-                                            uint32_t b, uint32_t lane, float x,
-                                            uint32_t* error_flag) {
-  const uint32_t col = head * j.cache.hd + 32u * b + lane;
-  if (j.out != nullptr) j.out[row * j.ldo + col] = attn_bf16(x);
-  if (j.oq == nullptr) return;
-  const uint32_t bits = __float_as_uint(x), mag = bits & 0x7FFFFFFFu;
-  const uint32_t key = __reduce_max_sync(0xFFFFFFFFu, j.vec_rule ? mag >> 23 : mag);
-  uint32_t scale;
-  const int32_t code = mxint8_code(bits, key, j.vec_rule != 0, scale);
-  j.oq[row * j.ldoq + col] = static_cast<int8_t>(code);
-  if (lane == 0u) j.oscale[row * (j.ldoq / 32u) + col / 32u] = static_cast<uint8_t>(scale);
-  if (mag >= 0x7F800000u && !j.vec_rule) atomicOr(error_flag, 1u);
 }
 
 template <uint32_t HD, uint32_t NT>
@@ -725,6 +680,11 @@ cudaError_t launch_rows(const AttnJob& job, uint32_t rows, uint32_t chunks, uint
 
 }  // namespace
 
+void launch_attn_join(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream) {
+  k_attn_join<<<dim3(job.max_q * job.heads, job.seqs), kJoinWarps * 32, 0, stream>>>(job,
+                                                                                   error_flag);
+}
+
 uint32_t attn_decode_chunk(const AttnJob& job, uint64_t total_kv, int sm_count) {
   // Enough chunks to fill the GPU about four times over with the requests'
   // keys, of 256 keys at least and 128 chunks a request at most.
@@ -749,8 +709,7 @@ int launch_attn_decode(const AttnJob& job, uint32_t* error_flag, cudaStream_t st
   }
   if (st != cudaSuccess) return -1;
   if (chunks == 1u) return 1;
-  k_attn_join<<<dim3(job.max_q * job.heads, job.seqs), kJoinWarps * 32, 0, stream>>>(job,
-                                                                                   error_flag);
+  launch_attn_join(job, error_flag, stream);
   return 2;
 }
 

@@ -1,0 +1,551 @@
+// hrb_attention for many rows a request (prompts and chunks of them), on the
+// tensor cores with TMEM accumulators.
+//
+// k_kv_expand decodes the requests' keys once into FP16 operand tiles of 128
+// keys in scratch memory: K [128 keys][hd] and V^T [hd][128 keys], rows of
+// 128 bytes in the 128-byte swizzle, exactly as the tensor cores read them
+// from shared memory, so that one bulk copy brings a tile.  (Every block of
+// rows would otherwise decode the same keys again: a prompt of 8191 tokens
+// with four query heads a key/value head reads each key 128 times.)
+//
+// k_attn_prompt: a block takes 256 rows (query token x query head of one
+// key/value head), two halves of 128 that alternate on the tensor cores:
+//   warps 0-3, 4-7  softmax of half A, B: a thread a row.  S = Q K^T from
+//                   TMEM, running maximum and sum, P = 2^(s - m) as FP16
+//                   back to TMEM over S, O scaled there when m moves
+//   warp 8          issues S_A, S_B and O_A += P_A V, O_B += P_B V
+//                   (tcgen05.mma kind::f16, P from TMEM)
+//   warp 9          bulk copies of K and V^T tiles, two stages each
+// While one half's softmax runs, the other half's products do.  m moves only
+// when a row's scores pass it by 2^8, so O is rarely scaled.
+//
+// Few blocks (a short chunk over a long cache) split the keys; k_attn_join
+// (attn_decode.cu) joins the rows' (m, l, O).
+#include <cuda_fp16.h>
+
+#include <atomic>
+#include <cstdint>
+
+#include "hrb_attn.cuh"
+#include "sm100.cuh"
+
+namespace hrb {
+namespace {
+
+using namespace sm100;
+
+constexpr uint32_t kKeys = 128;      // keys a tile
+constexpr uint32_t kHalf = 128;      // rows a half
+constexpr uint32_t kThreads = 384;    // three warpgroups: warps 10 and 11 only give up registers
+constexpr uint32_t kRowB = 128;      // bytes of a swizzled row
+
+// Bytes of a tile's parts: K in chunks of 64 dims, V^T in chunks of 64 keys.
+__host__ __device__ constexpr uint32_t k_bytes(uint32_t hd) { return (hd + 63u) / 64u * kKeys * kRowB; }
+__host__ __device__ constexpr uint32_t v_bytes(uint32_t hd) { return 2u * hd * kRowB; }
+__host__ __device__ constexpr uint32_t tile_bytes(uint32_t hd) { return k_bytes(hd) + v_bytes(hd); }
+
+// First tile in scratch of request n (a whole warp; the same in all lanes).
+__device__ __forceinline__ uint32_t first_tile(const AttnJob& j, uint32_t n) {
+  uint32_t sum = 0;
+  for (uint32_t i = threadIdx.x & 31u; i < n; i += 32u) {
+    int32_t q0, q_len, kv;
+    if (attn_request(j, i, &q0, &q_len, &kv) && q_len > 0) {
+      sum += (static_cast<uint32_t>(kv) + kKeys - 1u) / kKeys;
+    }
+  }
+  return __reduce_add_sync(0xFFFFFFFFu, sum);
+}
+
+// A block: one tile of one request and key/value head.
+template <uint32_t HD>
+__global__ void __launch_bounds__(256)
+    k_kv_expand(const AttnJob j, uint32_t* __restrict__ error_flag) {
+  constexpr uint32_t kLd = HD / 2u + 4u;  // padded row of codes in shared memory
+  __shared__ __align__(16) uint8_t codes[2][kKeys * kLd];
+  __shared__ uint8_t scales[2][kKeys * (HD / 32u)];
+  const uint32_t n = blockIdx.z, head = blockIdx.y, k0 = blockIdx.x * kKeys;
+  int32_t q0, q_len, kv;
+  if (!attn_request(j, n, &q0, &q_len, &kv)) {
+    if (head == 0u && blockIdx.x == 0u && threadIdx.x == 0u) atomicOr(error_flag, kErrKvSlot);
+    return;
+  }
+  if (q_len == 0 || k0 >= static_cast<uint32_t>(kv)) return;
+  const uint32_t tile = first_tile(j, n) + blockIdx.x;
+  if (tile >= j.tiles_cap) {  // more keys than total_kv said
+    if (threadIdx.x == 0u) atomicOr(error_flag, kErrKvSlot);
+    return;
+  }
+  const uint32_t keys = min(kKeys, static_cast<uint32_t>(kv) - k0);
+  // The tile's codes, a word a thread at a time; keys past the end and pages
+  // outside the cache are zeros.
+  bool bad = false;
+  const int32_t* table = j.table + static_cast<uint64_t>(n) * j.table_ld;
+  for (uint32_t i = threadIdx.x; i < kKeys * (HD / 8u); i += 256u) {
+    const uint32_t key = i / (HD / 8u), w = i % (HD / 8u);
+    uint32_t x[2] = {0u, 0u};
+    if (key < keys) {
+      const uint32_t page = static_cast<uint32_t>(__ldg(table + ((k0 + key) >> j.cache.page_log2)));
+      if (page < j.cache.pages) {
+        const uint32_t in = (k0 + key) & (j.cache.page - 1u);
+        const uint8_t* rec = kv_record(j.cache, page, head) + in * (HD / 2u) + 4u * w;
+        x[0] = *reinterpret_cast<const uint32_t*>(rec);
+        x[1] = *reinterpret_cast<const uint32_t*>(rec + kv_vcodes(j.cache));
+      } else {
+        bad = true;
+      }
+    }
+    *reinterpret_cast<uint32_t*>(&codes[0][key * kLd + 4u * w]) = x[0];
+    *reinterpret_cast<uint32_t*>(&codes[1][key * kLd + 4u * w]) = x[1];
+  }
+  for (uint32_t i = threadIdx.x; i < kKeys * (HD / 32u); i += 256u) {
+    const uint32_t key = i / (HD / 32u), b = i % (HD / 32u);
+    uint32_t x[2] = {127u, 127u};
+    if (key < keys) {
+      const uint32_t page = static_cast<uint32_t>(__ldg(table + ((k0 + key) >> j.cache.page_log2)));
+      if (page < j.cache.pages) {
+        const uint32_t in = (k0 + key) & (j.cache.page - 1u);
+        const uint8_t* rec = kv_record(j.cache, page, head) + kv_kscales(j.cache) + in * (HD / 32u) + b;
+        x[0] = rec[0];
+        x[1] = rec[kv_vcodes(j.cache)];
+      }
+    }
+    scales[0][i] = static_cast<uint8_t>(x[0]);
+    scales[1][i] = static_cast<uint8_t>(x[1]);
+  }
+  if (bad) atomicOr(error_flag, kErrKvSlot);
+  __syncthreads();
+  uint8_t* out = j.tiles + (static_cast<uint64_t>(head) * j.tiles_cap + tile) * tile_bytes(HD);
+  // K: 16 bytes (8 dims of a key) a step, neighbours in a row.
+  for (uint32_t i = threadIdx.x; i < kKeys * (HD / 8u); i += 256u) {
+    const uint32_t key = i / (HD / 8u), u = i % (HD / 8u);
+    uint32_t h[4];
+    e2m1x8_to_f16x2(*reinterpret_cast<const uint32_t*>(&codes[0][key * kLd + 4u * u]), h);
+    const uint32_t b = scales[0][key * (HD / 32u) + u / 4u];
+    const uint32_t sc = scale2(b, b);
+#pragma unroll
+    for (uint32_t d = 0; d < 4u; ++d) h[d] = mul2(h[d], sc);
+    *reinterpret_cast<uint4*>(out + (u / 8u) * (kKeys * kRowB) + key * kRowB +
+                              (((u & 7u) ^ (key & 7u)) * 16u)) = make_uint4(h[0], h[1], h[2], h[3]);
+  }
+  // V^T: a thread turns 8 keys x 8 dims; 8 neighbours fill a row.
+  out += k_bytes(HD);
+  for (uint32_t i = threadIdx.x; i < (kKeys / 8u) * (HD / 8u); i += 256u) {
+    const uint32_t kg = i % (kKeys / 8u), dg = i / (kKeys / 8u);
+    uint32_t h[8][4];  // dim, key pair
+#pragma unroll
+    for (uint32_t r = 0; r < 4u; ++r) {
+      const uint32_t key = 8u * kg + 2u * r;
+      const uint32_t a = *reinterpret_cast<const uint32_t*>(&codes[1][key * kLd + 4u * dg]);
+      const uint32_t b = *reinterpret_cast<const uint32_t*>(&codes[1][(key + 1u) * kLd + 4u * dg]);
+      const uint32_t sc = scale2(scales[1][key * (HD / 32u) + dg / 4u],
+                                 scales[1][(key + 1u) * (HD / 32u) + dg / 4u]);
+      uint32_t lo[4], hi[4];
+      e2m1x8_to_f16x2((a & 0x0F0F0F0Fu) | ((b << 4) & 0xF0F0F0F0u), lo);
+      e2m1x8_to_f16x2(((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u), hi);
+#pragma unroll
+      for (uint32_t d = 0; d < 4u; ++d) {
+        h[2u * d][r] = mul2(lo[d], sc);
+        h[2u * d + 1u][r] = mul2(hi[d], sc);
+      }
+    }
+#pragma unroll
+    for (uint32_t d = 0; d < 8u; ++d) {
+      const uint32_t row = 8u * dg + d;
+      *reinterpret_cast<uint4*>(out + (kg / 8u) * (HD * kRowB) + row * kRowB +
+                                (((kg & 7u) ^ (row & 7u)) * 16u)) =
+          make_uint4(h[d][0], h[d][1], h[d][2], h[d][3]);
+    }
+  }
+}
+
+template <uint32_t HD>
+struct Smem {
+  static constexpr uint32_t kQ = 2u * k_bytes(HD);
+  static constexpr uint32_t kK = kQ;                         // two K stages
+  static constexpr uint32_t kV = kK + 2u * k_bytes(HD);      // two V^T stages
+  static constexpr uint32_t kBars = kV + 2u * v_bytes(HD);
+  static constexpr uint32_t kUsed = kBars + 128u;
+  // Over half an SM's shared memory: one block an SM, for its 512 columns of
+  // TMEM.
+  static constexpr uint32_t kBytes = (kUsed > 120u * 1024u ? kUsed : 120u * 1024u) + 1024u;
+};
+
+// Instruction descriptor of kind::f16 with FP16 A and B, FP32 D, K-major
+// operands (the fields of idesc_bf16 with formats 0).
+constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) {
+  return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+template <uint32_t HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_attn_prompt(const AttnJob j, uint32_t* __restrict__ error_flag) {
+  using S = Smem<HD>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5,
+           *v_empty = bars + 7, *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 13;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+
+  const uint32_t head = blockIdx.x % j.cache.kv_heads, n = blockIdx.z;
+  const uint32_t chunk = blockIdx.x / j.cache.kv_heads;
+  int32_t q0, q_len, kv;
+  if (!attn_request(j, n, &q0, &q_len, &kv)) return;  // k_kv_expand reports it
+  const int32_t rows = q_len * static_cast<int32_t>(j.group);
+  // The last rows see the most keys: they start first.
+  const int32_t q_tiles = (rows + 2 * static_cast<int32_t>(kHalf) - 1) / (2 * static_cast<int32_t>(kHalf));
+  if (static_cast<int32_t>(blockIdx.y) >= q_tiles) return;
+  const int32_t r0 = (q_tiles - 1 - static_cast<int32_t>(blockIdx.y)) * 2 * static_cast<int32_t>(kHalf);
+  const int32_t r1 = min(rows, r0 + 2 * static_cast<int32_t>(kHalf));
+  const int32_t c0 = static_cast<int32_t>(chunk * j.chunk);
+  const bool whole = kv <= static_cast<int32_t>(j.chunk);
+  if (c0 >= kv && c0 > 0) return;
+  const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
+  const uint32_t base = first_tile(j, n);
+  if (base + (static_cast<uint32_t>(kv) + kKeys - 1u) / kKeys > j.tiles_cap) return;  // reported too
+  const uint32_t halves = r1 - r0 > static_cast<int32_t>(kHalf) ? 2u : 1u;
+
+  // The tiles that some row of the block sees: numbers 0 .. gap - 1 and
+  // resume .. of the chunk's, `count` in all.
+  const int32_t pre = j.prefix != nullptr ? __ldg(j.prefix + n) : 0;
+  const int32_t group = static_cast<int32_t>(j.group);
+  const Seen first = attn_seen(j, kv - q_len + r0 / group, kv, pre);
+  const Seen last = attn_seen(j, kv - q_len + (r1 - 1) / group, kv, pre);
+  auto tiles_to = [&](int32_t k) {
+    return (min(max(k, c0), c1) - c0 + static_cast<int32_t>(kKeys) - 1) / static_cast<int32_t>(kKeys);
+  };
+  const int32_t gap = tiles_to(first.pre), end = max(gap, tiles_to(last.hi));
+  const int32_t resume = max(gap, min(end, tiles_to(first.lo + 1 - static_cast<int32_t>(kKeys))));
+  const int32_t count = gap + end - resume;
+  auto tile_at = [&](int32_t it) { return it < gap ? it : it - gap + resume; };
+
+  if (threadIdx.x == 0u) {
+    mbar_init(q_full, 256);
+    for (uint32_t i = 0; i < 2u; ++i) {
+      mbar_init(k_full + i, 1);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, 1);
+      mbar_init(v_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, kHalf);
+      mbar_init(o_full + i, 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 8u) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // 384 threads x 168 registers at launch = 256 x 224 + 128 x 56: a softmax
+  // thread holds a row's 128 scores.
+  if (warp >= 8u) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  if (warp == 9u) {
+    if (lane == 0u) {
+      const uint8_t* src = j.tiles + (static_cast<uint64_t>(head) * j.tiles_cap + base +
+                                      static_cast<uint32_t>(c0) / kKeys) * tile_bytes(HD);
+      int32_t it = 0;
+      for (; it < count; ++it) {
+        const uint32_t st = static_cast<uint32_t>(it) & 1u, ph = (static_cast<uint32_t>(it) >> 1) & 1u;
+        const uint8_t* tile = src + static_cast<uint64_t>(tile_at(it)) * tile_bytes(HD);
+        if (it >= 2 && !mbar_wait(k_empty + st, ph ^ 1u, error_flag)) break;
+        mbar_arrive_expect_tx(k_full + st, k_bytes(HD));
+        bulk_g2s(smem + S::kK + st * k_bytes(HD), tile, k_bytes(HD), k_full + st);
+        if (it >= 2 && !mbar_wait(v_empty + st, ph ^ 1u, error_flag)) break;
+        mbar_arrive_expect_tx(v_full + st, v_bytes(HD));
+        bulk_g2s(smem + S::kV + st * v_bytes(HD), tile + k_bytes(HD), v_bytes(HD), v_full + st);
+      }
+      // Nothing of this block's may still be arriving when it ends.
+      for (int32_t w = max(it - 2, 0); w < min(it + 1, count); ++w) {
+        const uint32_t st = static_cast<uint32_t>(w) & 1u, ph = (static_cast<uint32_t>(w) >> 1) & 1u;
+        if (w < it && !mbar_wait(v_full + st, ph, error_flag)) break;
+        if (w == it && !mbar_wait(k_full + st, ph, error_flag, 1000u)) break;
+      }
+    }
+  } else if (warp == 8u) {
+    if (lane == 0u && count > 0) {
+      const uint32_t q_at = smem_addr(smem), k_at = smem_addr(smem + S::kK), v_at = smem_addr(smem + S::kV);
+      auto scores = [&](uint32_t h, uint32_t st) {
+#pragma unroll
+        for (uint32_t k = 0; k < HD / 16u; ++k) {
+          const uint32_t off = (k >> 2) * (kKeys * kRowB) + 32u * (k & 3u);
+          mma_bf16(tmem + 128u * h, desc_sw128(q_at + h * k_bytes(HD) + off),
+                   desc_sw128(k_at + st * k_bytes(HD) + off), idesc_f16(128, 128), k != 0u);
+        }
+        mma_commit(s_full + h);
+      };
+      bool ok = mbar_wait(q_full, 0, error_flag) && mbar_wait(k_full, 0, error_flag);
+      if (ok) {
+        tc_fence_after();
+        for (uint32_t h = 0; h < halves; ++h) scores(h, 0);
+        mma_commit(k_empty);
+      }
+      for (int32_t it = 0; it < count && ok; ++it) {
+        const uint32_t st = static_cast<uint32_t>(it) & 1u, ph = (static_cast<uint32_t>(it) >> 1) & 1u;
+        const bool more = it + 1 < count;
+        for (uint32_t h = 0; h < halves && ok; ++h) {
+          ok = mbar_wait(p_full + h, static_cast<uint32_t>(it) & 1u, error_flag) &&
+               (h != 0u || mbar_wait(v_full + st, ph, error_flag));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (uint32_t k = 0; k < kKeys / 16u; ++k) {
+            mma_bf16_ts(tmem + 256u + 128u * h, tmem + 128u * h + 8u * k,
+                        desc_sw128(v_at + st * v_bytes(HD) + (k >> 2) * (HD * kRowB) + 32u * (k & 3u)),
+                        idesc_f16(128, HD), it != 0 || k != 0u);
+          }
+          if (more) {
+            const uint32_t nst = static_cast<uint32_t>(it + 1) & 1u;
+            ok = h != 0u || mbar_wait(k_full + nst, (static_cast<uint32_t>(it + 1) >> 1) & 1u, error_flag);
+            if (!ok) break;
+            scores(h, nst);
+          } else {
+            mma_commit(o_full + h);
+          }
+        }
+        mma_commit(v_empty + st);
+        if (more) mma_commit(k_empty + (static_cast<uint32_t>(it + 1) & 1u));
+      }
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const uint32_t h = warp >> 2;
+    const uint32_t in_half = (warp & 3u) * 32u + lane;
+    const int32_t r = r0 + static_cast<int32_t>(h * kHalf + in_half);
+    const bool mine = r < r1;
+    const uint64_t row = static_cast<uint64_t>(q0 + (mine ? r : r0) / group);
+    const uint32_t qh = head * j.group + static_cast<uint32_t>((mine ? r : r0) % group);
+    float factor;
+    {
+      // The row of Q as FP16, scaled so that its largest value is in
+      // [2^13, 2^14) and signed so that the scores' factor is not negative.
+      const uint16_t* src = j.q + row * j.ldq + static_cast<uint64_t>(qh) * HD;
+      uint32_t top = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < HD / 8u; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (uint32_t d = 0; d < 4u; ++d) top = max(top, max(w[d] & 0x7FFFu, (w[d] >> 16) & 0x7FFFu));
+      }
+      const int32_t e = min(max(static_cast<int32_t>(top >> 7), 27), 254) - 127;
+      float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
+      if (!mine) up = 0.f;
+      if (j.scale < 0.f) up = -up;
+      factor = fabsf(j.scale) * __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23) *
+               (j.softcap != 0.f ? 1.0f : kLog2e);
+      factor = fmaxf(factor, 1.2e-38f);  // times a masked score's -inf is no NaN
+      uint8_t* dst = smem + h * k_bytes(HD) + in_half * kRowB;
+#pragma unroll
+      for (uint32_t i = 0; i < HD / 8u; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t o[4];
+#pragma unroll
+        for (uint32_t d = 0; d < 4u; ++d) {
+          o[d] = mine ? half2_bits(__floats2half2_rn(__uint_as_float(w[d] << 16) * up,
+                                                     __uint_as_float(w[d] & 0xFFFF0000u) * up))
+                      : 0u;
+        }
+        *reinterpret_cast<uint4*>(dst + (i >> 3) * (kKeys * kRowB) + (((i & 7u) ^ (in_half & 7u)) * 16u)) =
+            make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(q_full);
+    }
+    const int32_t pos = kv - q_len + (mine ? r : r0) / group;
+    Seen seen = attn_seen(j, pos, kv, pre);
+    if (!mine) seen.lo = seen.hi = seen.pre = 0;
+    const float slope = j.slopes != nullptr ? __ldg(j.slopes + qh) * kLog2e : 0.f;
+    const uint32_t lanes = ((warp & 3u) * 32u) << 16;
+    const uint32_t t_s = tmem + lanes + 128u * h, t_o = tmem + lanes + 256u + 128u * h;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    if (h < halves) {
+      for (int32_t it = 0; it < count; ++it) {
+        ok = mbar_wait(s_full + h, static_cast<uint32_t>(it) & 1u, error_flag);
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (uint32_t c = 0; c < 4u; ++c) tmem_ld32(t_s + 32u * c, s[c]);
+        tmem_wait_ld();
+        const int32_t k0 = c0 + tile_at(it) * static_cast<int32_t>(kKeys);
+        const int32_t k1 = k0 + static_cast<int32_t>(kKeys);
+        auto at = [&](uint32_t c, uint32_t i) -> float { return __uint_as_float(s[c][i]); };
+        float scale = factor;
+        if (j.softcap != 0.f || j.slopes != nullptr) {
+          scale = 1.0f;
+#pragma unroll
+          for (uint32_t c = 0; c < 4u; ++c)
+#pragma unroll
+            for (uint32_t i = 0; i < 32u; ++i) {
+              float x = at(c, i) * factor;
+              if (j.softcap != 0.f) {
+                x = j.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(x * j.cap_in)));
+              }
+              x -= slope * fabsf(static_cast<float>(pos - k0 - static_cast<int32_t>(32u * c + i)));
+              s[c][i] = __float_as_uint(x);
+            }
+        }
+        const bool clear = (k0 >= seen.lo && k1 <= seen.hi) || k1 <= seen.pre;
+        if (!__all_sync(0xFFFFFFFFu, clear)) {
+          // Keys [a, b) and [0, c) of the tile.
+          const int32_t a = seen.lo - k0, b = seen.hi - k0, cc = seen.pre - k0;
+#pragma unroll
+          for (uint32_t c = 0; c < 4u; ++c)
+#pragma unroll
+            for (uint32_t i = 0; i < 32u; ++i) {
+              const int32_t k = static_cast<int32_t>(32u * c + i);
+              if (!((k >= a && k < b) || k < cc)) s[c][i] = 0xFF800000u;
+            }
+        }
+        float top[4];
+#pragma unroll
+        for (uint32_t c = 0; c < 4u; ++c) {
+          top[c] = at(c, 0);
+#pragma unroll
+          for (uint32_t i = 1; i < 32u; ++i) top[c] = fmaxf(top[c], at(c, i));
+        }
+        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+        const bool moves = high > m + kLazy;
+        if (__any_sync(0xFFFFFFFFu, moves)) {
+          const float keep = moves ? ex2(m - high) : 1.0f;
+          if (moves) m = high;
+          l *= keep;
+          if (it != 0) {
+#pragma unroll
+            for (uint32_t c = 0; c < HD / 32u; ++c) {
+              uint32_t o[32];
+              tmem_ld32(t_o + 32u * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (uint32_t i = 0; i < 32u; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+              tmem_st32(t_o + 32u * c, o);
+            }
+          }
+        }
+        const float shift = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t c = 0; c < 2u; ++c) {
+          uint32_t p[32];
+#pragma unroll
+          for (uint32_t i = 0; i < 32u; ++i) {
+            const float x = ex2(fmaf(at(2u * c + i / 16u, 2u * (i % 16u)), scale, shift));
+            const float y = ex2(fmaf(at(2u * c + i / 16u, 2u * (i % 16u) + 1u), scale, shift));
+            sum[i & 1u] += x;
+            sum[2u + (i & 1u)] += y;
+            p[i] = half2_bits(__floats2half2_rn(x, y));
+          }
+          tmem_st32(t_s + 32u * c, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_full + h);
+      }
+      if (count > 0 && ok) ok = mbar_wait(o_full + h, 0, error_flag);
+      if (__all_sync(0xFFFFFFFFu, ok)) {
+        tc_fence_after();
+        const float inv = l != 0.f ? 1.0f / l : 0.f;
+        const uint64_t cell = (static_cast<uint64_t>(chunk) * j.total_q + row) * j.heads + qh;
+#pragma unroll
+        for (uint32_t c = 0; c < HD / 32u; ++c) {
+          uint32_t o[32];
+          __syncwarp();
+          if (count > 0) {
+            tmem_ld32(t_o + 32u * c, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 32u; ++i) o[i] = 0;
+          }
+          if (mine) {
+            float x[32];
+#pragma unroll
+            for (uint32_t i = 0; i < 32u; ++i) x[i] = __uint_as_float(o[i]) * (whole ? inv : 1.0f);
+            if (whole) {
+              write_row_block(j, row, qh, c, x, error_flag);
+            } else {
+              float4* to = reinterpret_cast<float4*>(j.part_o + cell * HD + 32u * c);
+#pragma unroll
+              for (uint32_t i = 0; i < 8u; ++i) {
+                to[i] = make_float4(x[4u * i], x[4u * i + 1u], x[4u * i + 2u], x[4u * i + 3u]);
+              }
+              if (c == 0u) j.part_ml[cell] = make_float2(m, l);
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8u) tmem_dealloc(tmem, 512);
+}
+
+template <uint32_t HD>
+int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stream) {
+  static std::atomic<uint64_t> set{0};  // devices whose limit is raised
+  if (((set.load(std::memory_order_relaxed) >> (job.device & 63u)) & 1u) == 0u || job.device > 63u) {
+    if (cudaFuncSetAttribute(k_attn_prompt<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Smem<HD>::kBytes) != cudaSuccess) {
+      return -1;
+    }
+    set.fetch_or(uint64_t{1} << (job.device & 63u), std::memory_order_relaxed);
+  }
+  const uint32_t key_tiles = (job.max_kv + kKeys - 1u) / kKeys;
+  const uint32_t q_tiles = (job.max_q * job.group + 2u * kHalf - 1u) / (2u * kHalf);
+  int n = 1;
+  if (key_tiles != 0u) {
+    k_kv_expand<HD><<<dim3(key_tiles, job.cache.kv_heads, job.seqs), 256, 0, stream>>>(job, err);
+    ++n;
+  }
+  k_attn_prompt<HD><<<dim3(chunks * job.cache.kv_heads, q_tiles, job.seqs), kThreads,
+                      Smem<HD>::kBytes, stream>>>(job, err);
+  return n;
+}
+
+}  // namespace
+
+uint64_t attn_prompt_tiles(const AttnJob& job, uint64_t total_kv) {
+  return total_kv / kKeys + job.seqs;
+}
+uint64_t attn_prompt_tile_bytes(const AttnJob& job) { return tile_bytes(job.cache.hd); }
+
+uint32_t attn_prompt_chunk(const AttnJob& job, int sm_count) {
+  // Blocks for every SM where the rows alone do not give them: chunks of 512
+  // keys at least.
+  const uint64_t rows = static_cast<uint64_t>(job.total_q) * job.group;
+  const uint64_t blocks = (rows + 2u * kHalf - 1u) / (2u * kHalf) * job.cache.kv_heads;
+  const uint64_t split = static_cast<uint64_t>(sm_count) / blocks;
+  uint64_t chunk = job.max_kv;
+  if (split > 1u) chunk = (job.max_kv + split - 1u) / split;
+  if (chunk < 512u) chunk = 512u;
+  return static_cast<uint32_t>((chunk + kKeys - 1u) / kKeys * kKeys);
+}
+
+int launch_attn_prompt(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream) {
+  const uint32_t chunks = job.max_kv == 0u ? 1u : (job.max_kv + job.chunk - 1u) / job.chunk;
+  int n;
+  switch (job.cache.hd) {
+    case 32: n = launch<32>(job, chunks, error_flag, stream); break;
+    case 64: n = launch<64>(job, chunks, error_flag, stream); break;
+    case 96: n = launch<96>(job, chunks, error_flag, stream); break;
+    default: n = launch<128>(job, chunks, error_flag, stream); break;
+  }
+  if (n < 0 || chunks == 1u) return n;
+  launch_attn_join(job, error_flag, stream);
+  return n + 1;
+}
+
+}  // namespace hrb

@@ -1,0 +1,100 @@
+// What the attention kernels (attn_decode.cu, attn_prompt.cu) share: the
+// exponential, FP16 operand arithmetic, the outputs.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "hrb_quant.cuh"
+#include "hrb_serve.cuh"
+
+namespace hrb {
+
+constexpr float kLazy = 8.0f;    // log2 of the most a weight may pass 1 before m moves
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) {
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  return half2_bits(__hmul2(*reinterpret_cast<const __half2*>(&a),
+                            *reinterpret_cast<const __half2*>(&b)));
+}
+
+// Two scale bytes as FP16 powers of two, `lo` in the low half.  Bytes
+// outside the cache's range (stale keys) become its ends after the
+// conversion, which takes two fewer instructions than before it.
+__device__ __forceinline__ uint32_t scale2(uint32_t lo, uint32_t hi) {
+  const __half2 h = __floats2half2_rn(__uint_as_float(lo << 23), __uint_as_float(hi << 23));
+  const __half2 most = __half2half2(__ushort_as_half(0x7000));   // 2^13
+  const __half2 least = __half2half2(__ushort_as_half(0x0002));  // 2^-23
+  return half2_bits(__hmax2(__hmin2(h, most), least));
+}
+
+// FP32 value of dim 32 b + lane of one output row and head, to BF16 and to
+// the MXINT8 copy.
+__device__ __forceinline__ void write_block(const AttnJob& j, uint64_t row, uint32_t head,
+                                            uint32_t b, uint32_t lane, float x,
+                                            uint32_t* error_flag) {
+  const uint32_t col = head * j.cache.hd + 32u * b + lane;
+  if (j.out != nullptr) j.out[row * j.ldo + col] = attn_bf16(x);
+  if (j.oq == nullptr) return;
+  const uint32_t bits = __float_as_uint(x), mag = bits & 0x7FFFFFFFu;
+  const uint32_t key = __reduce_max_sync(0xFFFFFFFFu, j.vec_rule ? mag >> 23 : mag);
+  uint32_t scale;
+  const int32_t code = mxint8_code(bits, key, j.vec_rule != 0, scale);
+  j.oq[row * j.ldoq + col] = static_cast<int8_t>(code);
+  if (lane == 0u) j.oscale[row * (j.ldoq / 32u) + col / 32u] = static_cast<uint8_t>(scale);
+  if (mag >= 0x7F800000u && !j.vec_rule) atomicOr(error_flag, 1u);
+}
+
+// The same for 32 dims (block b) in one thread.
+__device__ __forceinline__ void write_row_block(const AttnJob& j, uint64_t row, uint32_t head,
+                                                uint32_t b, const float (&x)[32],
+                                                uint32_t* error_flag) {
+  const uint64_t col = static_cast<uint64_t>(head) * j.cache.hd + 32u * b;
+  if (j.out != nullptr) {
+    uint4* to = reinterpret_cast<uint4*>(j.out + row * j.ldo + col);
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (uint32_t d = 0; d < 4u; ++d) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;"
+            : "=r"(w[d])
+            : "f"(x[8u * i + 2u * d + 1u]), "f"(x[8u * i + 2u * d]));
+      }
+      to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  if (j.oq == nullptr) return;
+  uint32_t top = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < 32u; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  const uint32_t key = j.vec_rule ? top >> 23 : top;
+  uint32_t scale = 0, w[8];
+#pragma unroll
+  for (uint32_t i = 0; i < 8u; ++i) {
+    w[i] = 0;
+#pragma unroll
+    for (uint32_t d = 0; d < 4u; ++d) {
+      const int32_t code = mxint8_code(__float_as_uint(x[4u * i + d]), key, j.vec_rule != 0, scale);
+      w[i] |= (static_cast<uint32_t>(code) & 0xFFu) << (8u * d);
+    }
+  }
+  uint4* to = reinterpret_cast<uint4*>(j.oq + row * j.ldoq + col);
+  to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  j.oscale[row * (j.ldoq / 32u) + col / 32u] = static_cast<uint8_t>(scale);
+  if (top >= 0x7F800000u && !j.vec_rule) atomicOr(error_flag, 1u);
+}
+
+}  // namespace hrb

@@ -69,6 +69,9 @@ struct AttnJob {
   uint32_t chunk;
   float2* part_ml;
   float* part_o;
+  // The prompt kernel's decoded keys: [kv_heads][tiles_cap] tiles.
+  uint8_t* tiles;
+  uint32_t tiles_cap;
 };
 
 // Rows [q0, q0 + q_len) and keys of request n, held to what the descriptor
@@ -123,6 +126,13 @@ constexpr uint32_t kDecodeRows = 32u;
 uint32_t attn_decode_chunk(const AttnJob& job, uint64_t total_kv, int sm_count);
 int launch_attn_decode(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
 
-void launch_attn_simple(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
+// Joins the chunks' results of all rows.
+void launch_attn_join(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
+
+// Any number of rows.  Scratch for attn_prompt_tiles tiles a key/value head.
+uint64_t attn_prompt_tiles(const AttnJob& job, uint64_t total_kv);
+uint64_t attn_prompt_tile_bytes(const AttnJob& job);
+uint32_t attn_prompt_chunk(const AttnJob& job, int sm_count);
+int launch_attn_prompt(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
 
 }  // namespace hrb

@@ -70,7 +70,7 @@ hrb_status check_attn(hrb_ctx* ctx, const hrb_attn_desc* d) {
   }
   if (d->seqs > 65535u) return refuse(ctx, HRB_EINVAL, "%u requests (at most 65535)", d->seqs);
   if (d->total_q > 0x7FFFFFFFu || d->max_q > d->total_q || d->max_kv > 0x7FFFFFFFu ||
-      uint64_t{d->max_q} * (d->heads / d->cache.kv_heads) > 0x7FFFFFFFull) {
+      uint64_t{d->max_q} * (d->heads / d->cache.kv_heads) > 256ull * 65535u) {
     return refuse(ctx, HRB_EINVAL, "%u rows, at most %u a request, %u keys", d->total_q, d->max_q,
                   d->max_kv);
   }
@@ -163,13 +163,22 @@ uint64_t up256(uint64_t x) { return (x + 255u) / 256u * 256u; }
 // (null: to learn the size).  Returns the scratch bytes.
 uint64_t attn_plan(const hrb_ctx* ctx, const hrb_attn_desc* d, hrb::AttnJob* j, uint8_t* base) {
   const uint64_t total_kv = d->total_kv != 0u ? d->total_kv : uint64_t{d->seqs} * d->max_kv;
-  if (j->max_q * j->group > hrb::kDecodeRows) return 0;
-  j->chunk = hrb::attn_decode_chunk(*j, total_kv, hrb::ctx_sm_count(ctx));
-  if (j->max_kv <= j->chunk) return 0;
+  uint64_t at = 0;
+  if (j->max_q * j->group <= hrb::kDecodeRows) {
+    j->chunk = hrb::attn_decode_chunk(*j, total_kv, hrb::ctx_sm_count(ctx));
+  } else {
+    const uint64_t tiles = hrb::attn_prompt_tiles(*j, total_kv);
+    j->tiles_cap = static_cast<uint32_t>(tiles < 0xFFFFFFFFull ? tiles : 0xFFFFFFFFull);
+    j->tiles = base;
+    at = up256(tiles * j->cache.kv_heads * hrb::attn_prompt_tile_bytes(*j));
+    j->chunk = hrb::attn_prompt_chunk(*j, hrb::ctx_sm_count(ctx));
+  }
+  if (j->max_kv <= j->chunk) return at;
   const uint64_t cells = (uint64_t{j->max_kv} + j->chunk - 1u) / j->chunk * j->total_q * j->heads;
-  j->part_ml = reinterpret_cast<float2*>(base);
-  j->part_o = reinterpret_cast<float*>(base + up256(cells * 8u));
-  return up256(cells * 8u) + cells * j->cache.hd * 4u;
+  j->part_ml = reinterpret_cast<float2*>(base + at);
+  at += up256(cells * 8u);
+  j->part_o = reinterpret_cast<float*>(base + at);
+  return at + cells * j->cache.hd * 4u;
 }
 
 }  // namespace
@@ -354,13 +363,11 @@ hrb_status hrb_attention(hrb_ctx* ctx, const hrb_attn_desc* d, void* stream) {
     attn_plan(ctx, d, &j, static_cast<uint8_t*>(base));
   }
   cudaStream_t s = hrb::ctx_stream(ctx, stream);
-  if (j.max_q * j.group <= hrb::kDecodeRows) {
-    const int n = hrb::launch_attn_decode(j, hrb::ctx_error_word(ctx), s);
-    if (n < 0) return refuse(ctx, HRB_ECUDA, "k_attn_decode: %s", cudaGetErrorString(cudaGetLastError()));
-    return launched(ctx, static_cast<uint32_t>(n), "hrb_attention");
-  }
-  hrb::launch_attn_simple(j, hrb::ctx_error_word(ctx), s);
-  return launched(ctx, 1, "hrb_attention");
+  const int n = j.max_q * j.group <= hrb::kDecodeRows
+                    ? hrb::launch_attn_decode(j, hrb::ctx_error_word(ctx), s)
+                    : hrb::launch_attn_prompt(j, hrb::ctx_error_word(ctx), s);
+  if (n < 0) return refuse(ctx, HRB_ECUDA, "hrb_attention: %s", cudaGetErrorString(cudaGetLastError()));
+  return launched(ctx, static_cast<uint32_t>(n), "hrb_attention");
 }
 
 }  // extern "C"
