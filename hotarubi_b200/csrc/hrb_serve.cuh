@@ -45,7 +45,7 @@ struct QkvJob {
 void launch_qkv_append(const QkvJob& job, bool bf16, bool vec, uint32_t* error_flag, int sm_count,
                        cudaStream_t stream);
 void launch_kv_read(const KvCache& cache, const int32_t* slots, uint32_t tokens, uint32_t dtype,
-                    void* k, void* v, uint32_t* error_flag, int sm_count, cudaStream_t stream);
+                    void* k, void* v, uint32_t* error_flag, cudaStream_t stream);
 
 struct AttnJob {
   KvCache cache;

@@ -5,13 +5,14 @@
 //   (y_a, y_b) = (y_a c - y_b s, y_b c + y_a s)      pairs of the first rot dims
 //   q -> BF16;  k, v -> 32-dim blocks, e = floor(log2 max) - 2, E2M1(y / 2^e)
 //
-// k_qkv: a lane holds four consecutive dims of a head, so a head is hd / 4
-// lanes (a warp holds 1, 2 or 4 heads at a time) and a 32-dim block 8 lanes:
-// the mean takes log2(hd / 4) shuffles, the block maximum three.  A half-split pair's
-// other dim is at the same place of the lane rot / 8 away, one shuffle each.
-// A warp takes one token and up to kSteps times its heads: the token's
-// position, slot and cos/sin pairs are read once for them, and all their
-// rows are loaded before the first is used.
+// k_qkv: a head is hd / 8 lanes (12 of 16 at hd = 96), a warp holds 8, 4 or
+// 2 heads at a time; a lane has the four dims 4l .. 4l + 3 and the four hd / 2
+// further, so that the pairs of a whole half-split rotation meet in a lane
+// and need no shuffle (those of a partial one take two a dim).  A warp takes
+// a token and a run of its heads, in steps that are all of q, of k or of v:
+// the token's position, slot and cos/sin pairs are read once for them, and
+// four steps' rows are in flight together.  With eight dims a lane the sums
+// and maxima over a head cost half the shuffles of four.
 //
 // Memory bound: each input is read once (FP32: 4 bytes a value, BF16: 2),
 // and per token heads * hd BF16 values and kv_heads * (hd + hd / 16) bytes
@@ -21,86 +22,151 @@
 
 #include <cstdint>
 
-#include "hrb_serve.cuh"
+#include "hrb_attn.cuh"
+#include "hrb_kernels.cuh"
 
 namespace hrb {
 namespace {
 
 constexpr uint32_t kWarps = 4;
-constexpr uint32_t kSteps = 4;  // heads a lane holds at once
+constexpr uint32_t kAhead = 4;  // steps whose rows are in flight
 
 __device__ __forceinline__ float bf16_bits(uint32_t bits) { return __uint_as_float(bits << 16); }
 
-// Four consecutive values of a row.
+// Four consecutive values of a row, as they are (BF16: two words).
 template <bool BF16, bool VEC>
-__device__ __forceinline__ float4 load4(const void* base, uint64_t at) {
+__device__ __forceinline__ uint4 load4(const void* base, uint64_t at) {
   if constexpr (BF16) {
     const uint16_t* p = static_cast<const uint16_t*>(base) + at;
     if constexpr (VEC) {
       const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-      return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u),
-                         __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
+      return make_uint4(v.x, v.y, 0, 0);
     } else {
-      return make_float4(bf16_bits(__ldg(p)), bf16_bits(__ldg(p + 1)), bf16_bits(__ldg(p + 2)),
-                         bf16_bits(__ldg(p + 3)));
+      return make_uint4(__ldg(p) | (static_cast<uint32_t>(__ldg(p + 1)) << 16),
+                        __ldg(p + 2) | (static_cast<uint32_t>(__ldg(p + 3)) << 16), 0, 0);
     }
   } else {
-    const float* p = static_cast<const float*>(base) + at;
+    const uint32_t* p = static_cast<const uint32_t*>(base) + at;
     if constexpr (VEC) {
-      return __ldg(reinterpret_cast<const float4*>(p));
+      return __ldg(reinterpret_cast<const uint4*>(p));
     } else {
-      return make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+      return make_uint4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
     }
   }
 }
+template <bool BF16>
+__device__ __forceinline__ void values4(const uint4& v, float* y) {
+  if constexpr (BF16) {
+    y[0] = bf16_bits(v.x);
+    y[1] = __uint_as_float(v.x & 0xFFFF0000u);
+    y[2] = bf16_bits(v.y);
+    y[3] = __uint_as_float(v.y & 0xFFFF0000u);
+  } else {
+    y[0] = __uint_as_float(v.x);
+    y[1] = __uint_as_float(v.y);
+    y[2] = __uint_as_float(v.z);
+    y[3] = __uint_as_float(v.w);
+  }
+}
+
+template <uint32_t W>
+struct Which {
+  static constexpr uint32_t value = W;
+};
+
+// Where a warp's run of steps lies: q, k and v steps of a token in order.
+struct Steps {
+  uint32_t q, k, all;  // steps of q, of q and k, of all three
+  uint32_t run;        // a warp's
+  uint32_t runs;       // a token's
+};
+
+// Pairs of FP32 in a 64-bit register: one instruction for both, each rounded
+// as the single ones are.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 
 template <uint32_t HD, bool BF16, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32)
-    k_qkv(const QkvJob j, uint32_t chunks, uint32_t steps, uint32_t* __restrict__ error_flag) {
-  constexpr uint32_t kLanes = HD / 4u;                        // lanes a head (24 at hd 96)
-  constexpr uint32_t kSpan = HD == 96u ? 32u : kLanes;        // lanes set apart for a head
-  constexpr uint32_t kHeads = 32u / kSpan;                    // heads a warp holds
+__global__ void __launch_bounds__(kWarps * 32, BF16 ? 8 : 6)
+    k_qkv(const QkvJob j, const Steps st, uint32_t* __restrict__ error_flag) {
+  constexpr uint32_t kLanes = HD / 8u;                  // lanes a head
+  constexpr uint32_t kSpan = HD == 96u ? 16u : kLanes;  // lanes set apart for one
+  constexpr uint32_t kHeads = 32u / kSpan;              // heads a step
   const uint32_t lane = threadIdx.x & 31u, sub = lane / kSpan, l = lane % kSpan;
   const bool on = l < kLanes;
-  const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (unit >= static_cast<uint64_t>(j.tokens) * chunks) return;
-  const uint32_t t = static_cast<uint32_t>(unit / chunks);
-  const uint32_t h0 = static_cast<uint32_t>(unit % chunks) * steps * kHeads + sub;
-  const uint32_t qk = j.heads + j.cache.kv_heads, all = qk + j.cache.kv_heads;
-  // All rows of this warp, in flight together.
-  float4 x[kSteps];
-#pragma unroll
-  for (uint32_t u = 0; u < kSteps; ++u) {
-    const uint32_t h = h0 + u * kHeads;
-    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (u < steps && h < all && on) {
-      const uint32_t which = h < j.heads ? 0u : h < qk ? 1u : 2u;
-      const uint32_t hh = which == 0u ? h : which == 1u ? h - j.heads : h - qk;
-      x[u] = load4<BF16, VEC>(j.x[which], t * j.ld[which] + hh * HD + 4u * l);
-    }
-  }
-  // The lane's four (cos, sin): half-split dims d use pair d mod half,
-  // interleaved dims 2p and 2p + 1 pair p.
+  // Runs of a token only split small calls: their number fits 32 bits.
+  const uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (unit >= j.tokens * st.runs) return;
+  const uint32_t t = unit / st.runs;
+  const uint32_t begin = (unit - t * st.runs) * st.run;
+  const uint32_t end = min(begin + st.run, st.all);
   bool bad_slot = false, non_finite = false;
-  float2 cs[4];
-  const bool turns = j.rope != nullptr && 4u * l < 2u * j.half && on;
+
+  // The lane's cos and sin, of its dims 4l + i (c = 0) and hd / 2 further
+  // (c = 1): half-split dims d use pair d mod half, interleaved dims 2p and
+  // 2p + 1 pair p.  Sines are negated where they multiply a pair's second.
+  const bool paired = !j.interleaved && 2u * j.half == HD;  // pairs meet in the lane
+  float co[2][4], si[2][4];
 #pragma unroll
-  for (uint32_t i = 0; i < 4u; ++i) cs[i] = make_float2(1.f, 0.f);
-  if (turns) {
+  for (uint32_t i = 0; i < 4u; ++i) {
+    co[0][i] = co[1][i] = 1.f;
+    si[0][i] = si[1][i] = 0.f;
+  }
+  if (j.rope != nullptr && begin < st.k) {
+    const int32_t p0 = __ldg(j.pos + t);
+    const int32_t p1 = j.cut[0] < j.half ? __ldg(j.pos + j.tokens + t) : 0;
+    const int32_t p2 = j.cut[1] < j.half ? __ldg(j.pos + 2ull * j.tokens + t) : 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) {
-      const uint32_t d = 4u * l + i;
-      if (j.interleaved && (i & 1u)) {
-        cs[i] = cs[i - 1u];
+    for (uint32_t c = 0; c < 2u; ++c) {
+      if (c == 1u && paired) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+          co[1][i] = co[0][i];
+          si[1][i] = si[0][i];
+        }
         continue;
       }
-      const uint32_t p = j.interleaved ? d / 2u : d < j.half ? d : d - j.half;
-      const uint32_t axis = (p >= j.cut[0] ? 1u : 0u) + (p >= j.cut[1] ? 1u : 0u);
-      const int32_t pos = __ldg(j.pos + static_cast<uint64_t>(axis) * j.tokens + t);
-      if (pos >= 0 && static_cast<uint32_t>(pos) < j.max_pos) {
-        cs[i] = __ldg(j.rope + static_cast<uint64_t>(pos) * j.half + p);
-      } else {
-        bad_slot = true;
+#pragma unroll
+      for (uint32_t i = 0; i < 4u; ++i) {
+        const uint32_t d = 4u * l + c * (HD / 2u) + i;
+        if (d >= 2u * j.half || !on) continue;
+        if (j.interleaved && (i & 1u)) {
+          co[c][i] = co[c][i - 1u];
+          si[c][i] = si[c][i - 1u];
+          continue;
+        }
+        const uint32_t p = j.interleaved ? d / 2u : d < j.half ? d : d - j.half;
+        const int32_t pos = p < j.cut[0] ? p0 : p < j.cut[1] ? p1 : p2;
+        if (pos >= 0 && static_cast<uint32_t>(pos) < j.max_pos) {
+          const float2 v = __ldg(j.rope + static_cast<uint64_t>(pos) * j.half + p);
+          co[c][i] = v.x;
+          si[c][i] = v.y;
+        } else {
+          bad_slot = true;
+        }
       }
     }
   }
@@ -108,152 +174,297 @@ __global__ void __launch_bounds__(kWarps * 32)
   const bool cached = slot >= 0 &&
                       (static_cast<uint32_t>(slot) >> j.cache.page_log2) < j.cache.pages;
   bad_slot |= slot >= 0 && !cached;
+
+  // Steps [begin, end) of q (W = 0), k (1) or v (2): numbers a .. b of its own.
+  auto phase = [&](auto which, uint32_t a, uint32_t b) {
+    constexpr uint32_t W = decltype(which)::value;
+    if (a >= b) return;
+    const uint32_t count = W == 0u ? j.heads : j.cache.kv_heads;
+    uint32_t h = a * kHeads + sub;
+    uint64_t at = t * j.ld[W] + h * HD + 4u * l;
+    float w[2][4];
+    const bool norm = W < 2u && j.norm[W < 2u ? W : 0u] != nullptr;
 #pragma unroll
-  for (uint32_t u = 0; u < kSteps; ++u) {
-    const uint32_t h = h0 + u * kHeads;
-    if (u >= steps || h0 - sub + u * kHeads >= all) break;  // the same for the whole warp
-    const bool mine = h < all && on;
-    const uint32_t which = h < j.heads ? 0u : h < qk ? 1u : 2u;
-    float y[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-    const float* w = which < 2u ? j.norm[which] : nullptr;
-    float ss = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
+    for (uint32_t c = 0; c < 2u; ++c)
 #pragma unroll
-    for (uint32_t d = kSpan / 2u; d > 0; d /= 2u) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
-    if (w != nullptr && mine) {
-      const float r = 1.0f / sqrtf(__fdiv_rn(ss, static_cast<float>(HD)) + j.eps);
-      const float* wl = w + 4u * l;
-#pragma unroll
-      for (uint32_t i = 0; i < 4u; ++i) y[i] = __fmul_rn(__fmul_rn(y[i], r), __ldg(wl + i));
+      for (uint32_t i = 0; i < 4u; ++i) {
+        w[c][i] = norm && on ? __ldg(j.norm[W < 2u ? W : 0u] + 4u * l + c * (HD / 2u) + i) : 0.f;
+      }
+    uint16_t* to = W == 0u ? static_cast<uint16_t*>(j.q_out) + t * j.ldqo + h * HD + 4u * l : nullptr;
+    uint8_t* rec = nullptr;
+    if (W != 0u && cached) {
+      rec = kv_record(j.cache, static_cast<uint32_t>(slot) >> j.cache.page_log2, h) +
+            (W == 1u ? 0u : kv_vcodes(j.cache)) +
+            (static_cast<uint32_t>(slot) & (j.cache.page - 1u)) * (HD / 2u) + 2u * l;
     }
-    if (j.rope != nullptr) {
-      float z[4];
-      if (j.interleaved) {
+    // From a lane's codes to its block's scale byte.
+    const uint32_t scales = W == 0u ? 0u
+        : kv_kscales(j.cache) - (static_cast<uint32_t>(slot) & (j.cache.page - 1u)) * (HD / 2u - HD / 32u) - 2u * l;
+    for (uint32_t s = a; s < b; s += kAhead) {
+      uint4 raw[kAhead][2];
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; i += 2u) {
-          z[i] = __fsub_rn(__fmul_rn(y[i], cs[i].x), __fmul_rn(y[i + 1u], cs[i].y));
-          z[i + 1u] = __fadd_rn(__fmul_rn(y[i + 1u], cs[i].x), __fmul_rn(y[i], cs[i].y));
+      for (uint32_t u = 0; u < kAhead; ++u) {
+        raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+        if (s + u < b && on && h + u * kHeads < count) {
+          raw[u][0] = load4<BF16, VEC>(j.x[W], at + u * (kHeads * HD));
+          raw[u][1] = load4<BF16, VEC>(j.x[W], at + u * (kHeads * HD) + HD / 2u);
         }
-      } else {
-        const bool first = 4u * l < j.half;
-        const uint32_t other = first ? l + j.half / 4u : l - j.half / 4u;
+      }
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-          const float o = __shfl_sync(0xFFFFFFFFu, y[i], sub * kSpan + (other & (kSpan - 1u)));
-          const float a = __fmul_rn(y[i], cs[i].x), b = __fmul_rn(o, cs[i].y);
-          z[i] = first ? __fsub_rn(a, b) : __fadd_rn(a, b);
+      for (uint32_t u = 0; u < kAhead; ++u) {
+        if (s + u >= b) break;  // the same for the whole warp
+        const bool mine = on && h + u * kHeads < count;
+        float y[2][4];
+        values4<BF16>(raw[u][0], y[0]);
+        values4<BF16>(raw[u][1], y[1]);
+        if constexpr (W < 2u) {
+          if (norm) {
+            uint64_t sq = 0;
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c)
+#pragma unroll
+              for (uint32_t i = 0; i < 4u; i += 2u) {
+                const uint64_t v = pack2(y[c][i], y[c][i + 1u]);
+                sq = fma_2(v, v, sq);
+              }
+            float ss = unpack2(sq).x + unpack2(sq).y;
+#pragma unroll
+            for (uint32_t d = kSpan / 2u; d > 0; d /= 2u) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
+            const float r = rsqrtf(ss * (1.0f / HD) + j.eps);
+            const uint64_t rr = pack2(r, r);
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c)
+#pragma unroll
+              for (uint32_t i = 0; i < 4u; i += 2u) {
+                const float2 v = unpack2(mul_2(mul_2(pack2(y[c][i], y[c][i + 1u]), rr),
+                                               pack2(w[c][i], w[c][i + 1u])));
+                y[c][i] = v.x;
+                y[c][i + 1u] = v.y;
+              }
+          }
+          if (paired) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i += 2u) {
+              const uint64_t va = pack2(y[0][i], y[0][i + 1u]), vb = pack2(y[1][i], y[1][i + 1u]);
+              const uint64_t c2 = pack2(co[0][i], co[0][i + 1u]);
+              const uint64_t s2 = pack2(si[0][i], si[0][i + 1u]);
+              const uint64_t n2 = pack2(-si[0][i], -si[0][i + 1u]);
+              const float2 x = unpack2(add_2(mul_2(va, c2), mul_2(vb, n2)));
+              const float2 z = unpack2(add_2(mul_2(vb, c2), mul_2(va, s2)));
+              y[0][i] = x.x;
+              y[0][i + 1u] = x.y;
+              y[1][i] = z.x;
+              y[1][i + 1u] = z.y;
+            }
+          } else if (j.interleaved) {
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c)
+#pragma unroll
+              for (uint32_t i = 0; i < 4u; i += 2u) {
+                const float p = y[c][i], q = y[c][i + 1u];
+                y[c][i] = __fsub_rn(__fmul_rn(p, co[c][i]), __fmul_rn(q, si[c][i]));
+                y[c][i + 1u] = __fadd_rn(__fmul_rn(q, co[c][i]), __fmul_rn(p, si[c][i]));
+              }
+          } else if (j.half != 0u) {
+            // Fours of dims: number f is slot f / kLanes of lane f % kLanes.
+            float z[2][4];
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c) {
+              const uint32_t f = l + c * kLanes, hf = j.half / 4u;
+              const bool low = f < hf;
+              const uint32_t from = low ? f + hf : f - hf;
+              const uint32_t lane_of = (sub * kSpan + from % kLanes) & 31u;
+#pragma unroll
+              for (uint32_t i = 0; i < 4u; ++i) {
+                const float o0 = __shfl_sync(0xFFFFFFFFu, y[0][i], lane_of);
+                const float o1 = __shfl_sync(0xFFFFFFFFu, y[1][i], lane_of);
+                const float p = __fmul_rn(y[c][i], co[c][i]);
+                const float q = __fmul_rn(from < kLanes ? o0 : o1, si[c][i]);
+                z[c][i] = f >= 2u * hf ? y[c][i] : low ? __fsub_rn(p, q) : __fadd_rn(p, q);
+              }
+            }
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c)
+#pragma unroll
+              for (uint32_t i = 0; i < 4u; ++i) y[c][i] = z[c][i];
+          }
+        }
+        if constexpr (W == 0u) {
+          if (mine) {
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c) {
+              const __nv_bfloat162 p = __floats2bfloat162_rn(y[c][0], y[c][1]);
+              const __nv_bfloat162 q = __floats2bfloat162_rn(y[c][2], y[c][3]);
+              *reinterpret_cast<uint2*>(to + u * (kHeads * HD) + c * (HD / 2u)) = make_uint2(
+                  *reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+            }
+          }
+        } else {
+          uint32_t top[2];
+#pragma unroll
+          for (uint32_t c = 0; c < 2u; ++c) {
+            top[c] = __float_as_uint(fmaxf(fmaxf(fabsf(y[c][0]), fabsf(y[c][1])),
+                                           fmaxf(fabsf(y[c][2]), fabsf(y[c][3]))));
+          }
+          // fmaxf passes NaNs over: a sum of the values' products with zero does not.
+          float odd = 0.f;
+#pragma unroll
+          for (uint32_t c = 0; c < 2u; ++c)
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) odd = fmaf(y[c][i], 0.f, odd);
+          if (odd != odd) {  // rare: NaN counts as zero, Inf saturates
+            non_finite = true;
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c)
+#pragma unroll
+              for (uint32_t i = 0; i < 4u; ++i) {
+                if (y[c][i] != y[c][i]) y[c][i] = 0.f;
+              }
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c) {
+              top[c] = __float_as_uint(fmaxf(fmaxf(fabsf(y[c][0]), fabsf(y[c][1])),
+                                             fmaxf(fabsf(y[c][2]), fabsf(y[c][3]))));
+            }
+          }
+          uint32_t block[2];  // the blocks that the lane's fours lie in
+          if constexpr (HD == 96u) {
+            uint32_t all[3];
+#pragma unroll
+            for (uint32_t k = 0; k < 3u; ++k) {
+              all[k] = max(l / 8u == k ? top[0] : 0u, (l + kLanes) / 8u == k ? top[1] : 0u);
+#pragma unroll
+              for (uint32_t d = 8; d > 0; d /= 2u) {
+                all[k] = max(all[k], __shfl_xor_sync(0xFFFFFFFFu, all[k], d));
+              }
+            }
+            block[0] = l / 8u;
+            block[1] = min((l + kLanes) / 8u, 2u);
+            top[0] = block[0] == 0u ? all[0] : all[1];
+            top[1] = block[1] == 1u ? all[1] : all[2];
+          } else if constexpr (HD == 32u) {
+            block[0] = block[1] = 0u;
+            top[0] = max(top[0], top[1]);
+            top[0] = max(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], 1));
+            top[0] = max(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], 2));
+            top[1] = top[0];
+          } else {
+            block[0] = l / 8u;
+            block[1] = HD / 64u + l / 8u;
+#pragma unroll
+            for (uint32_t d = 1; d < 8u; d *= 2u) {
+              top[0] = max(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], d));
+              top[1] = max(top[1], __shfl_xor_sync(0xFFFFFFFFu, top[1], d));
+            }
+          }
+          if (mine && cached) {
+            uint8_t* r8 = rec + static_cast<uint64_t>(u * kHeads) * j.cache.record;
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c) {
+              const int32_t e = kv_block_exp(top[c]);
+              const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+              const uint32_t codes = e2m1_pair(y[c][0] * inv, y[c][1] * inv) |
+                                     (e2m1_pair(y[c][2] * inv, y[c][3] * inv) << 8);
+              *reinterpret_cast<uint16_t*>(r8 + c * (HD / 4u)) = static_cast<uint16_t>(codes);
+              if ((l + c * kLanes) % 8u == 0u) {
+                r8[static_cast<int64_t>(static_cast<int32_t>(scales)) + block[c]] = static_cast<uint8_t>(e + 127);
+              }
+            }
+          }
         }
       }
-#pragma unroll
-      for (uint32_t i = 0; i < 4u; ++i) y[i] = turns && which < 2u ? z[i] : y[i];
+      h += kAhead * kHeads;
+      at += kAhead * kHeads * HD;
+      if (W == 0u) to += kAhead * kHeads * HD;
+      if (W != 0u && cached) rec += static_cast<uint64_t>(kAhead * kHeads) * j.cache.record;
     }
-    if (which == 0u) {
-      if (mine) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]);
-        const __nv_bfloat162 b = __floats2bfloat162_rn(y[2], y[3]);
-        uint2 v;
-        v.x = *reinterpret_cast<const uint32_t*>(&a);
-        v.y = *reinterpret_cast<const uint32_t*>(&b);
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(j.q_out) + t * j.ldqo +
-                                  static_cast<uint64_t>(h) * HD + 4u * l) = v;
-      }
-    }
-    if (__all_sync(0xFFFFFFFFu, which == 0u)) continue;
-    uint32_t top = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) {
-      const uint32_t mag = __float_as_uint(y[i]) & 0x7FFFFFFFu;
-      if (which != 0u && mag >= 0x7F800000u) {
-        non_finite = true;
-        if (mag > 0x7F800000u) y[i] = 0.f;
-      }
-      top = max(top, __float_as_uint(y[i]) & 0x7FFFFFFFu);
-    }
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-    if (which == 0u || !mine || !cached) continue;
-    const int32_t e = kv_block_exp(top);
-    const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    const uint32_t codes = e2m1_pair(y[0] * inv, y[1] * inv) |
-                           (e2m1_pair(y[2] * inv, y[3] * inv) << 8);
-    const uint32_t in_page = static_cast<uint32_t>(slot) & (j.cache.page - 1u);
-    uint8_t* rec = kv_record(j.cache, static_cast<uint32_t>(slot) >> j.cache.page_log2,
-                             which == 1u ? h - j.heads : h - qk) +
-                   (which == 1u ? 0u : kv_vcodes(j.cache));
-    *reinterpret_cast<uint16_t*>(rec + in_page * (HD / 2u) + 2u * l) =
-        static_cast<uint16_t>(codes);
-    if ((l & 7u) == 0u) {
-      rec[kv_kscales(j.cache) + in_page * (HD / 32u) + l / 8u] = static_cast<uint8_t>(e + 127);
-    }
-  }
+  };
+  phase(Which<0>{}, min(begin, st.q), min(end, st.q));
+  phase(Which<1>{}, max(begin, st.q) - st.q, min(max(end, st.q), st.k) - st.q);
+  phase(Which<2>{}, max(begin, st.k) - st.k, max(end, st.k) - st.k);
   const uint32_t err = (bad_slot ? kErrKvSlot : 0u) | (non_finite ? kErrKvNonFinite : 0u);
   if (err != 0u) atomicOr(error_flag, err);
 }
 
-// A thread reads eight dims (one word of codes) of K and of V.
-__global__ void __launch_bounds__(256)
-    k_kv_read(const KvCache c, const int32_t* __restrict__ slots, uint32_t tokens, uint32_t dtype,
-              void* k, void* v, uint32_t* __restrict__ error_flag) {
-  const uint32_t words = c.hd / 8u, row = c.kv_heads * words;
-  const uint64_t n = static_cast<uint64_t>(tokens) * row;
-  const uint64_t step = static_cast<uint64_t>(gridDim.x) * blockDim.x;
-  bool bad = false;
-  for (uint64_t at = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; at < n;
-       at += step) {
-    const uint32_t t = static_cast<uint32_t>(at / row), i = static_cast<uint32_t>(at % row);
-    const uint32_t head = i / words, w = i % words;
-    const int32_t slot = __ldg(slots + t);
-    const uint32_t page = static_cast<uint32_t>(slot) >> c.page_log2;
-    const bool there = slot >= 0 && page < c.pages;
-    bad |= slot >= 0 && !there;
+// Sixteen dims (two words of codes) of K and of V a step; a block takes
+// kTokens tokens.  Values are exact in FP16, and from there in each type.
+constexpr uint32_t kTokens = 8;
+
+template <uint32_t DT>
+__device__ __forceinline__ void put16(void* out, uint64_t at, const uint32_t (&h)[8]) {
+  if constexpr (DT == HRB_DT_E5M2) {
+    uint32_t r[4];
 #pragma unroll
-    for (uint32_t part = 0; part < 2u; ++part) {
-      void* out = part == 0u ? k : v;
-      if (out == nullptr) continue;
-      uint32_t h[4] = {0, 0, 0, 0};
-      float scale = 0.f;
-      if (there) {
-        const uint32_t in_page = static_cast<uint32_t>(slot) & (c.page - 1u);
-        const uint8_t* rec = kv_record(c, page, head) + (part == 0u ? 0u : kv_vcodes(c));
-        const uint32_t codes =
-            *reinterpret_cast<const uint32_t*>(rec + in_page * (c.hd / 2u) + 4u * w);
-        scale = kv_scale(rec[kv_kscales(c) + in_page * (c.hd / 32u) + w / 4u]);
-        e2m1x8_to_f16x2(codes, h);
-      }
-      float f[8];
+    for (uint32_t i = 0; i < 4u; ++i) {
+      uint16_t a, b;
+      asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(a) : "r"(h[2u * i]));
+      asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(b) : "r"(h[2u * i + 1u]));
+      r[i] = a | (static_cast<uint32_t>(b) << 16);
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + at) = make_uint4(r[0], r[1], r[2], r[3]);
+  } else {
 #pragma unroll
-      for (uint32_t b = 0; b < 4u; ++b) {
-        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&h[b]));
-        f[2u * b] = p.x * scale;
-        f[2u * b + 1u] = p.y * scale;
-      }
-      const uint64_t o = at * 8u;
-      if (dtype == HRB_DT_F32) {
-        float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + o);
-        p[0] = make_float4(f[0], f[1], f[2], f[3]);
-        p[1] = make_float4(f[4], f[5], f[6], f[7]);
-      } else if (dtype == HRB_DT_BF16) {
-        uint32_t r[4];
+    for (uint32_t i = 0; i < 2u; ++i) {
+      float2 f[4];
 #pragma unroll
-        for (uint32_t b = 0; b < 4u; ++b) {
-          const __nv_bfloat162 p = __floats2bfloat162_rn(f[2u * b], f[2u * b + 1u]);
-          r[b] = *reinterpret_cast<const uint32_t*>(&p);
-        }
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + o) =
-            make_uint4(r[0], r[1], r[2], r[3]);
+      for (uint32_t d = 0; d < 4u; ++d) f[d] = __half22float2(*reinterpret_cast<const __half2*>(&h[4u * i + d]));
+      if constexpr (DT == HRB_DT_F32) {
+        float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + at + 8u * i);
+        p[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+        p[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
       } else {
         uint32_t r[4];
 #pragma unroll
-        for (uint32_t b = 0; b < 4u; ++b) {
-          uint16_t two;
-          asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;"
-              : "=h"(two)
-              : "f"(f[2u * b + 1u]), "f"(f[2u * b]));
-          r[b] = two;
+        for (uint32_t d = 0; d < 4u; ++d) {
+          const __nv_bfloat162 p = __floats2bfloat162_rn(f[d].x, f[d].y);
+          r[d] = *reinterpret_cast<const uint32_t*>(&p);
         }
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(out) + o) =
-            make_uint2(r[0] | (r[1] << 16), r[2] | (r[3] << 16));
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at + 8u * i) =
+            make_uint4(r[0], r[1], r[2], r[3]);
       }
+    }
+  }
+}
+
+template <uint32_t DT>
+__global__ void __launch_bounds__(256)
+    k_kv_read(const KvCache c, const int32_t* __restrict__ slots, uint32_t tokens, FastDiv row_div,
+              FastDiv head_div, void* k, void* v, uint32_t* __restrict__ error_flag) {
+  const uint32_t t0 = blockIdx.x * kTokens, n = min(kTokens, tokens - t0) * row_div.d;
+  bool bad = false;
+  for (uint32_t i = threadIdx.x; i < n; i += 256u) {
+    const uint32_t t = fast_div(i, row_div), x = i - t * row_div.d;
+    const uint32_t head = fast_div(x, head_div), w = x - head * head_div.d;
+    const int32_t slot = __ldg(slots + t0 + t);
+    const uint32_t page = static_cast<uint32_t>(slot) >> c.page_log2;
+    const bool there = slot >= 0 && page < c.pages;
+    bad |= slot >= 0 && !there;
+    uint2 codes[2] = {make_uint2(0, 0), make_uint2(0, 0)};
+    uint32_t scale[2] = {127u, 127u};
+    if (there) {
+      const uint32_t in_page = static_cast<uint32_t>(slot) & (c.page - 1u);
+      const uint8_t* rec = kv_record(c, page, head);
+#pragma unroll
+      for (uint32_t p = 0; p < 2u; ++p) {
+        const uint8_t* part = rec + (p == 0u ? 0u : kv_vcodes(c));
+        codes[p] = *reinterpret_cast<const uint2*>(part + in_page * (c.hd / 2u) + 8u * w);
+        scale[p] = part[kv_kscales(c) + in_page * (c.hd / 32u) + w / 2u];
+      }
+    }
+    const uint64_t at = (static_cast<uint64_t>(t0 + t) * row_div.d + x) * 16u;
+#pragma unroll
+    for (uint32_t p = 0; p < 2u; ++p) {
+      void* out = p == 0u ? k : v;
+      if (out == nullptr) continue;
+      uint32_t a[4], b[4], h[8];
+      e2m1x8_to_f16x2(codes[p].x, a);
+      e2m1x8_to_f16x2(codes[p].y, b);
+      const uint32_t sc = scale2(scale[p], scale[p]);
+#pragma unroll
+      for (uint32_t d = 0; d < 4u; ++d) {
+        h[d] = mul2(a[d], sc);
+        h[4u + d] = mul2(b[d], sc);
+      }
+      put16<DT>(out, at, h);
     }
   }
   if (bad) atomicOr(error_flag, kErrKvSlot);
@@ -262,20 +473,27 @@ __global__ void __launch_bounds__(256)
 template <uint32_t HD>
 void launch_hd(const QkvJob& job, bool bf16, bool vec, uint32_t* err, int sm_count,
                cudaStream_t stream) {
-  constexpr uint32_t kHeads = HD == 32u ? 4u : HD == 64u ? 2u : 1u;
-  const uint32_t rows = (job.heads + 2u * job.cache.kv_heads + kHeads - 1u) / kHeads;
-  // One head step a warp while that does not fill the GPU.
-  const uint64_t fill = static_cast<uint64_t>(sm_count) * 32u;
-  const uint32_t steps = static_cast<uint64_t>(job.tokens) * rows > fill ? kSteps : 1u;
-  const uint32_t chunks = (rows + steps - 1u) / steps;
-  const uint64_t units = static_cast<uint64_t>(job.tokens) * chunks;
+  constexpr uint32_t kHeads = 32u / (HD == 96u ? 16u : HD / 8u);
+  Steps st;
+  st.q = (job.heads + kHeads - 1u) / kHeads;
+  const uint32_t kv = (job.cache.kv_heads + kHeads - 1u) / kHeads;
+  st.k = st.q + kv;
+  st.all = st.k + kv;
+  // A warp takes as many steps as leave two warps a scheduler, in whole
+  // loads of kAhead where that is more.
+  const uint64_t warps = static_cast<uint64_t>(sm_count) * 8u;
+  const uint64_t run = static_cast<uint64_t>(job.tokens) * st.all / warps;
+  st.run = run < 1u ? 1u : run < st.all ? static_cast<uint32_t>(run) : st.all;
+  if (st.run > kAhead) st.run = (st.run + kAhead - 1u) / kAhead * kAhead;
+  st.runs = (st.all + st.run - 1u) / st.run;
+  const uint64_t units = static_cast<uint64_t>(job.tokens) * st.runs;
   const unsigned grid = static_cast<unsigned>((units + kWarps - 1u) / kWarps);
   if (bf16) {
-    if (vec) k_qkv<HD, true, true><<<grid, kWarps * 32, 0, stream>>>(job, chunks, steps, err);
-    else k_qkv<HD, true, false><<<grid, kWarps * 32, 0, stream>>>(job, chunks, steps, err);
+    if (vec) k_qkv<HD, true, true><<<grid, kWarps * 32, 0, stream>>>(job, st, err);
+    else k_qkv<HD, true, false><<<grid, kWarps * 32, 0, stream>>>(job, st, err);
   } else {
-    if (vec) k_qkv<HD, false, true><<<grid, kWarps * 32, 0, stream>>>(job, chunks, steps, err);
-    else k_qkv<HD, false, false><<<grid, kWarps * 32, 0, stream>>>(job, chunks, steps, err);
+    if (vec) k_qkv<HD, false, true><<<grid, kWarps * 32, 0, stream>>>(job, st, err);
+    else k_qkv<HD, false, false><<<grid, kWarps * 32, 0, stream>>>(job, st, err);
   }
 }
 
@@ -292,11 +510,17 @@ void launch_qkv_append(const QkvJob& job, bool bf16, bool vec, uint32_t* error_f
 }
 
 void launch_kv_read(const KvCache& cache, const int32_t* slots, uint32_t tokens, uint32_t dtype,
-                    void* k, void* v, uint32_t* error_flag, int sm_count, cudaStream_t stream) {
-  const uint64_t n = static_cast<uint64_t>(tokens) * cache.kv_heads * (cache.hd / 8u);
-  const uint64_t blocks = (n + 255u) / 256u, most = static_cast<uint64_t>(sm_count) * 16u;
-  k_kv_read<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(
-      cache, slots, tokens, dtype, k, v, error_flag);
+                    void* k, void* v, uint32_t* error_flag, cudaStream_t stream) {
+  const FastDiv row = make_fast_div(cache.kv_heads * (cache.hd / 16u));
+  const FastDiv head = make_fast_div(cache.hd / 16u);
+  const unsigned grid = (tokens + kTokens - 1u) / kTokens;
+  if (dtype == HRB_DT_F32) {
+    k_kv_read<HRB_DT_F32><<<grid, 256, 0, stream>>>(cache, slots, tokens, row, head, k, v, error_flag);
+  } else if (dtype == HRB_DT_BF16) {
+    k_kv_read<HRB_DT_BF16><<<grid, 256, 0, stream>>>(cache, slots, tokens, row, head, k, v, error_flag);
+  } else {
+    k_kv_read<HRB_DT_E5M2><<<grid, 256, 0, stream>>>(cache, slots, tokens, row, head, k, v, error_flag);
+  }
 }
 
 }  // namespace hrb

@@ -325,8 +325,7 @@ hrb_status hrb_kv_read(hrb_ctx* ctx, const hrb_kv_cache* cache, const int32_t* s
     return refuse(ctx, HRB_ECUDA, "cudaSetDevice");
   }
   hrb::launch_kv_read(hrb::make_kv_cache(*cache), slots, tokens, dtype, k, v,
-                      hrb::ctx_error_word(ctx), hrb::ctx_sm_count(ctx),
-                      hrb::ctx_stream(ctx, stream));
+                      hrb::ctx_error_word(ctx), hrb::ctx_stream(ctx, stream));
   return launched(ctx, 1, "hrb_kv_read");
 }
 
