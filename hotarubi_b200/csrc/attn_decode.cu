@@ -196,6 +196,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int32_t e = min(max(static_cast<int32_t>(top >> 7), 27), 254) - 127;
     const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
     row_scale[nt] = __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
+    if (top >= 0x7F80u) row_scale[nt] = NAN;  // Inf or NaN in the row
 #pragma unroll
     for (uint32_t i = 0; i < HD / 8u; ++i) {
       const uint32_t h2 = half2_bits(__floats2half2_rn(__uint_as_float(w[i] << 16) * up,

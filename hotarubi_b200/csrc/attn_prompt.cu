@@ -164,7 +164,7 @@ struct Smem {
   static constexpr uint32_t kK = kQ;                         // two K stages
   static constexpr uint32_t kV = kK + 2u * k_bytes(HD);      // two V^T stages
   static constexpr uint32_t kBars = kV + 2u * v_bytes(HD);
-  static constexpr uint32_t kUsed = kBars + 128u;
+  static constexpr uint32_t kUsed = kBars + 144u;
   // Over half an SM's shared memory: one block an SM, for its 512 columns of
   // TMEM.
   static constexpr uint32_t kBytes = (kUsed > 120u * 1024u ? kUsed : 120u * 1024u) + 1024u;
@@ -176,6 +176,62 @@ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) {
   return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
+// Of eight pairs of weights, how many are taken on the FMA pipe.
+#ifndef POLY
+#define POLY 3u
+#endif
+constexpr uint32_t kPolyOf8 = POLY;
+
+// A row's raw scores to softcap log2(e) tanh(factor s / softcap).  Where all
+// of a warp's arguments are under 1/2, tanh is its power series up to x^11
+// (the next term is under 4.4e-7 there) on the FMA pipe; else 1 - 2 / (1 +
+// e^2x).
+__device__ __forceinline__ void cap_scores(const AttnJob& j, float factor, uint32_t (&s)[4][32]) {
+  const float f = factor * j.cap_inv;
+  const uint64_t f2 = pack2(f, f);
+  float top[4];
+#pragma unroll
+  for (uint32_t c = 0; c < 4u; ++c) {
+    top[c] = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < 32u; i += 2u) {
+      top[c] = fmaxf(fmaxf(top[c], fabsf(__uint_as_float(s[c][i]))), fabsf(__uint_as_float(s[c][i + 1u])));
+    }
+  }
+  const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+  const float b = j.cap_out;
+  if (__all_sync(0xFFFFFFFFu, high < 0.5f)) {
+    const uint64_t a1 = pack2(b, b), a3 = pack2(b * (-1.f / 3.f), b * (-1.f / 3.f));
+    const uint64_t a5 = pack2(b * (2.f / 15.f), b * (2.f / 15.f));
+    const uint64_t a7 = pack2(b * (-17.f / 315.f), b * (-17.f / 315.f));
+    const uint64_t a9 = pack2(b * (62.f / 2835.f), b * (62.f / 2835.f));
+    const uint64_t a11 = pack2(b * (-1382.f / 155925.f), b * (-1382.f / 155925.f));
+#pragma unroll
+    for (uint32_t c = 0; c < 4u; ++c)
+#pragma unroll
+      for (uint32_t i = 0; i < 32u; i += 2u) {
+        const uint64_t x = mul_2(pack2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1u])), f2);
+        const uint64_t u = mul_2(x, x);
+        uint64_t r = fma_2(u, a11, a9);
+        r = fma_2(r, u, a7);
+        r = fma_2(r, u, a5);
+        r = fma_2(r, u, a3);
+        r = fma_2(r, u, a1);
+        const float2 y = unpack2(mul_2(r, x));
+        s[c][i] = __float_as_uint(y.x);
+        s[c][i + 1u] = __float_as_uint(y.y);
+      }
+  } else {
+#pragma unroll
+    for (uint32_t c = 0; c < 4u; ++c)
+#pragma unroll
+      for (uint32_t i = 0; i < 32u; ++i) {
+        const float y = ex2(__uint_as_float(s[c][i]) * factor * j.cap_in);
+        s[c][i] = __float_as_uint(b * (1.0f - __fdividef(2.0f, 1.0f + y)));
+      }
+  }
+}
+
 template <uint32_t HD>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attn_prompt(const AttnJob j, uint32_t* __restrict__ error_flag) {
@@ -184,8 +240,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5,
-           *v_empty = bars + 7, *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 13;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+           *v_empty = bars + 7, *s_full = bars + 9, *o_full = bars + 11,
+           *p_full = bars + 13;  // [half][first or second 64 keys]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
 
   const uint32_t head = blockIdx.x % j.cache.kv_heads, n = blockIdx.z;
@@ -228,7 +285,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(v_full + i, 1);
       mbar_init(v_empty + i, 1);
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, kHalf);
+      mbar_init(p_full + 2u * i, kHalf);
+      mbar_init(p_full + 2u * i + 1u, kHalf);
       mbar_init(o_full + i, 1);
     }
     fence_barrier_init();
@@ -290,16 +348,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t st = static_cast<uint32_t>(it) & 1u, ph = (static_cast<uint32_t>(it) >> 1) & 1u;
         const bool more = it + 1 < count;
         for (uint32_t h = 0; h < halves && ok; ++h) {
-          ok = mbar_wait(p_full + h, static_cast<uint32_t>(it) & 1u, error_flag) &&
-               (h != 0u || mbar_wait(v_full + st, ph, error_flag));
-          if (!ok) break;
-          tc_fence_after();
+          if (h == 0u) ok = mbar_wait(v_full + st, ph, error_flag);
 #pragma unroll
-          for (uint32_t k = 0; k < kKeys / 16u; ++k) {
+          for (uint32_t k = 0; k < kKeys / 16u && ok; ++k) {
+            if ((k & 3u) == 0u) {  // 64 keys' weights
+              ok = mbar_wait(p_full + 2u * h + (k >> 2), static_cast<uint32_t>(it) & 1u, error_flag);
+              if (!ok) break;
+              tc_fence_after();
+            }
             mma_bf16_ts(tmem + 256u + 128u * h, tmem + 128u * h + 8u * k,
                         desc_sw128(v_at + st * v_bytes(HD) + (k >> 2) * (HD * kRowB) + 32u * (k & 3u)),
                         idesc_f16(128, HD), it != 0 || k != 0u);
           }
+          if (!ok) break;
           if (more) {
             const uint32_t nst = static_cast<uint32_t>(it + 1) & 1u;
             ok = h != 0u || mbar_wait(k_full + nst, (static_cast<uint32_t>(it + 1) >> 1) & 1u, error_flag);
@@ -323,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t row = static_cast<uint64_t>(q0 + (mine ? r : r0) / group);
     const uint32_t qh = head * j.group + static_cast<uint32_t>((mine ? r : r0) % group);
     float factor;
+    bool odd;  // Inf or NaN in the row of Q: its outputs are NaN
     {
       // The row of Q as FP16, scaled so that its largest value is in
       // [2^13, 2^14) and signed so that the scores' factor is not negative.
@@ -335,6 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (uint32_t d = 0; d < 4u; ++d) top = max(top, max(w[d] & 0x7FFFu, (w[d] >> 16) & 0x7FFFu));
       }
+      odd = top >= 0x7F80u;
       const int32_t e = min(max(static_cast<int32_t>(top >> 7), 27), 254) - 127;
       float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
       if (!mine) up = 0.f;
@@ -380,20 +443,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int32_t k0 = c0 + tile_at(it) * static_cast<int32_t>(kKeys);
         const int32_t k1 = k0 + static_cast<int32_t>(kKeys);
         auto at = [&](uint32_t c, uint32_t i) -> float { return __uint_as_float(s[c][i]); };
+        auto pair = [&](uint32_t c, uint32_t i) { return pack2(at(c, i), at(c, i + 1u)); };
         float scale = factor;
-        if (j.softcap != 0.f || j.slopes != nullptr) {
+        if (j.softcap != 0.f) {
           scale = 1.0f;
+          cap_scores(j, factor, s);
+        }
+        if (j.slopes != nullptr) {
+          const float far = static_cast<float>(pos - k0);
 #pragma unroll
           for (uint32_t c = 0; c < 4u; ++c)
 #pragma unroll
             for (uint32_t i = 0; i < 32u; ++i) {
-              float x = at(c, i) * factor;
-              if (j.softcap != 0.f) {
-                x = j.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(x * j.cap_in)));
-              }
-              x -= slope * fabsf(static_cast<float>(pos - k0 - static_cast<int32_t>(32u * c + i)));
-              s[c][i] = __float_as_uint(x);
+              s[c][i] = __float_as_uint(fmaf(-slope, fabsf(far - static_cast<float>(32u * c + i)),
+                                             at(c, i) * scale));
             }
+          scale = 1.0f;
         }
         const bool clear = (k0 >= seen.lo && k1 <= seen.hi) || k1 <= seen.pre;
         if (!__all_sync(0xFFFFFFFFu, clear)) {
@@ -410,9 +475,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         float top[4];
 #pragma unroll
         for (uint32_t c = 0; c < 4u; ++c) {
-          top[c] = at(c, 0);
+          top[c] = fmaxf(at(c, 0), at(c, 1));
 #pragma unroll
-          for (uint32_t i = 1; i < 32u; ++i) top[c] = fmaxf(top[c], at(c, i));
+          for (uint32_t i = 2; i < 32u; i += 2u) top[c] = fmaxf(fmaxf(top[c], at(c, i)), at(c, i + 1u));
         }
         const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
         const bool moves = high > m + kLazy;
@@ -433,28 +498,37 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float shift = m == -INFINITY ? 0.f : -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2x = pack2(scale, scale), shift2x = pack2(shift, shift);
+        uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (uint32_t c = 0; c < 2u; ++c) {
           uint32_t p[32];
 #pragma unroll
           for (uint32_t i = 0; i < 32u; ++i) {
-            const float x = ex2(fmaf(at(2u * c + i / 16u, 2u * (i % 16u)), scale, shift));
-            const float y = ex2(fmaf(at(2u * c + i / 16u, 2u * (i % 16u) + 1u), scale, shift));
-            sum[i & 1u] += x;
-            sum[2u + (i & 1u)] += y;
-            p[i] = half2_bits(__floats2half2_rn(x, y));
+            const uint64_t x = fma_2(pair(2u * c + i / 16u, 2u * (i % 16u)), scale2x, shift2x);
+            // kPolyOf8 of eight pairs on the FMA pipe, the others on MUFU.
+            float2 e;
+            if (((i * kPolyOf8) & 7u) < kPolyOf8) {
+              e = ex2_fma(x);
+            } else {
+              const float2 v = unpack2(x);
+              e = make_float2(ex2(v.x), ex2(v.y));
+            }
+            sum[i & 3u] = add_2(sum[i & 3u], pack2(e.x, e.y));
+            p[i] = half2_bits(__floats2half2_rn(e.x, e.y));
           }
           tmem_st32(t_s + 32u * c, p);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(p_full + 2u * h + c);  // the product of these 64 keys may start
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(p_full + h);
+        const float2 all = unpack2(add_2(add_2(sum[0], sum[1]), add_2(sum[2], sum[3])));
+        l += all.x + all.y;
       }
       if (count > 0 && ok) ok = mbar_wait(o_full + h, 0, error_flag);
       if (__all_sync(0xFFFFFFFFu, ok)) {
         tc_fence_after();
+        if (odd && (seen.lo < seen.hi || seen.pre > 0)) l = NAN;
         const float inv = l != 0.f ? 1.0f / l : 0.f;
         const uint64_t cell = (static_cast<uint64_t>(chunk) * j.total_q + row) * j.heads + qh;
 #pragma unroll

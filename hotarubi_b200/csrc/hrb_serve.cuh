@@ -63,7 +63,7 @@ struct AttnJob {
   uint32_t causal, window;
   uint32_t device;
   float scale, softcap;
-  float cap_in, cap_out;  // 2 log2(e) / softcap, softcap * log2(e)
+  float cap_inv, cap_in, cap_out;  // 1 / softcap, 2 log2(e) / softcap, softcap * log2(e)
   // Keys a block of the split kernels takes, and the chunks' results: rows
   // of (m, l) and O, [chunk][total_q][heads] and the same by [hd].
   uint32_t chunk;

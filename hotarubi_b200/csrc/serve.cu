@@ -152,6 +152,7 @@ hrb::AttnJob attn_job(const hrb_ctx* ctx, const hrb_attn_desc* d) {
   j.window = d->window;
   j.scale = d->scale;
   j.softcap = d->softcap;
+  j.cap_inv = d->softcap != 0.f ? 1.0f / d->softcap : 0.f;
   j.cap_in = d->softcap != 0.f ? 2.885390081777927f / d->softcap : 0.f;
   j.cap_out = d->softcap * 1.4426950408889634f;
   return j;

@@ -772,7 +772,8 @@ HRB_API hrb_status hrb_kv_read(hrb_ctx* ctx, const hrb_kv_cache* cache, const in
  *   slopes: s_j -= slopes[h] * |i - j|;  out = sum_j softmax_j(s) v_j
  * over the keys 0 <= j < kv_len[n] that row sees: all of them, or with
  * `causal` those with j <= i (and j > i - window, when window is not 0) and
- * those with j < prefix[n].  A row that sees none gives zeros.  Scores,
+ * those with j < prefix[n].  A row that sees none gives zeros, one that does
+ * and has an Inf or NaN in q gives NaN.  Scores,
  * softmax statistics and sums are FP32; q and the softmax weights enter the
  * tensor cores as FP16 (q after a power-of-two scaling of its row).
  * A negative length is no keys.  A table entry outside the cache reads as a
