@@ -2,8 +2,8 @@
 // ones): the cache is streamed once and everything else hides behind it.
 //
 // A block serves one request, one key/value head and a chunk of its keys;
-// all rows that read that head (rows of q times query heads a key/value head,
-// at most 8 NT) are one operand.  Each of its warps takes tiles of 32 keys
+// the rows that read that head (rows of q times query heads a key/value head)
+// are one operand, in blocks of 8 NT.  Each of its warps takes tiles of 32 keys
 // on its own: bulk copies bring a tile's codes and scales into the warp's
 // ring in shared memory, the lanes turn them into FP16 in registers
 // (cvt.e2m1x2, times the block scale: both exact) straight in the layout of
@@ -100,9 +100,13 @@ __global__ void __launch_bounds__(kWarps * 32)
     if (blockIdx.x == 0u && threadIdx.x == 0u) atomicOr(error_flag, kErrKvSlot);
     return;
   }
-  const int32_t rows = q_len * static_cast<int32_t>(j.group);
-  const int32_t c0 = static_cast<int32_t>(blockIdx.x * j.chunk);
-  if (rows == 0 || (c0 >= kv && c0 > 0)) return;
+  // Rows r0 .. r0 + rows - 1 of the request's, a block of kRows.
+  const int32_t group = static_cast<int32_t>(j.group);
+  const uint32_t chunk = blockIdx.x / j.row_blocks;
+  const int32_t r0 = static_cast<int32_t>((blockIdx.x - chunk * j.row_blocks) * kRows);
+  const int32_t rows = min(q_len * group - r0, static_cast<int32_t>(kRows));
+  const int32_t c0 = static_cast<int32_t>(chunk * j.chunk);
+  if (rows <= 0 || (c0 >= kv && c0 > 0)) return;
   const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
   const bool whole = kv <= static_cast<int32_t>(j.chunk);  // no other chunk of this request
 
@@ -112,7 +116,8 @@ __global__ void __launch_bounds__(kWarps * 32)
 
   // The keys that the rows see, and the tiles of this warp among them.
   const int32_t pre = j.prefix != nullptr ? __ldg(j.prefix + n) : 0;
-  const Seen first = attn_seen(j, kv - q_len, kv, pre), last = attn_seen(j, kv - 1, kv, pre);
+  const Seen first = attn_seen(j, kv - q_len + r0 / group, kv, pre);
+  const Seen last = attn_seen(j, kv - q_len + (r0 + rows - 1) / group, kv, pre);
 
   const TileGeom geo = tile_geom<HD>(j.cache.page);
   const int32_t* table = j.table + static_cast<uint64_t>(n) * j.table_ld;
@@ -174,8 +179,8 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
     for (uint32_t i = 0; i < HD / 8u; ++i) w[i] = 0;
     if (r < rows) {
-      const uint64_t row = static_cast<uint64_t>(q0 + r / static_cast<int32_t>(j.group));
-      const uint32_t h = head * j.group + static_cast<uint32_t>(r) % j.group;
+      const uint64_t row = static_cast<uint64_t>(q0 + (r0 + r) / group);
+      const uint32_t h = head * j.group + static_cast<uint32_t>((r0 + r) % group);
       const uint4* src = reinterpret_cast<const uint4*>(j.q + row * j.ldq + h * HD + t * (HD / 4u));
 #pragma unroll
       for (uint32_t i = 0; i < HD / 32u; ++i) {
@@ -223,11 +228,11 @@ __global__ void __launch_bounds__(kWarps * 32)
       factor[nt][c] = j.scale * sc * (capped ? 1.0f : kLog2e);
       m[nt][c] = -INFINITY;
       l[nt][c] = 0.f;
-      pos[nt][c] = kv - q_len + r / static_cast<int32_t>(j.group);
+      pos[nt][c] = kv - q_len + (r0 + r) / group;
       seen[nt][c] = attn_seen(j, pos[nt][c], kv, pre);
       if (r >= rows) seen[nt][c].lo = seen[nt][c].hi = seen[nt][c].pre = 0;
       slope[nt][c] = j.slopes != nullptr && r < rows
-                         ? __ldg(j.slopes + head * j.group + static_cast<uint32_t>(r) % j.group) * kLog2e
+                         ? __ldg(j.slopes + head * j.group + static_cast<uint32_t>((r0 + r) % group)) * kLog2e
                          : 0.f;
     }
   }
@@ -589,9 +594,9 @@ __global__ void __launch_bounds__(kWarps * 32)
       sum += mw == -INFINITY ? lw : lw * part[w];
       if (mw == -INFINITY && lw != 0.f) part[w] = 1.f;
     }
-    const uint64_t row = static_cast<uint64_t>(q0 + r / static_cast<int32_t>(j.group));
-    const uint32_t h = head * j.group + static_cast<uint32_t>(r) % j.group;
-    const uint64_t cell = (static_cast<uint64_t>(blockIdx.x) * j.total_q + row) * j.heads + h;
+    const uint64_t row = static_cast<uint64_t>(q0 + (r0 + r) / group);
+    const uint32_t h = head * j.group + static_cast<uint32_t>((r0 + r) % group);
+    const uint64_t cell = (static_cast<uint64_t>(chunk) * j.total_q + row) * j.heads + h;
     const float inv = sum != 0.f ? 1.0f / sum : 0.f;
 #pragma unroll
     for (uint32_t b = 0; b < HD / 32u; ++b) {
@@ -666,8 +671,10 @@ cudaError_t launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStrea
     if (st != cudaSuccess) return st;
     set.fetch_or(uint64_t{1} << (job.device & 63u), std::memory_order_relaxed);
   }
-  k_attn_decode<HD, NT><<<dim3(chunks, job.cache.kv_heads, job.seqs), kWarps * 32,
-                          Smem<HD, NT>::kBytes, stream>>>(job, err);
+  AttnJob j = job;
+  j.row_blocks = (job.max_q * job.group + 8u * NT - 1u) / (8u * NT);
+  k_attn_decode<HD, NT><<<dim3(chunks * j.row_blocks, job.cache.kv_heads, job.seqs), kWarps * 32,
+                          Smem<HD, NT>::kBytes, stream>>>(j, err);
   return cudaSuccess;
 }
 

@@ -44,8 +44,12 @@ __host__ __device__ constexpr uint32_t k_bytes(uint32_t hd) { return (hd + 63u) 
 __host__ __device__ constexpr uint32_t v_bytes(uint32_t hd) { return 2u * hd * kRowB; }
 __host__ __device__ constexpr uint32_t tile_bytes(uint32_t hd) { return k_bytes(hd) + v_bytes(hd); }
 
-// First tile in scratch of request n (a whole warp; the same in all lanes).
+// First tile in scratch of request n (a whole warp; the same in all lanes):
+// n times the most tiles of a request where the scratch has room for that
+// (tile_stride), else the requests' tiles one after another, which every
+// block adds up from their lengths.
 __device__ __forceinline__ uint32_t first_tile(const AttnJob& j, uint32_t n) {
+  if (j.tile_stride != 0u) return n * j.tile_stride;
   uint32_t sum = 0;
   for (uint32_t i = threadIdx.x & 31u; i < n; i += 32u) {
     int32_t q0, q_len, kv;
@@ -63,6 +67,7 @@ __global__ void __launch_bounds__(256)
   constexpr uint32_t kLd = HD / 2u + 4u;  // padded row of codes in shared memory
   __shared__ __align__(16) uint8_t codes[2][kKeys * kLd];
   __shared__ uint8_t scales[2][kKeys * (HD / 32u)];
+  griddep_launch_dependents();  // k_attn_prompt may set up meanwhile
   const uint32_t n = blockIdx.z, head = blockIdx.y, k0 = blockIdx.x * kKeys;
   int32_t q0, q_len, kv;
   if (!attn_request(j, n, &q0, &q_len, &kv)) {
@@ -176,11 +181,11 @@ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) {
   return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-// Of eight pairs of weights, how many are taken on the FMA pipe.
-#ifndef POLY
-#define POLY 3u
-#endif
-constexpr uint32_t kPolyOf8 = POLY;
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // A row's raw scores to softcap log2(e) tanh(factor s / softcap).  Where all
 // of a warp's arguments are under 1/2, tanh is its power series up to x^11
@@ -306,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == 9u) {
     if (lane == 0u) {
+      griddep_wait();  // k_kv_expand's tiles
       const uint8_t* src = j.tiles + (static_cast<uint64_t>(head) * j.tiles_cap + base +
                                       static_cast<uint32_t>(c0) / kKeys) * tile_bytes(HD);
       int32_t it = 0;
@@ -328,13 +334,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 8u) {
     if (lane == 0u && count > 0) {
-      const uint32_t q_at = smem_addr(smem), k_at = smem_addr(smem + S::kK), v_at = smem_addr(smem + S::kV);
+      // Descriptors advance by their start address alone, in 16-byte units.
+      const uint64_t q_at = desc_sw128(smem_addr(smem)), k_at = desc_sw128(smem_addr(smem + S::kK));
+      const uint64_t v_at = desc_sw128(smem_addr(smem + S::kV));
       auto scores = [&](uint32_t h, uint32_t st) {
 #pragma unroll
         for (uint32_t k = 0; k < HD / 16u; ++k) {
-          const uint32_t off = (k >> 2) * (kKeys * kRowB) + 32u * (k & 3u);
-          mma_bf16(tmem + 128u * h, desc_sw128(q_at + h * k_bytes(HD) + off),
-                   desc_sw128(k_at + st * k_bytes(HD) + off), idesc_f16(128, 128), k != 0u);
+          const uint32_t off = ((k >> 2) * (kKeys * kRowB) + 32u * (k & 3u)) / 16u;
+          mma_bf16(tmem + 128u * h, q_at + (h * (k_bytes(HD) / 16u) + off),
+                   k_at + (st * (k_bytes(HD) / 16u) + off), idesc_f16(128, 128), k != 0u);
         }
         mma_commit(s_full + h);
       };
@@ -346,32 +354,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int32_t it = 0; it < count && ok; ++it) {
         const uint32_t st = static_cast<uint32_t>(it) & 1u, ph = (static_cast<uint32_t>(it) >> 1) & 1u;
+        const uint32_t nst = st ^ 1u;
         const bool more = it + 1 < count;
+        // Both tiles' arrivals first: the softmax's are then the only waits
+        // between the products.
+        ok = mbar_wait(v_full + st, ph, error_flag) &&
+             (!more || mbar_wait(k_full + nst, (static_cast<uint32_t>(it + 1) >> 1) & 1u, error_flag));
         for (uint32_t h = 0; h < halves && ok; ++h) {
-          if (h == 0u) ok = mbar_wait(v_full + st, ph, error_flag);
 #pragma unroll
-          for (uint32_t k = 0; k < kKeys / 16u && ok; ++k) {
+          for (uint32_t k = 0; k < kKeys / 16u; ++k) {
             if ((k & 3u) == 0u) {  // 64 keys' weights
               ok = mbar_wait(p_full + 2u * h + (k >> 2), static_cast<uint32_t>(it) & 1u, error_flag);
               if (!ok) break;
               tc_fence_after();
             }
             mma_bf16_ts(tmem + 256u + 128u * h, tmem + 128u * h + 8u * k,
-                        desc_sw128(v_at + st * v_bytes(HD) + (k >> 2) * (HD * kRowB) + 32u * (k & 3u)),
+                        v_at + (st * v_bytes(HD) + (k >> 2) * (HD * kRowB) + 32u * (k & 3u)) / 16u,
                         idesc_f16(128, HD), it != 0 || k != 0u);
           }
           if (!ok) break;
           if (more) {
-            const uint32_t nst = static_cast<uint32_t>(it + 1) & 1u;
-            ok = h != 0u || mbar_wait(k_full + nst, (static_cast<uint32_t>(it + 1) >> 1) & 1u, error_flag);
-            if (!ok) break;
             scores(h, nst);
           } else {
             mma_commit(o_full + h);
           }
         }
         mma_commit(v_empty + st);
-        if (more) mma_commit(k_empty + (static_cast<uint32_t>(it + 1) & 1u));
+        if (more) mma_commit(k_empty + nst);
       }
     }
   }
@@ -390,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // [2^13, 2^14) and signed so that the scores' factor is not negative.
       const uint16_t* src = j.q + row * j.ldq + static_cast<uint64_t>(qh) * HD;
       uint32_t top = 0;
-#pragma unroll
+#pragma unroll 4
       for (uint32_t i = 0; i < HD / 8u; ++i) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -406,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                (j.softcap != 0.f ? 1.0f : kLog2e);
       factor = fmaxf(factor, 1.2e-38f);  // times a masked score's -inf is no NaN
       uint8_t* dst = smem + h * k_bytes(HD) + in_half * kRowB;
-#pragma unroll
+#pragma unroll 4
       for (uint32_t i = 0; i < HD / 8u; ++i) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -472,28 +481,37 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!((k >= a && k < b) || k < cc)) s[c][i] = 0xFF800000u;
             }
         }
-        float top[4];
+        float top[8];
 #pragma unroll
-        for (uint32_t c = 0; c < 4u; ++c) {
-          top[c] = fmaxf(at(c, 0), at(c, 1));
-#pragma unroll
-          for (uint32_t i = 2; i < 32u; i += 2u) top[c] = fmaxf(fmaxf(top[c], at(c, i)), at(c, i + 1u));
+        for (uint32_t c = 0; c < 8u; ++c) {
+          const uint32_t at0 = 16u * (c & 1u);
+          top[c] = max3(at(c >> 1, at0), at(c >> 1, at0 + 1u), at(c >> 1, at0 + 2u));
         }
-        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+#pragma unroll
+        for (uint32_t i = 3; i < 15u; i += 2u)
+#pragma unroll
+          for (uint32_t c = 0; c < 8u; ++c) {
+            const uint32_t at0 = 16u * (c & 1u) + i;
+            top[c] = max3(top[c], at(c >> 1, at0), at(c >> 1, at0 + 1u));
+          }
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) top[c] = fmaxf(top[c], at(c >> 1, 16u * (c & 1u) + 15u));
+        const float high = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]),
+                                fmaxf(top[6], top[7])) * scale;
         const bool moves = high > m + kLazy;
         if (__any_sync(0xFFFFFFFFu, moves)) {
           const float keep = moves ? ex2(m - high) : 1.0f;
           if (moves) m = high;
           l *= keep;
           if (it != 0) {
-#pragma unroll
-            for (uint32_t c = 0; c < HD / 32u; ++c) {
-              uint32_t o[32];
-              tmem_ld32(t_o + 32u * c, o);
+#pragma unroll 1
+            for (uint32_t c = 0; c < HD / 16u; ++c) {
+              uint32_t o[16];
+              tmem_ld16(t_o + 16u * c, o);
               tmem_wait_ld();
 #pragma unroll
-              for (uint32_t i = 0; i < 32u; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-              tmem_st32(t_o + 32u * c, o);
+              for (uint32_t i = 0; i < 16u; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+              tmem_st16(t_o + 16u * c, o);
             }
           }
         }
@@ -506,14 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (uint32_t i = 0; i < 32u; ++i) {
             const uint64_t x = fma_2(pair(2u * c + i / 16u, 2u * (i % 16u)), scale2x, shift2x);
-            // kPolyOf8 of eight pairs on the FMA pipe, the others on MUFU.
-            float2 e;
-            if (((i * kPolyOf8) & 7u) < kPolyOf8) {
-              e = ex2_fma(x);
-            } else {
-              const float2 v = unpack2(x);
-              e = make_float2(ex2(v.x), ex2(v.y));
-            }
+            const float2 v = unpack2(x), e = make_float2(ex2(v.x), ex2(v.y));
             sum[i & 3u] = add_2(sum[i & 3u], pack2(e.x, e.y));
             p[i] = half2_bits(__floats2half2_rn(e.x, e.y));
           }
@@ -531,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (odd && (seen.lo < seen.hi || seen.pre > 0)) l = NAN;
         const float inv = l != 0.f ? 1.0f / l : 0.f;
         const uint64_t cell = (static_cast<uint64_t>(chunk) * j.total_q + row) * j.heads + qh;
-#pragma unroll
+#pragma unroll 1
         for (uint32_t c = 0; c < HD / 32u; ++c) {
           uint32_t o[32];
           __syncwarp();
@@ -584,15 +595,33 @@ int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stre
     k_kv_expand<HD><<<dim3(key_tiles, job.cache.kv_heads, job.seqs), 256, 0, stream>>>(job, err);
     ++n;
   }
-  k_attn_prompt<HD><<<dim3(chunks * job.cache.kv_heads, q_tiles, job.seqs), kThreads,
-                      Smem<HD>::kBytes, stream>>>(job, err);
+  // Its blocks may start, load Q and set up while k_kv_expand still runs.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(chunks * job.cache.kv_heads, q_tiles, job.seqs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Smem<HD>::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = key_tiles != 0u ? 1u : 0u;
+  if (cudaLaunchKernelEx(&cfg, k_attn_prompt<HD>, job, err) != cudaSuccess) return -1;
   return n;
 }
 
 }  // namespace
 
-uint64_t attn_prompt_tiles(const AttnJob& job, uint64_t total_kv) {
-  return total_kv / kKeys + job.seqs;
+uint64_t attn_prompt_tiles(const AttnJob& job, uint64_t total_kv, uint32_t* stride) {
+  // Tiles at a fixed stride a request cost no sum over the requests before
+  // it (64 requests: 1.5 us a block); requests of very different lengths
+  // would waste scratch, so only up to twice what they need.
+  const uint64_t tight = total_kv / kKeys + job.seqs;
+  const uint64_t most = (job.max_kv + kKeys - 1u) / kKeys;
+  const uint64_t even = most * job.seqs;
+  const bool use = even <= 2u * tight && even <= 0xFFFFFFFFull;
+  *stride = use ? static_cast<uint32_t>(most) : 0u;
+  return use ? even : tight;
 }
 uint64_t attn_prompt_tile_bytes(const AttnJob& job) { return tile_bytes(job.cache.hd); }
 

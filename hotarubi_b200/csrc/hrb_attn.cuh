@@ -47,27 +47,6 @@ __device__ __forceinline__ uint64_t fma_2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// 2^x of a pair for x <= 8 on the FMA pipe (the MUFU pipe gives 16 a clock
-// and SM): x = i + f with i = round(x), f in [-1/2, 1/2]; 2^f by the degree 4
-// polynomial of least largest relative error there (2.6e-6, found by Remez'
-// exchange); i added to the exponent.  x under -125 gives about 2^-125, far
-// under FP16's range and what counts in a sum of FP32; NaN is not kept.
-__device__ __forceinline__ float2 ex2_fma(uint64_t x) {
-  const float2 v = unpack2(x);
-  const uint64_t y = pack2(fmaxf(v.x, -125.f), fmaxf(v.y, -125.f));
-  const uint64_t magic = pack2(12582912.f, 12582912.f);  // 1.5 * 2^23
-  const uint64_t t = add_2(y, magic);
-  const uint64_t i = add_2(t, pack2(-12582912.f, -12582912.f));
-  const uint64_t f = fma_2(i, pack2(-1.f, -1.f), y);
-  uint64_t r = fma_2(f, pack2(0.0095701f, 0.0095701f), pack2(0.05591786f, 0.05591786f));
-  r = fma_2(r, f, pack2(0.24024745f, 0.24024745f));
-  r = fma_2(r, f, pack2(0.69312181f, 0.69312181f));
-  r = fma_2(r, f, pack2(0.99999926f, 0.99999926f));
-  const float2 p = unpack2(r), e = unpack2(t);
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(e.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(e.y) << 23)));
-}
-
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }

@@ -67,11 +67,12 @@ struct AttnJob {
   // Keys a block of the split kernels takes, and the chunks' results: rows
   // of (m, l) and O, [chunk][total_q][heads] and the same by [hd].
   uint32_t chunk;
+  uint32_t row_blocks;    // of a request, in the decoding kernel
   float2* part_ml;
   float* part_o;
   // The prompt kernel's decoded keys: [kv_heads][tiles_cap] tiles.
   uint8_t* tiles;
-  uint32_t tiles_cap;
+  uint32_t tiles_cap, tile_stride;
 };
 
 // Rows [q0, q0 + q_len) and keys of request n, held to what the descriptor
@@ -130,7 +131,7 @@ int launch_attn_decode(const AttnJob& job, uint32_t* error_flag, cudaStream_t st
 void launch_attn_join(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
 
 // Any number of rows.  Scratch for attn_prompt_tiles tiles a key/value head.
-uint64_t attn_prompt_tiles(const AttnJob& job, uint64_t total_kv);
+uint64_t attn_prompt_tiles(const AttnJob& job, uint64_t total_kv, uint32_t* stride);
 uint64_t attn_prompt_tile_bytes(const AttnJob& job);
 uint32_t attn_prompt_chunk(const AttnJob& job, int sm_count);
 int launch_attn_prompt(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);

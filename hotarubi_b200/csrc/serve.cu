@@ -5,6 +5,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <cstdlib>
 
 #include "hrb_gemm.h"
 #include "hrb_kernels.cuh"
@@ -160,15 +161,21 @@ hrb::AttnJob attn_job(const hrb_ctx* ctx, const hrb_attn_desc* d) {
 
 uint64_t up256(uint64_t x) { return (x + 255u) / 256u * 256u; }
 
+bool decoding(const hrb::AttnJob& j) {
+  static const char* e = std::getenv("HRB_DEC");
+  const uint32_t lim = e ? atoi(e) : hrb::kDecodeRows;
+  return j.max_q * j.group <= lim;
+}
+
 // Fills in how the call is split and where its scratch lies from `base`
 // (null: to learn the size).  Returns the scratch bytes.
 uint64_t attn_plan(const hrb_ctx* ctx, const hrb_attn_desc* d, hrb::AttnJob* j, uint8_t* base) {
   const uint64_t total_kv = d->total_kv != 0u ? d->total_kv : uint64_t{d->seqs} * d->max_kv;
   uint64_t at = 0;
-  if (j->max_q * j->group <= hrb::kDecodeRows) {
+  if (decoding(*j)) {
     j->chunk = hrb::attn_decode_chunk(*j, total_kv, hrb::ctx_sm_count(ctx));
   } else {
-    const uint64_t tiles = hrb::attn_prompt_tiles(*j, total_kv);
+    const uint64_t tiles = hrb::attn_prompt_tiles(*j, total_kv, &j->tile_stride);
     j->tiles_cap = static_cast<uint32_t>(tiles < 0xFFFFFFFFull ? tiles : 0xFFFFFFFFull);
     j->tiles = base;
     at = up256(tiles * j->cache.kv_heads * hrb::attn_prompt_tile_bytes(*j));
@@ -363,7 +370,7 @@ hrb_status hrb_attention(hrb_ctx* ctx, const hrb_attn_desc* d, void* stream) {
     attn_plan(ctx, d, &j, static_cast<uint8_t*>(base));
   }
   cudaStream_t s = hrb::ctx_stream(ctx, stream);
-  const int n = j.max_q * j.group <= hrb::kDecodeRows
+  const int n = decoding(j)
                     ? hrb::launch_attn_decode(j, hrb::ctx_error_word(ctx), s)
                     : hrb::launch_attn_prompt(j, hrb::ctx_error_word(ctx), s);
   if (n < 0) return refuse(ctx, HRB_ECUDA, "hrb_attention: %s", cudaGetErrorString(cudaGetLastError()));
