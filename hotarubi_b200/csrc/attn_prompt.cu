@@ -36,7 +36,6 @@ using namespace sm100;
 
 constexpr uint32_t kKeys = 128;      // keys a tile
 constexpr uint32_t kHalf = 128;      // rows a half
-constexpr uint32_t kThreads = 384;    // three warpgroups: warps 10 and 11 only give up registers
 constexpr uint32_t kRowB = 128;      // bytes of a swizzled row
 
 // Bytes of a tile's parts: K in chunks of 64 dims, V^T in chunks of 64 keys.
@@ -163,16 +162,24 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template <uint32_t HD>
-struct Smem {
-  static constexpr uint32_t kQ = 2u * k_bytes(HD);
-  static constexpr uint32_t kK = kQ;                         // two K stages
-  static constexpr uint32_t kV = kK + 2u * k_bytes(HD);      // two V^T stages
-  static constexpr uint32_t kBars = kV + 2u * v_bytes(HD);
+// HV halves of 128 rows.  Two share their tiles and fill an SM: 384 threads
+// (three warpgroups, warps 10 and 11 only give up registers), all of TMEM.
+// One is half of that, two blocks an SM: for short histories, where a block
+// is mostly set-up, Q and output.
+template <uint32_t HD, uint32_t HV>
+struct Cfg {
+  static constexpr uint32_t kThreads = HV * 128u + 128u;
+  static constexpr uint32_t kStages = HV == 2u || HD <= 64u ? 2u : 1u;  // of K and of V^T
+  static constexpr uint32_t kO = HV * 128u;                    // TMEM column of O (S at 0)
+  static constexpr uint32_t kTmem = HV * 256u;
+  static constexpr uint32_t kQ = HV * k_bytes(HD);
+  static constexpr uint32_t kK = kQ;
+  static constexpr uint32_t kV = kK + kStages * k_bytes(HD);
+  static constexpr uint32_t kBars = kV + kStages * v_bytes(HD);
   static constexpr uint32_t kUsed = kBars + 144u;
-  // Over half an SM's shared memory: one block an SM, for its 512 columns of
-  // TMEM.
-  static constexpr uint32_t kBytes = (kUsed > 120u * 1024u ? kUsed : 120u * 1024u) + 1024u;
+  // No more blocks an SM than its 512 columns of TMEM hold.
+  static constexpr uint32_t kLeast = (HV == 2u ? 120u : 78u) * 1024u;
+  static constexpr uint32_t kBytes = (kUsed > kLeast ? kUsed : kLeast) + 1024u;
 };
 
 // Instruction descriptor of kind::f16 with FP16 A and B, FP32 D, K-major
@@ -237,10 +244,12 @@ __device__ __forceinline__ void cap_scores(const AttnJob& j, float factor, uint3
   }
 }
 
-template <uint32_t HD>
-__global__ void __launch_bounds__(kThreads, 1)
+template <uint32_t HD, uint32_t HV>
+__global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
     k_attn_prompt(const AttnJob j, uint32_t* __restrict__ error_flag) {
-  using S = Smem<HD>;
+  using S = Cfg<HD, HV>;
+  constexpr uint32_t kNs = S::kStages;
+  constexpr int32_t kBlockRows = static_cast<int32_t>(HV * kHalf);
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
@@ -256,17 +265,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!attn_request(j, n, &q0, &q_len, &kv)) return;  // k_kv_expand reports it
   const int32_t rows = q_len * static_cast<int32_t>(j.group);
   // The last rows see the most keys: they start first.
-  const int32_t q_tiles = (rows + 2 * static_cast<int32_t>(kHalf) - 1) / (2 * static_cast<int32_t>(kHalf));
+  const int32_t q_tiles = (rows + kBlockRows - 1) / kBlockRows;
   if (static_cast<int32_t>(blockIdx.y) >= q_tiles) return;
-  const int32_t r0 = (q_tiles - 1 - static_cast<int32_t>(blockIdx.y)) * 2 * static_cast<int32_t>(kHalf);
-  const int32_t r1 = min(rows, r0 + 2 * static_cast<int32_t>(kHalf));
+  const int32_t r0 = (q_tiles - 1 - static_cast<int32_t>(blockIdx.y)) * kBlockRows;
+  const int32_t r1 = min(rows, r0 + kBlockRows);
   const int32_t c0 = static_cast<int32_t>(chunk * j.chunk);
   const bool whole = kv <= static_cast<int32_t>(j.chunk);
   if (c0 >= kv && c0 > 0) return;
   const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
   const uint32_t base = first_tile(j, n);
   if (base + (static_cast<uint32_t>(kv) + kKeys - 1u) / kKeys > j.tiles_cap) return;  // reported too
-  const uint32_t halves = r1 - r0 > static_cast<int32_t>(kHalf) ? 2u : 1u;
+  const uint32_t halves = HV == 2u && r1 - r0 > static_cast<int32_t>(kHalf) ? 2u : 1u;
 
   // The tiles that some row of the block sees: numbers 0 .. gap - 1 and
   // resume .. of the chunk's, `count` in all.
@@ -282,8 +291,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int32_t count = gap + end - resume;
   auto tile_at = [&](int32_t it) { return it < gap ? it : it - gap + resume; };
 
+  // A softmax thread's row (its half's thread number) and its part of Q, on
+  // their way while the block sets up.
+  const uint32_t in_half = threadIdx.x & (kHalf - 1u);
+  const int32_t r = r0 + static_cast<int32_t>(threadIdx.x);
+  const bool mine = warp < 4u * HV && r < r1;
+  const uint64_t row = static_cast<uint64_t>(q0 + (mine ? r : r0) / group);
+  const uint32_t qh = head * j.group + static_cast<uint32_t>((mine ? r : r0) % group);
+  uint4 q_row[HD / 8u];
+#pragma unroll
+  for (uint32_t i = 0; i < HD / 8u; ++i) {
+    q_row[i] = mine ? __ldg(reinterpret_cast<const uint4*>(j.q + row * j.ldq + static_cast<uint64_t>(qh) * HD) + i)
+                    : make_uint4(0, 0, 0, 0);
+  }
+
   if (threadIdx.x == 0u) {
-    mbar_init(q_full, 256);
+    mbar_init(q_full, HV * 128u);
     for (uint32_t i = 0; i < 2u; ++i) {
       mbar_init(k_full + i, 1);
       mbar_init(k_empty + i, 1);
@@ -296,8 +319,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_barrier_init();
   }
-  if (warp == 8u) {
-    tmem_alloc(tmem_slot, 512);
+  if (warp == 4u * HV) {
+    tmem_alloc(tmem_slot, S::kTmem);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -305,34 +328,39 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // 384 threads x 168 registers at launch = 256 x 224 + 128 x 56: a softmax
-  // thread holds a row's 128 scores.
-  if (warp >= 8u) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  if (warp == 9u) {
+  // A softmax thread holds a row's 128 scores.  Registers at launch: 384 x
+  // 168 = 256 x 224 + 128 x 56 (HV 2), 256 x 128 = 128 x 208 + 128 x 48.
+  if (warp >= 4u * HV) {
+    if constexpr (HV == 2u) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    }
+  if (warp == 4u * HV + 1u) {
     if (lane == 0u) {
       griddep_wait();  // k_kv_expand's tiles
       const uint8_t* src = j.tiles + (static_cast<uint64_t>(head) * j.tiles_cap + base +
                                       static_cast<uint32_t>(c0) / kKeys) * tile_bytes(HD);
       int32_t it = 0;
       for (; it < count; ++it) {
-        const uint32_t st = static_cast<uint32_t>(it) & 1u, ph = (static_cast<uint32_t>(it) >> 1) & 1u;
+        const uint32_t st = static_cast<uint32_t>(it) % kNs, ph = (static_cast<uint32_t>(it) / kNs) & 1u;
+        const bool wait = it >= static_cast<int32_t>(kNs);
         const uint8_t* tile = src + static_cast<uint64_t>(tile_at(it)) * tile_bytes(HD);
-        if (it >= 2 && !mbar_wait(k_empty + st, ph ^ 1u, error_flag)) break;
+        if (wait && !mbar_wait(k_empty + st, ph ^ 1u, error_flag)) break;
         mbar_arrive_expect_tx(k_full + st, k_bytes(HD));
         bulk_g2s(smem + S::kK + st * k_bytes(HD), tile, k_bytes(HD), k_full + st);
-        if (it >= 2 && !mbar_wait(v_empty + st, ph ^ 1u, error_flag)) break;
+        if (wait && !mbar_wait(v_empty + st, ph ^ 1u, error_flag)) break;
         mbar_arrive_expect_tx(v_full + st, v_bytes(HD));
         bulk_g2s(smem + S::kV + st * v_bytes(HD), tile + k_bytes(HD), v_bytes(HD), v_full + st);
       }
       // Nothing of this block's may still be arriving when it ends.
-      for (int32_t w = max(it - 2, 0); w < min(it + 1, count); ++w) {
-        const uint32_t st = static_cast<uint32_t>(w) & 1u, ph = (static_cast<uint32_t>(w) >> 1) & 1u;
+      for (int32_t w = max(it - static_cast<int32_t>(kNs), 0); w < min(it + 1, count); ++w) {
+        const uint32_t st = static_cast<uint32_t>(w) % kNs, ph = (static_cast<uint32_t>(w) / kNs) & 1u;
         if (w < it && !mbar_wait(v_full + st, ph, error_flag)) break;
         if (w == it && !mbar_wait(k_full + st, ph, error_flag, 1000u)) break;
       }
     }
-  } else if (warp == 8u) {
+  } else if (warp == 4u * HV) {
     if (lane == 0u && count > 0) {
       // Descriptors advance by their start address alone, in 16-byte units.
       const uint64_t q_at = desc_sw128(smem_addr(smem)), k_at = desc_sw128(smem_addr(smem + S::kK));
@@ -353,13 +381,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit(k_empty);
       }
       for (int32_t it = 0; it < count && ok; ++it) {
-        const uint32_t st = static_cast<uint32_t>(it) & 1u, ph = (static_cast<uint32_t>(it) >> 1) & 1u;
-        const uint32_t nst = st ^ 1u;
+        const uint32_t st = static_cast<uint32_t>(it) % kNs, ph = (static_cast<uint32_t>(it) / kNs) & 1u;
+        const uint32_t nst = static_cast<uint32_t>(it + 1) % kNs;
         const bool more = it + 1 < count;
         // Both tiles' arrivals first: the softmax's are then the only waits
         // between the products.
         ok = mbar_wait(v_full + st, ph, error_flag) &&
-             (!more || mbar_wait(k_full + nst, (static_cast<uint32_t>(it + 1) >> 1) & 1u, error_flag));
+             (!more || mbar_wait(k_full + nst, (static_cast<uint32_t>(it + 1) / kNs) & 1u, error_flag));
         for (uint32_t h = 0; h < halves && ok; ++h) {
 #pragma unroll
           for (uint32_t k = 0; k < kKeys / 16u; ++k) {
@@ -368,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!ok) break;
               tc_fence_after();
             }
-            mma_bf16_ts(tmem + 256u + 128u * h, tmem + 128u * h + 8u * k,
+            mma_bf16_ts(tmem + S::kO + 128u * h, tmem + 128u * h + 8u * k,
                         v_at + (st * v_bytes(HD) + (k >> 2) * (HD * kRowB) + 32u * (k & 3u)) / 16u,
                         idesc_f16(128, HD), it != 0 || k != 0u);
           }
@@ -385,46 +413,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if constexpr (HV == 2u) {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    }
     const uint32_t h = warp >> 2;
-    const uint32_t in_half = (warp & 3u) * 32u + lane;
-    const int32_t r = r0 + static_cast<int32_t>(h * kHalf + in_half);
-    const bool mine = r < r1;
-    const uint64_t row = static_cast<uint64_t>(q0 + (mine ? r : r0) / group);
-    const uint32_t qh = head * j.group + static_cast<uint32_t>((mine ? r : r0) % group);
     float factor;
     bool odd;  // Inf or NaN in the row of Q: its outputs are NaN
     {
       // The row of Q as FP16, scaled so that its largest value is in
       // [2^13, 2^14) and signed so that the scores' factor is not negative.
-      const uint16_t* src = j.q + row * j.ldq + static_cast<uint64_t>(qh) * HD;
       uint32_t top = 0;
-#pragma unroll 4
+#pragma unroll
       for (uint32_t i = 0; i < HD / 8u; ++i) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t w[4] = {q_row[i].x, q_row[i].y, q_row[i].z, q_row[i].w};
 #pragma unroll
         for (uint32_t d = 0; d < 4u; ++d) top = max(top, max(w[d] & 0x7FFFu, (w[d] >> 16) & 0x7FFFu));
       }
       odd = top >= 0x7F80u;
       const int32_t e = min(max(static_cast<int32_t>(top >> 7), 27), 254) - 127;
       float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
-      if (!mine) up = 0.f;
       if (j.scale < 0.f) up = -up;
       factor = fabsf(j.scale) * __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23) *
                (j.softcap != 0.f ? 1.0f : kLog2e);
       factor = fmaxf(factor, 1.2e-38f);  // times a masked score's -inf is no NaN
       uint8_t* dst = smem + h * k_bytes(HD) + in_half * kRowB;
-#pragma unroll 4
+#pragma unroll
       for (uint32_t i = 0; i < HD / 8u; ++i) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t w[4] = {q_row[i].x, q_row[i].y, q_row[i].z, q_row[i].w};
         uint32_t o[4];
 #pragma unroll
         for (uint32_t d = 0; d < 4u; ++d) {
-          o[d] = mine ? half2_bits(__floats2half2_rn(__uint_as_float(w[d] << 16) * up,
-                                                     __uint_as_float(w[d] & 0xFFFF0000u) * up))
-                      : 0u;
+          o[d] = half2_bits(__floats2half2_rn(__uint_as_float(w[d] << 16) * up,
+                                              __uint_as_float(w[d] & 0xFFFF0000u) * up));
         }
         *reinterpret_cast<uint4*>(dst + (i >> 3) * (kKeys * kRowB) + (((i & 7u) ^ (in_half & 7u)) * 16u)) =
             make_uint4(o[0], o[1], o[2], o[3]);
@@ -437,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!mine) seen.lo = seen.hi = seen.pre = 0;
     const float slope = j.slopes != nullptr ? __ldg(j.slopes + qh) * kLog2e : 0.f;
     const uint32_t lanes = ((warp & 3u) * 32u) << 16;
-    const uint32_t t_s = tmem + lanes + 128u * h, t_o = tmem + lanes + 256u + 128u * h;
+    const uint32_t t_s = tmem + lanes + 128u * h, t_o = tmem + lanes + S::kO + 128u * h;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     if (h < halves) {
@@ -575,21 +597,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8u) tmem_dealloc(tmem, 512);
+  if (warp == 4u * HV) tmem_dealloc(tmem, S::kTmem);
 }
 
-template <uint32_t HD>
+template <uint32_t HD, uint32_t HV>
 int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stream) {
+  using S = Cfg<HD, HV>;
   static std::atomic<uint64_t> set{0};  // devices whose limit is raised
   if (((set.load(std::memory_order_relaxed) >> (job.device & 63u)) & 1u) == 0u || job.device > 63u) {
-    if (cudaFuncSetAttribute(k_attn_prompt<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Smem<HD>::kBytes) != cudaSuccess) {
+    if (cudaFuncSetAttribute(k_attn_prompt<HD, HV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             S::kBytes) != cudaSuccess) {
       return -1;
     }
     set.fetch_or(uint64_t{1} << (job.device & 63u), std::memory_order_relaxed);
   }
   const uint32_t key_tiles = (job.max_kv + kKeys - 1u) / kKeys;
-  const uint32_t q_tiles = (job.max_q * job.group + 2u * kHalf - 1u) / (2u * kHalf);
+  const uint32_t q_tiles = (job.max_q * job.group + HV * kHalf - 1u) / (HV * kHalf);
   int n = 1;
   if (key_tiles != 0u) {
     k_kv_expand<HD><<<dim3(key_tiles, job.cache.kv_heads, job.seqs), 256, 0, stream>>>(job, err);
@@ -598,16 +621,27 @@ int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stre
   // Its blocks may start, load Q and set up while k_kv_expand still runs.
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(chunks * job.cache.kv_heads, q_tiles, job.seqs);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Smem<HD>::kBytes;
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = key_tiles != 0u ? 1u : 0u;
-  if (cudaLaunchKernelEx(&cfg, k_attn_prompt<HD>, job, err) != cudaSuccess) return -1;
+  if (cudaLaunchKernelEx(&cfg, k_attn_prompt<HD, HV>, job, err) != cudaSuccess) return -1;
   return n;
+}
+
+template <uint32_t HD>
+int launch_hd(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stream) {
+  // Short histories of small heads: 32 prompts of 141 tokens (15/5 heads of
+  // 64) 42.7 us with two halves a block, 35.2 with one; one of 512 20.9 and
+  // 16.9.  At hd 128 one half a block is slower throughout (98.6 and 103.2 us
+  // for 32 of 141 with 32/8 heads), as is a long history (43.4 and 47.1 us for
+  // 200 rows over 8000 keys at hd 64).
+  return HD <= 64u && job.max_kv <= 1024u ? launch<HD, 1>(job, chunks, err, stream)
+                                          : launch<HD, 2>(job, chunks, err, stream);
 }
 
 }  // namespace
@@ -641,10 +675,10 @@ int launch_attn_prompt(const AttnJob& job, uint32_t* error_flag, cudaStream_t st
   const uint32_t chunks = job.max_kv == 0u ? 1u : (job.max_kv + job.chunk - 1u) / job.chunk;
   int n;
   switch (job.cache.hd) {
-    case 32: n = launch<32>(job, chunks, error_flag, stream); break;
-    case 64: n = launch<64>(job, chunks, error_flag, stream); break;
-    case 96: n = launch<96>(job, chunks, error_flag, stream); break;
-    default: n = launch<128>(job, chunks, error_flag, stream); break;
+    case 32: n = launch_hd<32>(job, chunks, error_flag, stream); break;
+    case 64: n = launch_hd<64>(job, chunks, error_flag, stream); break;
+    case 96: n = launch_hd<96>(job, chunks, error_flag, stream); break;
+    default: n = launch_hd<128>(job, chunks, error_flag, stream); break;
   }
   if (n < 0 || chunks == 1u) return n;
   launch_attn_join(job, error_flag, stream);
