@@ -83,7 +83,7 @@ struct Smem {
 };
 
 template <uint32_t HD, uint32_t NT>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     k_attn_decode(const AttnJob j, uint32_t* __restrict__ error_flag) {
   using S = Smem<HD, NT>;
   constexpr uint32_t kSteps = HD / 16u;           // MMAs along dims; m16 tiles of dims
@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     page_b = page_a;
     if (j.cache.page == 16u) page_b = k + 16 < kv ? __ldg(table + ((k + 16) >> 4)) : -2;
   };
+  const uint8_t* const head_data = j.cache.data + static_cast<uint64_t>(head) * j.cache.record;
   // -2: no keys there; other values outside the cache read as zeros.
   auto issue = [&](int32_t number, uint32_t stage) {
     const int32_t i = static_cast<int32_t>(warp) + number * static_cast<int32_t>(kWarps);
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int32_t pa = __shfl_sync(0xFFFFFFFFu, page_a, number - base);
     const int32_t pb = __shfl_sync(0xFFFFFFFFu, page_b, number - base);
     const int32_t page = lane == 1u && j.cache.page == 16u ? pb : pa;
-    const bool there = page >= 0 && static_cast<uint32_t>(page) < j.cache.pages;
+    const bool there = static_cast<uint32_t>(page) < j.cache.pages;
     uint8_t* dst = ring + stage * S::kStageBytes;
     uint32_t bytes, from;
     if (j.cache.page <= 32u) {
@@ -154,13 +155,16 @@ __global__ void __launch_bounds__(kWarps * 32)
              (scales ? kv_kscales(j.cache) + in * (HD / 32u) : in * (HD / 2u));
       dst += (lane >= 2u ? geo.v : 0u) + (scales ? geo.ks : 0u);
     }
-    const bool copy = lane < copies && there;
-    const uint32_t total = __reduce_add_sync(0xFFFFFFFFu, copy ? bytes : 0u);
+    const uint32_t in_a = static_cast<uint32_t>(pa) < j.cache.pages ? 1u : 0u;
+    const uint32_t in_b = static_cast<uint32_t>(pb) < j.cache.pages ? 1u : 0u;
+    // Two records, one, or a tile's part of a larger one.
+    const uint32_t total = j.cache.page == 16u ? (in_a + in_b) * j.cache.record
+                                               : in_a * S::kStageBytes;
     if (lane == 0u) mbar_arrive_expect_tx(full + stage, total);
     __syncwarp();
-    if (copy) {
-      bulk_g2s(dst, kv_record(j.cache, static_cast<uint32_t>(page), head) + from, bytes,
-               full + stage);
+    if (lane < copies && there) {
+      bulk_g2s(dst, head_data + static_cast<uint64_t>(static_cast<uint32_t>(page)) * j.cache.page_stride + from,
+               bytes, full + stage);
     }
   };
 
@@ -199,7 +203,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
     const int32_t e = min(max(static_cast<int32_t>(top >> 7), 27), 254) - 127;
-    const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
+    float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
+    if (j.scale < 0.f) up = -up;  // the scores' factor is not negative
     row_scale[nt] = __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
     if (top >= 0x7F80u) row_scale[nt] = NAN;  // Inf or NaN in the row
 #pragma unroll
@@ -214,6 +219,10 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
   }
   if constexpr (NT > 2u) __syncthreads();
+  // Lanes t = 2, 3 take the two keys of a pair the other way round, in V and
+  // in P: the four t of a load are then in different banks at hd 64, and two
+  // share one instead of four at hd 128.
+  const uint32_t swap = t >> 1, order = swap != 0u ? 0x1032u : 0x3210u;
   // The lane's two rows of each n tile in S^T and O^T: 8 nt + 2 t + {0, 1}.
   float factor[NT][2], m[NT][2], l[NT][2], slope[NT][2];
   Seen seen[NT][2];
@@ -225,7 +234,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (uint32_t c = 0; c < 2u; ++c) {
       const int32_t r = static_cast<int32_t>(8u * nt + 2u * t + c);
       const float sc = __shfl_sync(0xFFFFFFFFu, row_scale[nt], (2u * t + c) * 4u);
-      factor[nt][c] = j.scale * sc * (capped ? 1.0f : kLog2e);
+      factor[nt][c] = fmaxf(fabsf(j.scale) * sc, 1.2e-38f) * (capped ? 1.0f : kLog2e);
+      if (sc != sc) factor[nt][c] = sc;
       m[nt][c] = -INFINITY;
       l[nt][c] = 0.f;
       pos[nt][c] = kv - q_len + (r0 + r) / group;
@@ -378,27 +388,20 @@ __global__ void __launch_bounds__(kWarps * 32)
     // a request's last for single tokens) skip the masks.
     const int32_t k1 = k0 + static_cast<int32_t>(kTile);
     const bool clear = (k0 >= last.lo && k1 <= first.hi) || k1 <= first.pre;
-#pragma unroll
-    for (uint32_t nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (uint32_t c = 0; c < 8u; ++c) s[nt][c / 4u][c & 3u] *= factor[nt][c & 1u];
-    if (capped) {
+    const bool shaped = capped || j.slopes != nullptr;
+    if (shaped) {
       // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2x / cap)))
 #pragma unroll
       for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (uint32_t c = 0; c < 8u; ++c) {
-          const float y = ex2(s[nt][c / 4u][c & 3u] * j.cap_in);
-          s[nt][c / 4u][c & 3u] = j.cap_out * (1.0f - __fdividef(2.0f, 1.0f + y));
-        }
-    }
-    if (j.slopes != nullptr) {
-#pragma unroll
-      for (uint32_t nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (uint32_t c = 0; c < 8u; ++c) {
+          float x = s[nt][c / 4u][c & 3u] * factor[nt][c & 1u];
+          if (capped) x = j.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(x * j.cap_in)));
           const int32_t k = k0 + static_cast<int32_t>(16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g);
-          s[nt][c / 4u][c & 3u] -= slope[nt][c & 1u] * fabsf(static_cast<float>(pos[nt][c & 1u] - k));
+          if (j.slopes != nullptr) {
+            x -= slope[nt][c & 1u] * fabsf(static_cast<float>(pos[nt][c & 1u] - k));
+          }
+          s[nt][c / 4u][c & 3u] = x;
         }
     }
     if (!clear) {
@@ -417,7 +420,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (uint32_t nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (uint32_t c = 0; c < 2u; ++c) {
-        top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][c + 2u]), fmaxf(s[nt][1][c], s[nt][1][c + 2u]));
+        top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][c + 2u]), fmaxf(s[nt][1][c], s[nt][1][c + 2u])) *
+                     (shaped ? 1.0f : factor[nt][c]);
         moves |= top[nt][c] > m[nt][c] + kLazy;
       }
     }
@@ -446,16 +450,18 @@ __global__ void __launch_bounds__(kWarps * 32)
     uint32_t p[NT][2][2];
 #pragma unroll
     for (uint32_t nt = 0; nt < NT; ++nt) {
-      const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
-      const float m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+      const float m0 = m[nt][0] == -INFINITY ? 0.f : -m[nt][0];
+      const float m1 = m[nt][1] == -INFINITY ? 0.f : -m[nt][1];
+      const float f0 = shaped ? 1.0f : factor[nt][0], f1 = shaped ? 1.0f : factor[nt][1];
 #pragma unroll
       for (uint32_t hf = 0; hf < 2u; ++hf) {
 #pragma unroll
         for (uint32_t r = 0; r < 2u; ++r) {
-          const float x = ex2(s[nt][hf][2u * r] - m0), y = ex2(s[nt][hf][2u * r + 1u] - m1);
+          const float x = ex2(fmaf(s[nt][hf][2u * r], f0, m0));
+          const float y = ex2(fmaf(s[nt][hf][2u * r + 1u], f1, m1));
           l[nt][0] += x;
           l[nt][1] += y;
-          p[nt][hf][r] = transpose8x8(half2_bits(__floats2half2_rn(x, y)));
+          p[nt][hf][r] = __byte_perm(transpose8x8(half2_bits(__floats2half2_rn(x, y))), 0u, order);
         }
       }
     }
@@ -476,7 +482,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       uint32_t w[4][kWords], sc[2][2];
 #pragma unroll
       for (uint32_t r = 0; r < 4u; ++r) {  // keys 2t, 2t + 1, 2t + 8, 2t + 9
-        const uint32_t key = 2u * t + (r & 1u) + 8u * (r >> 1);
+        const uint32_t key = 2u * t + ((r & 1u) ^ swap) + 8u * (r >> 1);
         const uint8_t* p8 = vc + key * (HD / 2u);
         if constexpr (HD == 128u) {
           const uint2 v = *reinterpret_cast<const uint2*>(p8 + 8u * g);
@@ -495,8 +501,9 @@ __global__ void __launch_bounds__(kWarps * 32)
       for (uint32_t r = 0; r < 2u; ++r) {
         const uint8_t* q = vs + (2u * t + 8u * r) * (HD / 32u);
         const uint32_t b = HD == 128u ? g >> 1 : HD == 32u ? 0u : g >> 2;
-        sc[r][0] = scale2(q[b], q[b + HD / 32u]);
-        sc[r][1] = HD == 96u ? scale2(q[2], q[2u + HD / 32u]) : sc[r][0];
+        const uint32_t one = swap * (HD / 32u), two = (swap ^ 1u) * (HD / 32u);
+        sc[r][0] = scale2(q[b + one], q[b + two]);
+        sc[r][1] = HD == 96u ? scale2(q[2u + one], q[2u + two]) : sc[r][0];
       }
 #pragma unroll
       for (uint32_t x = 0; x < kWords; ++x) {
@@ -546,6 +553,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
   if (bad_page && lane == 0u) atomicOr(error_flag, kErrKvSlot);
 
+  griddep_launch_dependents();  // k_attn_join may be set up
   // Join the warps: rows of (m, l, O) in shared memory over the rings.
   __syncthreads();
   constexpr uint32_t kLd = HD + 4u;
@@ -615,16 +623,20 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-// Joins the chunks of a request's rows: a block a row and head, its warps
-// summing every kJoinWarps-th chunk (many chunks have many loads in flight;
-// their order does not depend on anything but their number).
+// Joins the chunks of a request's rows, W warps a row and head, each summing
+// every W-th chunk (many chunks have many loads in flight; their order does
+// not depend on anything but their number).
 constexpr uint32_t kJoinWarps = 8;
 
+template <uint32_t W>
 __global__ void __launch_bounds__(kJoinWarps * 32)
     k_attn_join(const AttnJob j, uint32_t* __restrict__ error_flag) {
-  __shared__ float part[kJoinWarps][128], sums[kJoinWarps];
-  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, hd = j.cache.hd;
-  const uint32_t r = blockIdx.x / j.heads, h = blockIdx.x % j.heads;
+  __shared__ float part[kJoinWarps][W > 1u ? 128 : 1], sums[kJoinWarps];
+  const uint32_t lane = threadIdx.x & 31u, hd = j.cache.hd;
+  const uint32_t warp = W > 1u ? threadIdx.x >> 5 : 0u;
+  const uint32_t cell = W > 1u ? blockIdx.x : blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+  const uint32_t r = cell / j.heads, h = cell % j.heads;
+  griddep_wait();
   int32_t q0, q_len, kv;
   attn_request(j, blockIdx.y, &q0, &q_len, &kv);
   if (static_cast<int32_t>(r) >= q_len) return;
@@ -638,7 +650,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   for (uint32_t d = 16; d > 0; d /= 2u) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
   float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (uint32_t c = warp; c < chunks; c += kJoinWarps) {
+  for (uint32_t c = warp; c < chunks; c += W) {
     const float2 ml = j.part_ml[c * stride + unit];
     const float* o = j.part_o + (c * stride + unit) * hd + lane;
     const float w = ml.x == -INFINITY ? (ml.y != 0.f ? 1.f : 0.f) : ex2(ml.x - top);
@@ -648,15 +660,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
       if (b < hd / 32u) x[b] += w * o[32u * b];
     }
   }
+  if constexpr (W == 1u) {
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
 #pragma unroll
-  for (uint32_t b = 0; b < 4u; ++b) part[warp][32u * b + lane] = x[b];
+    for (uint32_t b = 0; b < 4u; ++b) {
+      if (b < hd / 32u) write_block(j, row, h, b, lane, x[b] * inv, error_flag);
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t b = 0; b < 4u; ++b) part[warp][W > 1u ? 32u * b + lane : 0u] = x[b];
   if (lane == 0u) sums[warp] = sum;
   __syncthreads();
   if (warp >= hd / 32u) return;
   float y = 0.f, all = 0.f;
 #pragma unroll
   for (uint32_t w = 0; w < kJoinWarps; ++w) {
-    y += part[w][32u * warp + lane];
+    y += part[w][W > 1u ? 32u * warp + lane : 0u];
     all += sums[w];
   }
   write_block(j, row, h, warp, lane, y * (all != 0.f ? 1.0f / all : 0.f), error_flag);
@@ -688,16 +708,43 @@ cudaError_t launch_rows(const AttnJob& job, uint32_t rows, uint32_t chunks, uint
 
 }  // namespace
 
-void launch_attn_join(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream) {
-  k_attn_join<<<dim3(job.max_q * job.heads, job.seqs), kJoinWarps * 32, 0, stream>>>(job,
-                                                                                   error_flag);
+int launch_attn_join(const AttnJob& job, cudaStream_t stream, uint32_t* error_flag) {
+  const uint32_t cells = job.max_q * job.heads;
+  const uint32_t chunks = (job.max_kv + job.chunk - 1u) / job.chunk;
+  // A block a row and head where there are many chunks (74 of one request:
+  // 32 blocks), else a warp.
+  const bool many = chunks > 8u;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(many ? cells : (cells + kJoinWarps - 1u) / kJoinWarps, job.seqs);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t st = many ? cudaLaunchKernelEx(&cfg, k_attn_join<kJoinWarps>, job, error_flag)
+                              : cudaLaunchKernelEx(&cfg, k_attn_join<1>, job, error_flag);
+  return st == cudaSuccess ? 1 : -1;
 }
 
 uint32_t attn_decode_chunk(const AttnJob& job, uint64_t total_kv, int sm_count) {
-  // Enough chunks to fill the GPU about four times over with the requests'
-  // keys, of 256 keys at least and 128 chunks a request at most.
-  const uint64_t blocks = static_cast<uint64_t>(sm_count) * 16u;
-  uint64_t chunk = total_kv * job.cache.kv_heads / blocks;
+  // Blocks that the GPU holds at once (4 an SM with one n tile, 2 else; their
+  // registers).  Requests of one length take one wave of chunks, others four
+  // smaller ones that even out (64 requests of 4 K to 16 K keys: 185 us with
+  // four, 225 with one; one of 131071 keys 47 and 53).  Chunks have 256 keys at
+  // least, and a request 128 chunks at most.
+  const uint32_t rows = job.max_q * job.group, nt = rows <= 8u ? 1u : rows <= 16u ? 2u : 4u;
+  const uint64_t row_blocks = (rows + 8u * nt - 1u) / (8u * nt);
+  const uint64_t wave = static_cast<uint64_t>(sm_count) * (nt == 1u ? 4u : 2u);
+  const uint64_t units = job.cache.kv_heads * row_blocks;  // chunks of all of these are blocks
+  uint64_t chunk;
+  if (total_kv == static_cast<uint64_t>(job.seqs) * job.max_kv) {
+    const uint64_t each = wave / (units * job.seqs);
+    chunk = each > 1u ? (job.max_kv + each - 1u) / each : job.max_kv;
+  } else {
+    chunk = total_kv * units / (4u * wave);
+  }
   const uint64_t least = (static_cast<uint64_t>(job.max_kv) + 127u) / 128u;
   if (chunk < least) chunk = least;
   if (chunk < 256u) chunk = 256u;
@@ -717,8 +764,7 @@ int launch_attn_decode(const AttnJob& job, uint32_t* error_flag, cudaStream_t st
   }
   if (st != cudaSuccess) return -1;
   if (chunks == 1u) return 1;
-  launch_attn_join(job, error_flag, stream);
-  return 2;
+  return launch_attn_join(job, stream, error_flag) < 0 ? -1 : 2;
 }
 
 }  // namespace hrb

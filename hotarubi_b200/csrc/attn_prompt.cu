@@ -681,8 +681,7 @@ int launch_attn_prompt(const AttnJob& job, uint32_t* error_flag, cudaStream_t st
     default: n = launch_hd<128>(job, chunks, error_flag, stream); break;
   }
   if (n < 0 || chunks == 1u) return n;
-  launch_attn_join(job, error_flag, stream);
-  return n + 1;
+  return launch_attn_join(job, stream, error_flag) < 0 ? -1 : n + 1;
 }
 
 }  // namespace hrb

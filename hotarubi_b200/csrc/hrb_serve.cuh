@@ -128,7 +128,7 @@ uint32_t attn_decode_chunk(const AttnJob& job, uint64_t total_kv, int sm_count);
 int launch_attn_decode(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
 
 // Joins the chunks' results of all rows.
-void launch_attn_join(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
+int launch_attn_join(const AttnJob& job, cudaStream_t stream, uint32_t* error_flag);
 
 // Any number of rows.  Scratch for attn_prompt_tiles tiles a key/value head.
 uint64_t attn_prompt_tiles(const AttnJob& job, uint64_t total_kv, uint32_t* stride);
