@@ -54,23 +54,19 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Where a tile's parts lie in a stage: pages of 16 tokens bring two records,
-// larger pages 32 tokens of one.
-struct TileGeom {
-  uint32_t ks, v, vs;          // K scales, V codes, V scales (K codes at 0)
-  uint32_t code_half, scale_half;  // from tokens 0..15 to 16..31
+// Where a tile's parts lie in a stage: pages of 16 tokens (P16) bring two
+// records, larger pages 32 tokens of one.  Fixed when the kernel is built, so
+// that a load's offset is in its instruction.
+template <uint32_t HD, bool P16>
+struct Geom {
+  static constexpr uint32_t kN = P16 ? 16u : 32u;
+  static constexpr uint32_t kKs = kN * (HD / 2u);                 // K scales (K codes at 0)
+  static constexpr uint32_t kV = kN * (HD / 2u + HD / 32u);       // V codes
+  static constexpr uint32_t kVs = kV + kN * (HD / 2u);            // V scales
+  // From tokens 0..15 to 16..31.
+  static constexpr uint32_t kCodeHalf = P16 ? 16u * (HD + HD / 16u) : 16u * (HD / 2u);
+  static constexpr uint32_t kScaleHalf = P16 ? 16u * (HD + HD / 16u) : 16u * (HD / 32u);
 };
-template <uint32_t HD>
-__device__ __forceinline__ TileGeom tile_geom(uint32_t page) {
-  const uint32_t n = min(page, kTile);
-  TileGeom g;
-  g.ks = n * (HD / 2u);
-  g.v = n * (HD / 2u + HD / 32u);
-  g.vs = g.v + n * (HD / 2u);
-  g.code_half = page == 16u ? 16u * (HD + HD / 16u) : 16u * (HD / 2u);
-  g.scale_half = page == 16u ? 16u * (HD + HD / 16u) : 16u * (HD / 32u);
-  return g;
-}
 
 template <uint32_t HD, uint32_t NT>
 struct Smem {
@@ -79,20 +75,26 @@ struct Smem {
   static constexpr uint32_t kJoin = kWarps * 8u * NT * (HD + 4u) * 4u;
   static constexpr uint32_t kBuf = kRing > kJoin ? kRing : kJoin;
   static constexpr uint32_t kQ = NT > 2u ? 8u * NT * HD * 2u : 0u;  // Q fragments, see below
-  static constexpr uint32_t kBytes = kBuf + kQ + kWarps * kStages * 8u;
+  static constexpr uint32_t kScales = kBuf + kQ;               // [256] words
+  static constexpr uint32_t kBars = kScales + 1024u;
+  static constexpr uint32_t kBytes = kBars + kWarps * kStages * 8u;
 };
 
-template <uint32_t HD, uint32_t NT>
+template <uint32_t HD, uint32_t NT, bool P16>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     k_attn_decode(const AttnJob j, uint32_t* __restrict__ error_flag) {
   using S = Smem<HD, NT>;
+  using Geo = Geom<HD, P16>;
   constexpr uint32_t kSteps = HD / 16u;           // MMAs along dims; m16 tiles of dims
   constexpr uint32_t kRows = 8u * NT;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   const uint32_t g = lane >> 2, t = lane & 3u;
   uint8_t* ring = smem + warp * kStages * S::kStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBuf + S::kQ) + warp * kStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars) + warp * kStages;
+  // Every scale byte as a pair of FP16: a load instead of a shift, a
+  // conversion and two clamps, which the pipe of the codes' conversions takes.
+  uint32_t* scales = reinterpret_cast<uint32_t*>(smem + S::kScales);
 
   const uint32_t n = blockIdx.z, head = blockIdx.y;
   int32_t q0, q_len, kv;
@@ -110,6 +112,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
   const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
   const bool whole = kv <= static_cast<int32_t>(j.chunk);  // no other chunk of this request
 
+  for (uint32_t b = threadIdx.x; b < 256u; b += kWarps * 32u) scales[b] = scale2(b, b);
   if (lane < kStages) mbar_init(full + lane, 1);
   fence_barrier_init();
   __syncwarp();
@@ -119,9 +122,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
   const Seen first = attn_seen(j, kv - q_len + r0 / group, kv, pre);
   const Seen last = attn_seen(j, kv - q_len + (r0 + rows - 1) / group, kv, pre);
 
-  const TileGeom geo = tile_geom<HD>(j.cache.page);
   const int32_t* table = j.table + static_cast<uint64_t>(n) * j.table_ld;
-  const uint32_t copies = j.cache.page == 16u ? 2u : j.cache.page == 32u ? 1u : 4u;
+  const uint32_t copies = P16 ? 2u : j.cache.page == 32u ? 1u : 4u;
   // Lane l holds the pages of the warp's tile number base + l.
   int32_t page_a = -1, page_b = -1, base = 0;
   auto load_pages = [&](int32_t at) {  // tiles number at .. at + 31 of this warp
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     const int32_t k = c0 + i * static_cast<int32_t>(kTile);
     page_a = k < kv ? __ldg(table + (k >> j.cache.page_log2)) : -2;
     page_b = page_a;
-    if (j.cache.page == 16u) page_b = k + 16 < kv ? __ldg(table + ((k + 16) >> 4)) : -2;
+    if (P16) page_b = k + 16 < kv ? __ldg(table + ((k + 16) >> 4)) : -2;
   };
   const uint8_t* const head_data = j.cache.data + static_cast<uint64_t>(head) * j.cache.record;
   // -2: no keys there; other values outside the cache read as zeros.
@@ -139,7 +141,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     const uint32_t k = static_cast<uint32_t>(c0 + i * static_cast<int32_t>(kTile));
     const int32_t pa = __shfl_sync(0xFFFFFFFFu, page_a, number - base);
     const int32_t pb = __shfl_sync(0xFFFFFFFFu, page_b, number - base);
-    const int32_t page = lane == 1u && j.cache.page == 16u ? pb : pa;
+    const int32_t page = lane == 1u && P16 ? pb : pa;
     const bool there = static_cast<uint32_t>(page) < j.cache.pages;
     uint8_t* dst = ring + stage * S::kStageBytes;
     uint32_t bytes, from;
@@ -149,16 +151,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
       dst += lane * j.cache.record;
     } else {
       const uint32_t in = k & (j.cache.page - 1u);
-      const bool scales = (lane & 1u) != 0u;
-      bytes = scales ? kTile * (HD / 32u) : kTile * (HD / 2u);
+      const bool of_scales = (lane & 1u) != 0u;
+      bytes = of_scales ? kTile * (HD / 32u) : kTile * (HD / 2u);
       from = (lane >= 2u ? kv_vcodes(j.cache) : 0u) +
-             (scales ? kv_kscales(j.cache) + in * (HD / 32u) : in * (HD / 2u));
-      dst += (lane >= 2u ? geo.v : 0u) + (scales ? geo.ks : 0u);
+             (of_scales ? kv_kscales(j.cache) + in * (HD / 32u) : in * (HD / 2u));
+      dst += (lane >= 2u ? Geo::kV : 0u) + (of_scales ? Geo::kKs : 0u);
     }
     const uint32_t in_a = static_cast<uint32_t>(pa) < j.cache.pages ? 1u : 0u;
     const uint32_t in_b = static_cast<uint32_t>(pb) < j.cache.pages ? 1u : 0u;
     // Two records, one, or a tile's part of a larger one.
-    const uint32_t total = j.cache.page == 16u ? (in_a + in_b) * j.cache.record
+    const uint32_t total = P16 ? (in_a + in_b) * j.cache.record
                                                : in_a * S::kStageBytes;
     if (lane == 0u) mbar_arrive_expect_tx(full + stage, total);
     __syncwarp();
@@ -218,11 +220,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
       }
     }
   }
-  if constexpr (NT > 2u) __syncthreads();
-  // Lanes t = 2, 3 take the two keys of a pair the other way round, in V and
-  // in P: the four t of a load are then in different banks at hd 64, and two
-  // share one instead of four at hd 128.
-  const uint32_t swap = t >> 1, order = swap != 0u ? 0x1032u : 0x3210u;
+  __syncthreads();  // the scales, and Q
   // The lane's two rows of each n tile in S^T and O^T: 8 nt + 2 t + {0, 1}.
   float factor[NT][2], m[NT][2], l[NT][2], slope[NT][2];
   Seen seen[NT][2];
@@ -307,8 +305,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     float s[NT][2][4];
 #pragma unroll
     for (uint32_t hf = 0; hf < 2u; ++hf) {
-      const uint8_t* kc = tile + hf * geo.code_half;
-      const uint8_t* ks = tile + geo.ks + hf * geo.scale_half;
+      const uint8_t* kc = tile + hf * Geo::kCodeHalf;
+      const uint8_t* ks = tile + Geo::kKs + hf * Geo::kScaleHalf;
       uint32_t w[2][HD / 32u];
       uint32_t sc[2][2];  // the lane's block scales (two blocks at hd 96)
 #pragma unroll
@@ -330,10 +328,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
         }
         const uint8_t* q = ks + (g + 8u * r) * (HD / 32u);
         const uint32_t b0 = q[t * (HD / 4u) / 32u];
-        sc[r][0] = scale2(b0, b0);
+        sc[r][0] = scales[b0];
         if constexpr (HD == 96u) {
           const uint32_t b1 = q[(t * 24u + 23u) / 32u];
-          sc[r][1] = scale2(b1, b1);
+          sc[r][1] = scales[b1];
         } else {
           sc[r][1] = sc[r][0];
         }
@@ -461,7 +459,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
           const float y = ex2(fmaf(s[nt][hf][2u * r + 1u], f1, m1));
           l[nt][0] += x;
           l[nt][1] += y;
-          p[nt][hf][r] = __byte_perm(transpose8x8(half2_bits(__floats2half2_rn(x, y))), 0u, order);
+          p[nt][hf][r] = transpose8x8(half2_bits(__floats2half2_rn(x, y)));
         }
       }
     }
@@ -476,13 +474,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     // its rows g + 8, two dims of one byte.
 #pragma unroll
     for (uint32_t hf = 0; hf < 2u; ++hf) {
-      const uint8_t* vc = tile + geo.v + hf * geo.code_half;
-      const uint8_t* vs = tile + geo.vs + hf * geo.scale_half;
+      const uint8_t* vc = tile + Geo::kV + hf * Geo::kCodeHalf;
+      const uint8_t* vs = tile + Geo::kVs + hf * Geo::kScaleHalf;
       constexpr uint32_t kWords = (HD + 63u) / 64u;  // words of codes a lane and key (the last half used at hd 96 and 32)
       uint32_t w[4][kWords], sc[2][2];
 #pragma unroll
       for (uint32_t r = 0; r < 4u; ++r) {  // keys 2t, 2t + 1, 2t + 8, 2t + 9
-        const uint32_t key = 2u * t + ((r & 1u) ^ swap) + 8u * (r >> 1);
+        const uint32_t key = 2u * t + (r & 1u) + 8u * (r >> 1);
         const uint8_t* p8 = vc + key * (HD / 2u);
         if constexpr (HD == 128u) {
           const uint2 v = *reinterpret_cast<const uint2*>(p8 + 8u * g);
@@ -501,9 +499,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
       for (uint32_t r = 0; r < 2u; ++r) {
         const uint8_t* q = vs + (2u * t + 8u * r) * (HD / 32u);
         const uint32_t b = HD == 128u ? g >> 1 : HD == 32u ? 0u : g >> 2;
-        const uint32_t one = swap * (HD / 32u), two = (swap ^ 1u) * (HD / 32u);
-        sc[r][0] = scale2(q[b + one], q[b + two]);
-        sc[r][1] = HD == 96u ? scale2(q[2u + one], q[2u + two]) : sc[r][0];
+        sc[r][0] = __byte_perm(scales[q[b]], scales[q[b + HD / 32u]], 0x5410);
+        sc[r][1] = HD == 96u ? __byte_perm(scales[q[2]], scales[q[2u + HD / 32u]], 0x5410) : sc[r][0];
       }
 #pragma unroll
       for (uint32_t x = 0; x < kWords; ++x) {
@@ -682,28 +679,34 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   write_block(j, row, h, warp, lane, y * (all != 0.f ? 1.0f / all : 0.f), error_flag);
 }
 
-template <uint32_t HD, uint32_t NT>
+template <uint32_t HD, uint32_t NT, bool P16>
 cudaError_t launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stream) {
   static std::atomic<uint64_t> set{0};  // devices whose limit is raised
   if (((set.load(std::memory_order_relaxed) >> (job.device & 63u)) & 1u) == 0u || job.device > 63u) {
     const cudaError_t st = cudaFuncSetAttribute(
-        k_attn_decode<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, NT>::kBytes);
+        k_attn_decode<HD, NT, P16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, NT>::kBytes);
     if (st != cudaSuccess) return st;
     set.fetch_or(uint64_t{1} << (job.device & 63u), std::memory_order_relaxed);
   }
   AttnJob j = job;
   j.row_blocks = (job.max_q * job.group + 8u * NT - 1u) / (8u * NT);
-  k_attn_decode<HD, NT><<<dim3(chunks * j.row_blocks, job.cache.kv_heads, job.seqs), kWarps * 32,
-                          Smem<HD, NT>::kBytes, stream>>>(j, err);
+  k_attn_decode<HD, NT, P16><<<dim3(chunks * j.row_blocks, job.cache.kv_heads, job.seqs), kWarps * 32,
+                               Smem<HD, NT>::kBytes, stream>>>(j, err);
   return cudaSuccess;
+}
+
+template <uint32_t HD, uint32_t NT>
+cudaError_t launch_page(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stream) {
+  return job.cache.page == 16u ? launch<HD, NT, true>(job, chunks, err, stream)
+                               : launch<HD, NT, false>(job, chunks, err, stream);
 }
 
 template <uint32_t HD>
 cudaError_t launch_rows(const AttnJob& job, uint32_t rows, uint32_t chunks, uint32_t* err,
                         cudaStream_t stream) {
-  if (rows <= 8u) return launch<HD, 1>(job, chunks, err, stream);
-  if (rows <= 16u) return launch<HD, 2>(job, chunks, err, stream);
-  return launch<HD, 4>(job, chunks, err, stream);
+  if (rows <= 8u) return launch_page<HD, 1>(job, chunks, err, stream);
+  if (rows <= 16u) return launch_page<HD, 2>(job, chunks, err, stream);
+  return launch_page<HD, 4>(job, chunks, err, stream);
 }
 
 }  // namespace
