@@ -59,6 +59,41 @@ __device__ __forceinline__ uint32_t first_tile(const AttnJob& j, uint32_t n) {
   return __reduce_add_sync(0xFFFFFFFFu, sum);
 }
 
+// Eight dims of a key (a word of codes) as FP16.
+__device__ __forceinline__ uint4 key_dims(uint32_t word, uint32_t scale) {
+  uint32_t h[4];
+  e2m1x8_to_f16x2(word, h);
+  return make_uint4(mul2(h[0], scale), mul2(h[1], scale), mul2(h[2], scale), mul2(h[3], scale));
+}
+
+// Eight dims of eight keys (a word of codes each, a scale byte each) turned:
+// row d holds dim d of the keys.
+__device__ __forceinline__ void turn_values(const uint32_t (&w)[8], const uint32_t (&sb)[8],
+                                            uint32_t (&h)[8][4]) {
+#pragma unroll
+  for (uint32_t r = 0; r < 4u; ++r) {
+    const uint32_t a = w[2u * r], b = w[2u * r + 1u], sc = scale2(sb[2u * r], sb[2u * r + 1u]);
+    uint32_t lo[4], hi[4];
+    e2m1x8_to_f16x2((a & 0x0F0F0F0Fu) | ((b << 4) & 0xF0F0F0F0u), lo);
+    e2m1x8_to_f16x2(((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u), hi);
+#pragma unroll
+    for (uint32_t d = 0; d < 4u; ++d) {
+      h[2u * d][r] = mul2(lo[d], sc);
+      h[2u * d + 1u][r] = mul2(hi[d], sc);
+    }
+  }
+}
+
+// Where eight dims (number u) of a key lie in a K tile, and eight keys
+// (number kg) of a dim in a V^T tile.
+__device__ __forceinline__ uint32_t k_place(uint32_t key, uint32_t u) {
+  return (u / 8u) * (kKeys * kRowB) + key * kRowB + (((u & 7u) ^ (key & 7u)) * 16u);
+}
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t v_place(uint32_t dim, uint32_t kg) {
+  return (kg / 8u) * (HD * kRowB) + dim * kRowB + (((kg & 7u) ^ (dim & 7u)) * 16u);
+}
+
 // A block: one tile of one request and key/value head.
 template <uint32_t HD>
 __global__ void __launch_bounds__(256)
@@ -122,41 +157,24 @@ __global__ void __launch_bounds__(256)
   // K: 16 bytes (8 dims of a key) a step, neighbours in a row.
   for (uint32_t i = threadIdx.x; i < kKeys * (HD / 8u); i += 256u) {
     const uint32_t key = i / (HD / 8u), u = i % (HD / 8u);
-    uint32_t h[4];
-    e2m1x8_to_f16x2(*reinterpret_cast<const uint32_t*>(&codes[0][key * kLd + 4u * u]), h);
     const uint32_t b = scales[0][key * (HD / 32u) + u / 4u];
-    const uint32_t sc = scale2(b, b);
-#pragma unroll
-    for (uint32_t d = 0; d < 4u; ++d) h[d] = mul2(h[d], sc);
-    *reinterpret_cast<uint4*>(out + (u / 8u) * (kKeys * kRowB) + key * kRowB +
-                              (((u & 7u) ^ (key & 7u)) * 16u)) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(out + k_place(key, u)) =
+        key_dims(*reinterpret_cast<const uint32_t*>(&codes[0][key * kLd + 4u * u]), scale2(b, b));
   }
   // V^T: a thread turns 8 keys x 8 dims; 8 neighbours fill a row.
   out += k_bytes(HD);
   for (uint32_t i = threadIdx.x; i < (kKeys / 8u) * (HD / 8u); i += 256u) {
     const uint32_t kg = i % (kKeys / 8u), dg = i / (kKeys / 8u);
-    uint32_t h[8][4];  // dim, key pair
+    uint32_t w[8], sb[8], h[8][4];
 #pragma unroll
-    for (uint32_t r = 0; r < 4u; ++r) {
-      const uint32_t key = 8u * kg + 2u * r;
-      const uint32_t a = *reinterpret_cast<const uint32_t*>(&codes[1][key * kLd + 4u * dg]);
-      const uint32_t b = *reinterpret_cast<const uint32_t*>(&codes[1][(key + 1u) * kLd + 4u * dg]);
-      const uint32_t sc = scale2(scales[1][key * (HD / 32u) + dg / 4u],
-                                 scales[1][(key + 1u) * (HD / 32u) + dg / 4u]);
-      uint32_t lo[4], hi[4];
-      e2m1x8_to_f16x2((a & 0x0F0F0F0Fu) | ((b << 4) & 0xF0F0F0F0u), lo);
-      e2m1x8_to_f16x2(((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u), hi);
-#pragma unroll
-      for (uint32_t d = 0; d < 4u; ++d) {
-        h[2u * d][r] = mul2(lo[d], sc);
-        h[2u * d + 1u][r] = mul2(hi[d], sc);
-      }
+    for (uint32_t r = 0; r < 8u; ++r) {
+      w[r] = *reinterpret_cast<const uint32_t*>(&codes[1][(8u * kg + r) * kLd + 4u * dg]);
+      sb[r] = scales[1][(8u * kg + r) * (HD / 32u) + dg / 4u];
     }
+    turn_values(w, sb, h);
 #pragma unroll
     for (uint32_t d = 0; d < 8u; ++d) {
-      const uint32_t row = 8u * dg + d;
-      *reinterpret_cast<uint4*>(out + (kg / 8u) * (HD * kRowB) + row * kRowB +
-                                (((kg & 7u) ^ (row & 7u)) * 16u)) =
+      *reinterpret_cast<uint4*>(out + v_place<HD>(8u * dg + d, kg)) =
           make_uint4(h[d][0], h[d][1], h[d][2], h[d][3]);
     }
   }
@@ -290,6 +308,9 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   const int32_t resume = max(gap, min(end, tiles_to(first.lo + 1 - static_cast<int32_t>(kKeys))));
   const int32_t count = gap + end - resume;
   auto tile_at = [&](int32_t it) { return it < gap ? it : it - gap + resume; };
+  // Of the last tile only the first 64 keys, where no row sees another.
+  const int32_t half_end = c0 + tile_at(count - 1) * static_cast<int32_t>(kKeys) + 64;
+  const bool last_half = min(max(last.hi, first.pre), c1) <= half_end;
 
   // A softmax thread's row (its half's thread number) and its part of Q, on
   // their way while the block sets up.
@@ -391,6 +412,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
         for (uint32_t h = 0; h < halves && ok; ++h) {
 #pragma unroll
           for (uint32_t k = 0; k < kKeys / 16u; ++k) {
+            if (k == 4u && last_half && !more) break;
             if ((k & 3u) == 0u) {  // 64 keys' weights
               ok = mbar_wait(p_full + 2u * h + (k >> 2), static_cast<uint32_t>(it) & 1u, error_flag);
               if (!ok) break;
@@ -468,9 +490,18 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
         if (!__all_sync(0xFFFFFFFFu, ok)) break;
         tc_fence_after();
         uint32_t s[4][32];
-#pragma unroll
-        for (uint32_t c = 0; c < 4u; ++c) tmem_ld32(t_s + 32u * c, s[c]);
+        const bool both = !(last_half && it == count - 1);  // 64s of keys
+        tmem_ld32(t_s, s[0]);
+        tmem_ld32(t_s + 32u, s[1]);
+        if (both) {
+          tmem_ld32(t_s + 64u, s[2]);
+          tmem_ld32(t_s + 96u, s[3]);
+        }
         tmem_wait_ld();
+        if (!both) {
+#pragma unroll
+          for (uint32_t i = 0; i < 32u; ++i) s[2][i] = s[3][i] = 0xFF800000u;
+        }
         const int32_t k0 = c0 + tile_at(it) * static_cast<int32_t>(kKeys);
         const int32_t k1 = k0 + static_cast<int32_t>(kKeys);
         auto at = [&](uint32_t c, uint32_t i) -> float { return __uint_as_float(s[c][i]); };
@@ -542,6 +573,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
         uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (uint32_t c = 0; c < 2u; ++c) {
+          if (c == 1u && !both) break;
           uint32_t p[32];
 #pragma unroll
           for (uint32_t i = 0; i < 32u; ++i) {
@@ -613,10 +645,9 @@ int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stre
   }
   const uint32_t key_tiles = (job.max_kv + kKeys - 1u) / kKeys;
   const uint32_t q_tiles = (job.max_q * job.group + HV * kHalf - 1u) / (HV * kHalf);
-  int n = 1;
-  if (key_tiles != 0u) {
+  const bool expand = key_tiles != 0u;
+  if (expand) {
     k_kv_expand<HD><<<dim3(key_tiles, job.cache.kv_heads, job.seqs), 256, 0, stream>>>(job, err);
-    ++n;
   }
   // Its blocks may start, load Q and set up while k_kv_expand still runs.
   cudaLaunchConfig_t cfg{};
@@ -628,9 +659,9 @@ int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stre
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = key_tiles != 0u ? 1u : 0u;
+  cfg.numAttrs = expand ? 1u : 0u;
   if (cudaLaunchKernelEx(&cfg, k_attn_prompt<HD, HV>, job, err) != cudaSuccess) return -1;
-  return n;
+  return expand ? 2 : 1;
 }
 
 template <uint32_t HD>
@@ -640,8 +671,9 @@ int launch_hd(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t s
   // 16.9.  At hd 128 one half a block is slower throughout (98.6 and 103.2 us
   // for 32 of 141 with 32/8 heads), as is a long history (43.4 and 47.1 us for
   // 200 rows over 8000 keys at hd 64).
-  return HD <= 64u && job.max_kv <= 1024u ? launch<HD, 1>(job, chunks, err, stream)
-                                          : launch<HD, 2>(job, chunks, err, stream);
+  constexpr uint32_t kOne = HD <= 64u ? 1u : 2u;
+  return job.max_kv <= 1024u ? launch<HD, kOne>(job, chunks, err, stream)
+                             : launch<HD, 2>(job, chunks, err, stream);
 }
 
 }  // namespace
