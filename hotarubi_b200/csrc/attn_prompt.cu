@@ -206,6 +206,42 @@ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) {
   return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
+// The low word of a desc_sw128 descriptor (its start address, in 16-byte
+// units, and fields that do not change); the high word is the same for all.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_byte_addr) {
+  return static_cast<uint32_t>(desc_sw128(smem_byte_addr));
+}
+// Keeps a value where it is: what is added to it is not computed ahead for a
+// whole loop, in registers the issuing thread does not have.
+__device__ __forceinline__ uint32_t here(uint32_t x) {
+  asm volatile("" : "+r"(x));
+  return x;
+}
+
+// kind::f16 with FP16 operands: A and B in shared memory, and A in TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -262,7 +298,9 @@ __device__ __forceinline__ void cap_scores(const AttnJob& j, float factor, uint3
   }
 }
 
-template <uint32_t HD, uint32_t HV>
+// SHAPED: a cap or a distance bias on the scores; apart, because their code
+// would cost the plain kernel registers.
+template <uint32_t HD, uint32_t HV, bool SHAPED>
 __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
     k_attn_prompt(const AttnJob j, uint32_t* __restrict__ error_flag) {
   using S = Cfg<HD, HV>;
@@ -350,12 +388,12 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   const uint32_t tmem = *tmem_slot;
 
   // A softmax thread holds a row's 128 scores.  Registers at launch: 384 x
-  // 168 = 256 x 224 + 128 x 56 (HV 2), 256 x 128 = 128 x 208 + 128 x 48.
+  // 168 = 256 x 216 + 128 x 72 (HV 2), 256 x 128 = 128 x 200 + 128 x 56.
   if (warp >= 4u * HV) {
     if constexpr (HV == 2u) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     }
   if (warp == 4u * HV + 1u) {
     if (lane == 0u) {
@@ -383,15 +421,15 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
     }
   } else if (warp == 4u * HV) {
     if (lane == 0u && count > 0) {
-      // Descriptors advance by their start address alone, in 16-byte units.
-      const uint64_t q_at = desc_sw128(smem_addr(smem)), k_at = desc_sw128(smem_addr(smem + S::kK));
-      const uint64_t v_at = desc_sw128(smem_addr(smem + S::kV));
+      const uint32_t q_at = desc_low(smem_addr(smem)), k_at = desc_low(smem_addr(smem + S::kK));
+      const uint32_t v_at = desc_low(smem_addr(smem + S::kV));
       auto scores = [&](uint32_t h, uint32_t st) {
+        const uint32_t a = here(q_at + h * (k_bytes(HD) / 16u));
+        const uint32_t b = here(k_at + st * (k_bytes(HD) / 16u));
 #pragma unroll
         for (uint32_t k = 0; k < HD / 16u; ++k) {
           const uint32_t off = ((k >> 2) * (kKeys * kRowB) + 32u * (k & 3u)) / 16u;
-          mma_bf16(tmem + 128u * h, q_at + (h * (k_bytes(HD) / 16u) + off),
-                   k_at + (st * (k_bytes(HD) / 16u) + off), idesc_f16(128, 128), k != 0u);
+          mma_ss(tmem + 128u * h, a + off, b + off, idesc_f16(128, 128), k != 0u);
         }
         mma_commit(s_full + h);
       };
@@ -410,6 +448,8 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
         ok = mbar_wait(v_full + st, ph, error_flag) &&
              (!more || mbar_wait(k_full + nst, (static_cast<uint32_t>(it + 1) / kNs) & 1u, error_flag));
         for (uint32_t h = 0; h < halves && ok; ++h) {
+          const uint32_t a = here(tmem + 128u * h), b = here(v_at + st * (v_bytes(HD) / 16u));
+          const uint32_t d = tmem + S::kO + 128u * h;
 #pragma unroll
           for (uint32_t k = 0; k < kKeys / 16u; ++k) {
             if (k == 4u && last_half && !more) break;
@@ -418,9 +458,8 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
               if (!ok) break;
               tc_fence_after();
             }
-            mma_bf16_ts(tmem + S::kO + 128u * h, tmem + 128u * h + 8u * k,
-                        v_at + (st * v_bytes(HD) + (k >> 2) * (HD * kRowB) + 32u * (k & 3u)) / 16u,
-                        idesc_f16(128, HD), it != 0 || k != 0u);
+            mma_ts(d, a + 8u * k, b + ((k >> 2) * (HD * kRowB) + 32u * (k & 3u)) / 16u, idesc_f16(128, HD),
+                   it != 0 || k != 0u);
           }
           if (!ok) break;
           if (more) {
@@ -436,9 +475,9 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   }
   } else {
     if constexpr (HV == 2u) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     } else {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     }
     const uint32_t h = warp >> 2;
     float factor;
@@ -458,7 +497,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
       float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
       if (j.scale < 0.f) up = -up;
       factor = fabsf(j.scale) * __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23) *
-               (j.softcap != 0.f ? 1.0f : kLog2e);
+               (SHAPED && j.softcap != 0.f ? 1.0f : kLog2e);
       factor = fmaxf(factor, 1.2e-38f);  // times a masked score's -inf is no NaN
       uint8_t* dst = smem + h * k_bytes(HD) + in_half * kRowB;
 #pragma unroll
@@ -479,7 +518,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
     const int32_t pos = kv - q_len + (mine ? r : r0) / group;
     Seen seen = attn_seen(j, pos, kv, pre);
     if (!mine) seen.lo = seen.hi = seen.pre = 0;
-    const float slope = j.slopes != nullptr ? __ldg(j.slopes + qh) * kLog2e : 0.f;
+    const float slope = SHAPED && j.slopes != nullptr ? __ldg(j.slopes + qh) * kLog2e : 0.f;
     const uint32_t lanes = ((warp & 3u) * 32u) << 16;
     const uint32_t t_s = tmem + lanes + 128u * h, t_o = tmem + lanes + S::kO + 128u * h;
     float m = -INFINITY, l = 0.f;
@@ -507,11 +546,11 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
         auto at = [&](uint32_t c, uint32_t i) -> float { return __uint_as_float(s[c][i]); };
         auto pair = [&](uint32_t c, uint32_t i) { return pack2(at(c, i), at(c, i + 1u)); };
         float scale = factor;
-        if (j.softcap != 0.f) {
+        if (SHAPED && j.softcap != 0.f) {
           scale = 1.0f;
           cap_scores(j, factor, s);
         }
-        if (j.slopes != nullptr) {
+        if (SHAPED && j.slopes != nullptr) {
           const float far = static_cast<float>(pos - k0);
 #pragma unroll
           for (uint32_t c = 0; c < 4u; ++c)
@@ -632,12 +671,12 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   if (warp == 4u * HV) tmem_dealloc(tmem, S::kTmem);
 }
 
-template <uint32_t HD, uint32_t HV>
+template <uint32_t HD, uint32_t HV, bool SHAPED>
 int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stream) {
   using S = Cfg<HD, HV>;
   static std::atomic<uint64_t> set{0};  // devices whose limit is raised
   if (((set.load(std::memory_order_relaxed) >> (job.device & 63u)) & 1u) == 0u || job.device > 63u) {
-    if (cudaFuncSetAttribute(k_attn_prompt<HD, HV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(k_attn_prompt<HD, HV, SHAPED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              S::kBytes) != cudaSuccess) {
       return -1;
     }
@@ -660,7 +699,7 @@ int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stre
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = expand ? 1u : 0u;
-  if (cudaLaunchKernelEx(&cfg, k_attn_prompt<HD, HV>, job, err) != cudaSuccess) return -1;
+  if (cudaLaunchKernelEx(&cfg, k_attn_prompt<HD, HV, SHAPED>, job, err) != cudaSuccess) return -1;
   return expand ? 2 : 1;
 }
 
@@ -672,8 +711,13 @@ int launch_hd(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t s
   // for 32 of 141 with 32/8 heads), as is a long history (43.4 and 47.1 us for
   // 200 rows over 8000 keys at hd 64).
   constexpr uint32_t kOne = HD <= 64u ? 1u : 2u;
-  return job.max_kv <= 1024u ? launch<HD, kOne>(job, chunks, err, stream)
-                             : launch<HD, 2>(job, chunks, err, stream);
+  const bool shaped = job.softcap != 0.f || job.slopes != nullptr;
+  if (job.max_kv <= 1024u) {
+    return shaped ? launch<HD, kOne, true>(job, chunks, err, stream)
+                  : launch<HD, kOne, false>(job, chunks, err, stream);
+  }
+  return shaped ? launch<HD, 2, true>(job, chunks, err, stream)
+                : launch<HD, 2, false>(job, chunks, err, stream);
 }
 
 }  // namespace
