@@ -96,6 +96,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
   // conversion and two clamps, which the pipe of the codes' conversions takes.
   uint32_t* scales = reinterpret_cast<uint32_t*>(smem + S::kScales);
 
+  for (uint32_t b = threadIdx.x; b < 256u; b += kWarps * 32u) scales[b] = scale2(b, b);
+  if (lane < kStages) mbar_init(full + lane, 1);
+  fence_barrier_init();
+  __syncwarp();
+  griddep_wait();
+
   const uint32_t n = blockIdx.z, head = blockIdx.y;
   int32_t q0, q_len, kv;
   if (!attn_request(j, n, &q0, &q_len, &kv)) {
@@ -112,13 +118,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
   const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
   const bool whole = kv <= static_cast<int32_t>(j.chunk);  // no other chunk of this request
 
-  for (uint32_t b = threadIdx.x; b < 256u; b += kWarps * 32u) scales[b] = scale2(b, b);
-  if (lane < kStages) mbar_init(full + lane, 1);
-  fence_barrier_init();
-  __syncwarp();
-
   // The keys that the rows see, and the tiles of this warp among them.
-  const int32_t pre = j.prefix != nullptr ? __ldg(j.prefix + n) : 0;
+  const int32_t pre = j.prefix != nullptr ? ld(j.prefix + n) : 0;
   const Seen first = attn_seen(j, kv - q_len + r0 / group, kv, pre);
   const Seen last = attn_seen(j, kv - q_len + (r0 + rows - 1) / group, kv, pre);
 
@@ -130,9 +131,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     base = at;
     const int32_t i = static_cast<int32_t>(warp) + (at + static_cast<int32_t>(lane)) * static_cast<int32_t>(kWarps);
     const int32_t k = c0 + i * static_cast<int32_t>(kTile);
-    page_a = k < kv ? __ldg(table + (k >> j.cache.page_log2)) : -2;
+    page_a = k < kv ? ld(table + (k >> j.cache.page_log2)) : -2;
     page_b = page_a;
-    if (P16) page_b = k + 16 < kv ? __ldg(table + ((k + 16) >> 4)) : -2;
+    if (P16) page_b = k + 16 < kv ? ld(table + ((k + 16) >> 4)) : -2;
   };
   const uint8_t* const head_data = j.cache.data + static_cast<uint64_t>(head) * j.cache.record;
   // -2: no keys there; other values outside the cache read as zeros.
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
       const uint4* src = reinterpret_cast<const uint4*>(j.q + row * j.ldq + h * HD + t * (HD / 4u));
 #pragma unroll
       for (uint32_t i = 0; i < HD / 32u; ++i) {
-        const uint4 v = __ldg(src + i);
+        const uint4 v = ld(src + i);
         w[4u * i] = v.x;
         w[4u * i + 1u] = v.y;
         w[4u * i + 2u] = v.z;
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
       seen[nt][c] = attn_seen(j, pos[nt][c], kv, pre);
       if (r >= rows) seen[nt][c].lo = seen[nt][c].hi = seen[nt][c].pre = 0;
       slope[nt][c] = j.slopes != nullptr && r < rows
-                         ? __ldg(j.slopes + head * j.group + static_cast<uint32_t>((r0 + r) % group)) * kLog2e
+                         ? ld(j.slopes + head * j.group + static_cast<uint32_t>((r0 + r) % group)) * kLog2e
                          : 0.f;
     }
   }
@@ -550,7 +551,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
   }
   if (bad_page && lane == 0u) atomicOr(error_flag, kErrKvSlot);
 
-  griddep_launch_dependents();  // k_attn_join may be set up
   // Join the warps: rows of (m, l, O) in shared memory over the rings.
   __syncthreads();
   constexpr uint32_t kLd = HD + 4u;
@@ -690,9 +690,9 @@ cudaError_t launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStrea
   }
   AttnJob j = job;
   j.row_blocks = (job.max_q * job.group + 8u * NT - 1u) / (8u * NT);
-  k_attn_decode<HD, NT, P16><<<dim3(chunks * j.row_blocks, job.cache.kv_heads, job.seqs), kWarps * 32,
-                               Smem<HD, NT>::kBytes, stream>>>(j, err);
-  return cudaSuccess;
+  return launch_early(k_attn_decode<HD, NT, P16>,
+                      dim3(chunks * j.row_blocks, job.cache.kv_heads, job.seqs), kWarps * 32,
+                      Smem<HD, NT>::kBytes, stream, j, err);
 }
 
 template <uint32_t HD, uint32_t NT>
@@ -717,17 +717,10 @@ int launch_attn_join(const AttnJob& job, cudaStream_t stream, uint32_t* error_fl
   // A block a row and head where there are many chunks (74 of one request:
   // 32 blocks), else a warp.
   const bool many = chunks > 8u;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(many ? cells : (cells + kJoinWarps - 1u) / kJoinWarps, job.seqs);
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t st = many ? cudaLaunchKernelEx(&cfg, k_attn_join<kJoinWarps>, job, error_flag)
-                              : cudaLaunchKernelEx(&cfg, k_attn_join<1>, job, error_flag);
+  const dim3 grid(many ? cells : (cells + kJoinWarps - 1u) / kJoinWarps, job.seqs);
+  const cudaError_t st =
+      many ? launch_early(k_attn_join<kJoinWarps>, grid, kJoinWarps * 32, 0, stream, job, error_flag)
+           : launch_early(k_attn_join<1>, grid, kJoinWarps * 32, 0, stream, job, error_flag);
   return st == cudaSuccess ? 1 : -1;
 }
 

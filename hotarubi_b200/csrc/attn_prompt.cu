@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256)
     const uint32_t key = i / (HD / 8u), w = i % (HD / 8u);
     uint32_t x[2] = {0u, 0u};
     if (key < keys) {
-      const uint32_t page = static_cast<uint32_t>(__ldg(table + ((k0 + key) >> j.cache.page_log2)));
+      const uint32_t page = static_cast<uint32_t>(ld(table + ((k0 + key) >> j.cache.page_log2)));
       if (page < j.cache.pages) {
         const uint32_t in = (k0 + key) & (j.cache.page - 1u);
         const uint8_t* rec = kv_record(j.cache, page, head) + in * (HD / 2u) + 4u * w;
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(256)
     const uint32_t key = i / (HD / 32u), b = i % (HD / 32u);
     uint32_t x[2] = {127u, 127u};
     if (key < keys) {
-      const uint32_t page = static_cast<uint32_t>(__ldg(table + ((k0 + key) >> j.cache.page_log2)));
+      const uint32_t page = static_cast<uint32_t>(ld(table + ((k0 + key) >> j.cache.page_log2)));
       if (page < j.cache.pages) {
         const uint32_t in = (k0 + key) & (j.cache.page - 1u);
         const uint8_t* rec = kv_record(j.cache, page, head) + kv_kscales(j.cache) + in * (HD / 32u) + b;
@@ -330,12 +330,15 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   if (c0 >= kv && c0 > 0) return;
   const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
   const uint32_t base = first_tile(j, n);
-  if (base + (static_cast<uint32_t>(kv) + kKeys - 1u) / kKeys > j.tiles_cap) return;  // reported too
+  if (base + (static_cast<uint32_t>(kv) + kKeys - 1u) / kKeys > j.tiles_cap) {  // reported too
+    griddep_wait();  // what follows in the stream must find k_kv_expand done
+    return;
+  }
   const uint32_t halves = HV == 2u && r1 - r0 > static_cast<int32_t>(kHalf) ? 2u : 1u;
 
   // The tiles that some row of the block sees: numbers 0 .. gap - 1 and
   // resume .. of the chunk's, `count` in all.
-  const int32_t pre = j.prefix != nullptr ? __ldg(j.prefix + n) : 0;
+  const int32_t pre = j.prefix != nullptr ? ld(j.prefix + n) : 0;
   const int32_t group = static_cast<int32_t>(j.group);
   const Seen first = attn_seen(j, kv - q_len + r0 / group, kv, pre);
   const Seen last = attn_seen(j, kv - q_len + (r1 - 1) / group, kv, pre);
@@ -360,7 +363,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   uint4 q_row[HD / 8u];
 #pragma unroll
   for (uint32_t i = 0; i < HD / 8u; ++i) {
-    q_row[i] = mine ? __ldg(reinterpret_cast<const uint4*>(j.q + row * j.ldq + static_cast<uint64_t>(qh) * HD) + i)
+    q_row[i] = mine ? ld(reinterpret_cast<const uint4*>(j.q + row * j.ldq + static_cast<uint64_t>(qh) * HD) + i)
                     : make_uint4(0, 0, 0, 0);
   }
 
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
     const int32_t pos = kv - q_len + (mine ? r : r0) / group;
     Seen seen = attn_seen(j, pos, kv, pre);
     if (!mine) seen.lo = seen.hi = seen.pre = 0;
-    const float slope = SHAPED && j.slopes != nullptr ? __ldg(j.slopes + qh) * kLog2e : 0.f;
+    const float slope = SHAPED && j.slopes != nullptr ? ld(j.slopes + qh) * kLog2e : 0.f;
     const uint32_t lanes = ((warp & 3u) * 32u) << 16;
     const uint32_t t_s = tmem + lanes + 128u * h, t_o = tmem + lanes + S::kO + 128u * h;
     float m = -INFINITY, l = 0.f;
@@ -688,18 +691,17 @@ int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stre
   if (expand) {
     k_kv_expand<HD><<<dim3(key_tiles, job.cache.kv_heads, job.seqs), 256, 0, stream>>>(job, err);
   }
-  // Its blocks may start, load Q and set up while k_kv_expand still runs.
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(chunks * job.cache.kv_heads, q_tiles, job.seqs);
-  cfg.blockDim = dim3(S::kThreads);
-  cfg.dynamicSmemBytes = S::kBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = expand ? 1u : 0u;
-  if (cudaLaunchKernelEx(&cfg, k_attn_prompt<HD, HV, SHAPED>, job, err) != cudaSuccess) return -1;
+  // Its blocks may start, load Q and set up while k_kv_expand still runs: that
+  // is launched when all before it is done, so Q and the lists are there.
+  const dim3 grid(chunks * job.cache.kv_heads, q_tiles, job.seqs);
+  if (expand) {
+    if (launch_early(k_attn_prompt<HD, HV, SHAPED>, grid, S::kThreads, S::kBytes, stream, job, err) !=
+        cudaSuccess) {
+      return -1;
+    }
+  } else {
+    k_attn_prompt<HD, HV, SHAPED><<<grid, S::kThreads, S::kBytes, stream>>>(job, err);
+  }
   return expand ? 2 : 1;
 }
 

@@ -17,6 +17,7 @@
 
 #include "hrb_kv.cuh"
 #include "hrb_serve.cuh"
+#include "sm100.cuh"
 
 namespace hrb {
 namespace {
@@ -65,6 +66,7 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t t0 = blockIdx.x * kThreads, t1 = min(t0 + kThreads, j.max_tokens);
   const uint32_t share = (j.seqs + gridDim.x - 1u) / gridDim.x;
   const uint32_t s0 = blockIdx.x * share, s1 = s0 + share;
+  sm100::griddep_wait();
   const uint32_t head = j.head_in != nullptr ? static_cast<uint32_t>(*j.head_in) : 0u;
   const uint32_t mask = (1u << j.page_log2) - 1u;
   bool bad = false, short_of = false;
@@ -74,8 +76,8 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t i = c + threadIdx.x;
     int32_t cached = 0, fresh = 0;
     if (i < j.seqs) {
-      cached = __ldg(j.cached + i);
-      fresh = __ldg(j.fresh + i);
+      cached = ld(j.cached + i);
+      fresh = ld(j.fresh + i);
       bad |= cached < 0 || fresh < 0;
       cached = max(cached, 0);
       fresh = max(fresh, 0);
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(kThreads)
           page = *entry;
         } else {
           const uint64_t f = uint64_t{head} + r.base + (n - r.have);
-          if (f < j.nfree) page = __ldg(j.free_pages + f);
+          if (f < j.nfree) page = ld(j.free_pages + f);
           if ((p & mask) == 0) *entry = page;
         }
       }
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(kThreads)
 
 void launch_block_tables(const BlocksJob& job, uint32_t* error_flag, cudaStream_t stream) {
   const uint32_t grid = (job.max_tokens + kThreads - 1u) / kThreads;
-  k_block_tables<<<grid != 0 ? grid : 1u, kThreads, 0, stream>>>(job, error_flag);
+  launch_early(k_block_tables, dim3(grid != 0 ? grid : 1u), kThreads, 0, stream, job, error_flag);
 }
 
 }  // namespace hrb

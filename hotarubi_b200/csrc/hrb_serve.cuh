@@ -12,6 +12,33 @@
 
 namespace hrb {
 
+// A plain load.  The kernels start before the one that writes their inputs
+// has ended (launch_early), so these are not loads of data that is constant
+// for the kernel's life (__ldg, which may also be moved ahead of the wait).
+template <typename T>
+__device__ __forceinline__ T ld(const T* p) {
+  return *p;
+}
+
+// Launches a kernel that may start while the one before it in the stream
+// still runs (programmatic stream serialisation): it calls griddep_wait()
+// before it touches global memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, uint32_t threads, size_t smem,
+                         cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 // Context fields for serve.cu (defined in capi.cu).
 cudaStream_t ctx_stream(const hrb_ctx* ctx, void* stream);
 uint32_t* ctx_error_word(const hrb_ctx* ctx);
@@ -79,9 +106,9 @@ struct AttnJob {
 // says there are; false (and no rows) where the lists contradict it.
 __device__ __forceinline__ bool attn_request(const AttnJob& j, uint32_t n, int32_t* q0,
                                              int32_t* q_len, int32_t* kv) {
-  *q0 = __ldg(j.q_start + n);
-  *q_len = __ldg(j.q_start + n + 1u) - *q0;
-  const int32_t len = __ldg(j.kv_len + n);
+  *q0 = ld(j.q_start + n);
+  *q_len = ld(j.q_start + n + 1u) - *q0;
+  const int32_t len = ld(j.kv_len + n);
   *kv = min(max(len, 0), static_cast<int32_t>(j.max_kv));
   if (*q0 >= 0 && *q_len >= 0 && *q_len <= static_cast<int32_t>(j.max_q) &&
       *q0 <= static_cast<int32_t>(j.total_q) - *q_len && len <= static_cast<int32_t>(j.max_kv)) {

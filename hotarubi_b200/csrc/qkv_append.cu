@@ -24,6 +24,7 @@
 
 #include "hrb_attn.cuh"
 #include "hrb_kernels.cuh"
+#include "sm100.cuh"
 
 namespace hrb {
 namespace {
@@ -39,18 +40,18 @@ __device__ __forceinline__ uint4 load4(const void* base, uint64_t at) {
   if constexpr (BF16) {
     const uint16_t* p = static_cast<const uint16_t*>(base) + at;
     if constexpr (VEC) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      const uint2 v = ld(reinterpret_cast<const uint2*>(p));
       return make_uint4(v.x, v.y, 0, 0);
     } else {
-      return make_uint4(__ldg(p) | (static_cast<uint32_t>(__ldg(p + 1)) << 16),
-                        __ldg(p + 2) | (static_cast<uint32_t>(__ldg(p + 3)) << 16), 0, 0);
+      return make_uint4(ld(p) | (static_cast<uint32_t>(ld(p + 1)) << 16),
+                        ld(p + 2) | (static_cast<uint32_t>(ld(p + 3)) << 16), 0, 0);
     }
   } else {
     const uint32_t* p = static_cast<const uint32_t*>(base) + at;
     if constexpr (VEC) {
-      return __ldg(reinterpret_cast<const uint4*>(p));
+      return ld(reinterpret_cast<const uint4*>(p));
     } else {
-      return make_uint4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+      return make_uint4(ld(p), ld(p + 1), ld(p + 2), ld(p + 3));
     }
   }
 }
@@ -82,7 +83,7 @@ struct Steps {
 };
 
 template <uint32_t HD, bool BF16, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32, BF16 ? 8 : 6)
+__global__ void __launch_bounds__(kWarps * 32, BF16 ? 7 : 6)
     k_qkv(const QkvJob j, const Steps st, uint32_t* __restrict__ error_flag) {
   constexpr uint32_t kLanes = HD / 8u;                  // lanes a head
   constexpr uint32_t kSpan = HD == 96u ? 16u : kLanes;  // lanes set apart for one
@@ -96,6 +97,7 @@ __global__ void __launch_bounds__(kWarps * 32, BF16 ? 8 : 6)
   const uint32_t begin = (unit - t * st.runs) * st.run;
   const uint32_t end = min(begin + st.run, st.all);
   bool bad_slot = false, non_finite = false;
+  sm100::griddep_wait();
 
   // The lane's cos and sin, of its dims 4l + i (c = 0) and hd / 2 further
   // (c = 1): half-split dims d use pair d mod half, interleaved dims 2p and
@@ -108,9 +110,9 @@ __global__ void __launch_bounds__(kWarps * 32, BF16 ? 8 : 6)
     si[0][i] = si[1][i] = 0.f;
   }
   if (j.rope != nullptr && begin < st.k) {
-    const int32_t p0 = __ldg(j.pos + t);
-    const int32_t p1 = j.cut[0] < j.half ? __ldg(j.pos + j.tokens + t) : 0;
-    const int32_t p2 = j.cut[1] < j.half ? __ldg(j.pos + 2ull * j.tokens + t) : 0;
+    const int32_t p0 = ld(j.pos + t);
+    const int32_t p1 = j.cut[0] < j.half ? ld(j.pos + j.tokens + t) : 0;
+    const int32_t p2 = j.cut[1] < j.half ? ld(j.pos + 2ull * j.tokens + t) : 0;
 #pragma unroll
     for (uint32_t c = 0; c < 2u; ++c) {
       if (c == 1u && paired) {
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(kWarps * 32, BF16 ? 8 : 6)
         const uint32_t p = j.interleaved ? d / 2u : d < j.half ? d : d - j.half;
         const int32_t pos = p < j.cut[0] ? p0 : p < j.cut[1] ? p1 : p2;
         if (pos >= 0 && static_cast<uint32_t>(pos) < j.max_pos) {
-          const float2 v = __ldg(j.rope + static_cast<uint64_t>(pos) * j.half + p);
+          const float2 v = ld(j.rope + static_cast<uint64_t>(pos) * j.half + p);
           co[c][i] = v.x;
           si[c][i] = v.y;
         } else {
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(kWarps * 32, BF16 ? 8 : 6)
       }
     }
   }
-  const int32_t slot = __ldg(j.slots + t);
+  const int32_t slot = ld(j.slots + t);
   const bool cached = slot >= 0 &&
                       (static_cast<uint32_t>(slot) >> j.cache.page_log2) < j.cache.pages;
   bad_slot |= slot >= 0 && !cached;
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(kWarps * 32, BF16 ? 8 : 6)
     for (uint32_t c = 0; c < 2u; ++c)
 #pragma unroll
       for (uint32_t i = 0; i < 4u; ++i) {
-        w[c][i] = norm && on ? __ldg(j.norm[W < 2u ? W : 0u] + 4u * l + c * (HD / 2u) + i) : 0.f;
+        w[c][i] = norm && on ? ld(j.norm[W < 2u ? W : 0u] + 4u * l + c * (HD / 2u) + i) : 0.f;
       }
     uint16_t* to = W == 0u ? static_cast<uint16_t*>(j.q_out) + t * j.ldqo + h * HD + 4u * l : nullptr;
     uint8_t* rec = nullptr;
@@ -399,14 +401,15 @@ __device__ __forceinline__ void put16(void* out, uint64_t at, const uint32_t (&h
 
 template <uint32_t DT>
 __global__ void __launch_bounds__(256)
-    k_kv_read(const KvCache c, const int32_t* __restrict__ slots, uint32_t tokens, FastDiv row_div,
+    k_kv_read(const KvCache c, const int32_t* slots, uint32_t tokens, FastDiv row_div,
               FastDiv head_div, void* k, void* v, uint32_t* __restrict__ error_flag) {
   const uint32_t t0 = blockIdx.x * kTokens, n = min(kTokens, tokens - t0) * row_div.d;
   bool bad = false;
+  sm100::griddep_wait();
   for (uint32_t i = threadIdx.x; i < n; i += 256u) {
     const uint32_t t = fast_div(i, row_div), x = i - t * row_div.d;
     const uint32_t head = fast_div(x, head_div), w = x - head * head_div.d;
-    const int32_t slot = __ldg(slots + t0 + t);
+    const int32_t slot = ld(slots + t0 + t);
     const uint32_t page = static_cast<uint32_t>(slot) >> c.page_log2;
     const bool there = slot >= 0 && page < c.pages;
     bad |= slot >= 0 && !there;
@@ -461,11 +464,11 @@ void launch_hd(const QkvJob& job, bool bf16, bool vec, uint32_t* err, int sm_cou
   const uint64_t units = static_cast<uint64_t>(job.tokens) * st.runs;
   const unsigned grid = static_cast<unsigned>((units + kWarps - 1u) / kWarps);
   if (bf16) {
-    if (vec) k_qkv<HD, true, true><<<grid, kWarps * 32, 0, stream>>>(job, st, err);
-    else k_qkv<HD, true, false><<<grid, kWarps * 32, 0, stream>>>(job, st, err);
+    if (vec) launch_early(k_qkv<HD, true, true>, dim3(grid), kWarps * 32, 0, stream, job, st, err);
+    else launch_early(k_qkv<HD, true, false>, dim3(grid), kWarps * 32, 0, stream, job, st, err);
   } else {
-    if (vec) k_qkv<HD, false, true><<<grid, kWarps * 32, 0, stream>>>(job, st, err);
-    else k_qkv<HD, false, false><<<grid, kWarps * 32, 0, stream>>>(job, st, err);
+    if (vec) launch_early(k_qkv<HD, false, true>, dim3(grid), kWarps * 32, 0, stream, job, st, err);
+    else launch_early(k_qkv<HD, false, false>, dim3(grid), kWarps * 32, 0, stream, job, st, err);
   }
 }
 
@@ -487,11 +490,14 @@ void launch_kv_read(const KvCache& cache, const int32_t* slots, uint32_t tokens,
   const FastDiv head = make_fast_div(cache.hd / 16u);
   const unsigned grid = (tokens + kTokens - 1u) / kTokens;
   if (dtype == HRB_DT_F32) {
-    k_kv_read<HRB_DT_F32><<<grid, 256, 0, stream>>>(cache, slots, tokens, row, head, k, v, error_flag);
+    launch_early(k_kv_read<HRB_DT_F32>, dim3(grid), 256, 0, stream, cache, slots, tokens, row, head, k, v,
+                 error_flag);
   } else if (dtype == HRB_DT_BF16) {
-    k_kv_read<HRB_DT_BF16><<<grid, 256, 0, stream>>>(cache, slots, tokens, row, head, k, v, error_flag);
+    launch_early(k_kv_read<HRB_DT_BF16>, dim3(grid), 256, 0, stream, cache, slots, tokens, row, head, k, v,
+                 error_flag);
   } else {
-    k_kv_read<HRB_DT_E5M2><<<grid, 256, 0, stream>>>(cache, slots, tokens, row, head, k, v, error_flag);
+    launch_early(k_kv_read<HRB_DT_E5M2>, dim3(grid), 256, 0, stream, cache, slots, tokens, row, head, k, v,
+                 error_flag);
   }
 }
 
