@@ -1,5 +1,5 @@
 // hrb_attention for few rows a request (single tokens, a few speculated
-// ones): the cache is streamed once and everything else hides behind it.
+// ones): the cache is streamed once.
 //
 // A block serves one request, one key/value head and a chunk of its keys;
 // the rows that read that head (rows of q times query heads a key/value head)
@@ -22,7 +22,11 @@
 // Chunks of one request are joined by k_attn_join from the rows' (m, l, O)
 // in FP32.
 //
-// Bound by HBM for long histories: hd + hd / 16 bytes a key and head.
+// Its floor is HBM: hd + hd / 16 bytes a key and head.  Measured (32/8 heads of
+// 128): 64 requests of up to 16384 keys 177 us, 4.1 TB/s, 63 % of a copy's
+// rate; one request of 131071 keys 43 us; one of 241 keys (15/5 heads of 64)
+// 4.4 us.  Bound by the lanes' work: with all pages in L2 it takes as long, 64 %
+// of the issue slots and 54 % of the ALU pipe (the conversions) are used.
 #include <cuda_fp16.h>
 
 #include <atomic>
