@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(kThreads)
           if ((p & mask) == 0) *entry = page;
         }
       }
-      if (page >= 0) {
+      // A page whose slots pass 31 bits is no page of any cache.
+      if (page >= 0 && page <= static_cast<int32_t>(0x7FFFFFFFu >> j.page_log2)) {
         slot = static_cast<int32_t>((static_cast<uint32_t>(page) << j.page_log2) + (p & mask));
       } else {
         short_of = true;

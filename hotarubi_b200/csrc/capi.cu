@@ -891,7 +891,7 @@ hrb_status hrb_sync(hrb_ctx* ctx) {
   HRB_CUDA(ctx, cudaMemcpy(&flag, ctx->d_error, sizeof flag, cudaMemcpyDeviceToHost));
   if (flag != 0) {
     HRB_CUDA(ctx, cudaMemset(ctx->d_error, 0, sizeof(uint32_t)));
-    if (flag & 2u) return fail(ctx, HRB_ECUDA, "a tensor-core GEMM timed out waiting");
+    if (flag & 2u) return fail(ctx, HRB_ECUDA, "a tensor-core kernel timed out waiting");
     if (flag & 4u) return fail(ctx, HRB_EDATA, "a GACC entry names a row outside the feature rows");
     if (flag & hrb::kErrRowOutside) {
       return fail(ctx, HRB_EDATA, "a ROW_INDEXED entry names a unit outside the DDR window");

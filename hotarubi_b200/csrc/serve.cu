@@ -70,7 +70,7 @@ hrb_status check_attn(hrb_ctx* ctx, const hrb_attn_desc* d) {
   }
   if (d->seqs > 65535u) return refuse(ctx, HRB_EINVAL, "%u requests (at most 65535)", d->seqs);
   if (d->total_q > 0x7FFFFFFFu || d->max_q > d->total_q || d->max_kv > 0x7FFFFFFFu ||
-      uint64_t{d->max_q} * (d->heads / d->cache.kv_heads) > 256ull * 65535u) {
+      uint64_t{d->max_q} * (d->heads / d->cache.kv_heads) > 128ull * 65535u) {
     return refuse(ctx, HRB_EINVAL, "%u rows, at most %u a request, %u keys", d->total_q, d->max_q,
                   d->max_kv);
   }

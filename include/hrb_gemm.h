@@ -700,8 +700,10 @@ typedef enum hrb_dtype {
  * tokens from q_start[seqs] up to max_tokens become -1 and 0 (a step padded
  * to a fixed size).  Tokens whose page is missing (the free list has run out,
  * the row is full, or the table's own entry is negative) get slot -1, a table
- * entry without a page becomes -1, tokens past max_tokens are dropped, a
- * negative length counts as 0: hrb_sync then reports HRB_EDATA. */
+ * entry without a page becomes -1, tokens past max_tokens are dropped (with
+ * the table entries of pages that only they use), a negative length counts as
+ * 0: hrb_sync then reports HRB_EDATA.  The step's tokens together, and each
+ * request's, are fewer than 2^31. */
 typedef struct hrb_blocks_desc {
   uint32_t seqs;               /* at most 65536 */
   uint32_t page;               /* tokens a page, as hrb_kv_cache's */
@@ -776,7 +778,7 @@ HRB_API hrb_status hrb_kv_read(hrb_ctx* ctx, const hrb_kv_cache* cache, const in
  * and has an Inf or NaN in q gives NaN.  Scores,
  * softmax statistics and sums are FP32; q and the softmax weights enter the
  * tensor cores as FP16 (q after a power-of-two scaling of its row).
- * A negative length is no keys.  A table entry outside the cache reads as a
+ * Rows of q past q_start[seqs] are left alone.  A negative length is no keys.  A table entry outside the cache reads as a
  * page of zeros; a request whose rows or keys pass the descriptor's bounds
  * (total_q, max_q, max_kv) is left out: both are HRB_EDATA from hrb_sync. */
 typedef struct hrb_attn_desc {
@@ -785,7 +787,8 @@ typedef struct hrb_attn_desc {
   const void* q;             /* BF16 [total_q][ldq], 16-byte aligned rows */
   uint64_t ldq;
   const int32_t* q_start;    /* [seqs + 1] */
-  uint32_t total_q, max_q;   /* rows of q and out; most rows of one request */
+  uint32_t total_q, max_q;   /* rows of q and out; most rows of one request, times
+                                query heads a key/value head at most 2^23 - 128 */
   const int32_t* kv_len;     /* [seqs] */
   uint32_t max_kv;           /* most keys of one request */
   uint64_t total_kv;         /* keys of all requests together, or more; 0: seqs * max_kv */

@@ -509,6 +509,63 @@ def test_attention_mxint8_copy(hrb, rule, lens, heads, kvh, hd):
             (mass == 0).any()
 
 
+@pytest.mark.parametrize("lens", [[(1, 0), (2, 0)], [(100, 0), (7, 0)]])
+def test_attention_without_any_key(hrb, lens):
+    rng = np.random.default_rng(6)
+    s = Step(rng, lens, 4, 2, 64, 16)
+    assert not s.run(hrb, oq=True).any()
+    assert not s.codes[:, :256].any()
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(48, 1, 64), (64, 2, 128), (40, 2, 96), (9, 1, 32)])
+@pytest.mark.parametrize("lens", [DECODE, [(40, 90), (2, 400)]], ids=["one", "prompt"])
+def test_attention_many_query_heads_a_head(hrb, heads, kvh, hd, lens):
+    rng = np.random.default_rng(heads)
+    s = Step(rng, lens, heads, kvh, hd, 16)
+    close(s.run(hrb), *s.want())
+
+
+def test_attention_more_keys_than_total_kv_says(hrb):
+    """Scratch for 5 tiles: the first request's four fit, the others are left
+    out and reported; the next call is not disturbed."""
+    rng = np.random.default_rng(7)
+    s = Step(rng, [(100, 500), (100, 500), (100, 400)], 4, 2, 64, 16)
+    want, mass = s.want()
+    with pytest.raises(capi.HrbError) as e:
+        s.run(hrb, total_kv=300)
+    assert e.value.status == capi.HRB_EDATA
+    torch.cuda.synchronize()
+    got = s.out.double().cpu().numpy().reshape(s.rows, s.heads, s.hd)
+    close(got[:100], want[:100], mass[:100])
+    assert (got[100:] == 5.0).all()
+    close(s.run(hrb, total_kv=1400), want, mass)
+
+
+def test_block_tables_refuse_pages_past_31_bits(hrb):
+    table = np.full((1, 4), -1, np.int32)
+    free = np.array([(1 << 28) + 3, 5], np.int32)
+    got, err = run_tables(hrb, [0], [20], free, 0, table, 16, 20)
+    assert err is not None and err.status == capi.HRB_EDATA
+    assert (got[1][:16] == -1).all() and np.array_equal(got[1][16:], 80 + np.arange(4))
+
+
+@pytest.mark.parametrize("hd,rot", [(128, 64), (96, 48), (64, 24), (32, 16)])
+def test_qkv_append_partial_half_split_rotation(hrb, hd, rot):
+    rng = np.random.default_rng(hd + rot)
+    c = ref.Cache(4, 16, 2, hd)
+    x = [rng.standard_normal((50, h, hd)).astype(np.float32) for h in (5, 2, 2)]
+    table, pos = capi.rope_table(64, rot), rng.integers(0, 64, (1, 50))
+    slots = rng.permutation(64)[:50]
+    q, got, used, err = run_qkv(hrb, c, x, 5, table=table, pos=pos, rot=rot, sections=(rot // 2,), slots=slots)
+    assert err is None
+    want = ref.norm_rotate(x[0], None, 0, table, pos, rot, False, (rot // 2,))
+    pair = np.abs(x[0]) + np.abs(x[0]).max(-1, keepdims=True)
+    assert (np.abs(q - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -19 * pair).all()
+    k = ref.norm_rotate(x[1], None, 0, table, pos, rot, False, (rot // 2,))
+    for t in range(50):
+        check_codes(got.read(slots[t])[0], k[t], exact=False)
+
+
 def test_attention_extreme_scores(hrb):
     """Scores of thousands (one key takes all), and queries near BF16's ends."""
     rng = np.random.default_rng(12)
