@@ -125,47 +125,49 @@ __global__ void __launch_bounds__(256)
     return;
   }
   const uint32_t keys = min(kKeys, static_cast<uint32_t>(kv) - k0);
-  // The tile's codes, a word a thread at a time; keys past the end and pages
-  // outside the cache are zeros.
+  // The second 64 keys of a request's last tile are not read where it has
+  // none there (the products stop before them): not written either.
+  const uint32_t span = keys <= 64u ? 64u : kKeys;
+  // A block of 32 dims of a key's K and V, and its scales, a thread at a time;
+  // keys past the end and pages outside the cache are zeros.
   bool bad = false;
   const int32_t* table = j.table + static_cast<uint64_t>(n) * j.table_ld;
-  for (uint32_t i = threadIdx.x; i < kKeys * (HD / 8u); i += 256u) {
-    const uint32_t key = i / (HD / 8u), w = i % (HD / 8u);
-    uint32_t x[2] = {0u, 0u};
+#pragma unroll
+  for (uint32_t i = threadIdx.x; i < kKeys * (HD / 32u); i += 256u) {
+    const uint32_t key = i / (HD / 32u), b = i % (HD / 32u);
+    uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    uint32_t sb[2] = {127u, 127u};
     if (key < keys) {
       const uint32_t page = static_cast<uint32_t>(ld(table + ((k0 + key) >> j.cache.page_log2)));
       if (page < j.cache.pages) {
         const uint32_t in = (k0 + key) & (j.cache.page - 1u);
-        const uint8_t* rec = kv_record(j.cache, page, head) + in * (HD / 2u) + 4u * w;
-        x[0] = *reinterpret_cast<const uint32_t*>(rec);
-        x[1] = *reinterpret_cast<const uint32_t*>(rec + kv_vcodes(j.cache));
+        const uint8_t* rec = kv_record(j.cache, page, head);
+#pragma unroll
+        for (uint32_t p = 0; p < 2u; ++p) {
+          const uint8_t* part = rec + (p == 0u ? 0u : kv_vcodes(j.cache));
+          x[p] = ld(reinterpret_cast<const uint4*>(part + in * (HD / 2u) + 16u * b));
+          sb[p] = part[kv_kscales(j.cache) + in * (HD / 32u) + b];
+        }
       } else {
         bad = true;
       }
     }
-    *reinterpret_cast<uint32_t*>(&codes[0][key * kLd + 4u * w]) = x[0];
-    *reinterpret_cast<uint32_t*>(&codes[1][key * kLd + 4u * w]) = x[1];
-  }
-  for (uint32_t i = threadIdx.x; i < kKeys * (HD / 32u); i += 256u) {
-    const uint32_t key = i / (HD / 32u), b = i % (HD / 32u);
-    uint32_t x[2] = {127u, 127u};
-    if (key < keys) {
-      const uint32_t page = static_cast<uint32_t>(ld(table + ((k0 + key) >> j.cache.page_log2)));
-      if (page < j.cache.pages) {
-        const uint32_t in = (k0 + key) & (j.cache.page - 1u);
-        const uint8_t* rec = kv_record(j.cache, page, head) + kv_kscales(j.cache) + in * (HD / 32u) + b;
-        x[0] = rec[0];
-        x[1] = rec[kv_vcodes(j.cache)];
-      }
+#pragma unroll
+    for (uint32_t p = 0; p < 2u; ++p) {
+      uint32_t* to = reinterpret_cast<uint32_t*>(&codes[p][key * kLd + 16u * b]);
+      to[0] = x[p].x;
+      to[1] = x[p].y;
+      to[2] = x[p].z;
+      to[3] = x[p].w;
+      scales[p][i] = static_cast<uint8_t>(sb[p]);
     }
-    scales[0][i] = static_cast<uint8_t>(x[0]);
-    scales[1][i] = static_cast<uint8_t>(x[1]);
   }
   if (bad) atomicOr(error_flag, kErrKvSlot);
   __syncthreads();
   uint8_t* out = j.tiles + (static_cast<uint64_t>(head) * j.tiles_cap + tile) * tile_bytes(HD);
   // K: 16 bytes (8 dims of a key) a step, neighbours in a row.
-  for (uint32_t i = threadIdx.x; i < kKeys * (HD / 8u); i += 256u) {
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < span * (HD / 8u); i += 256u) {
     const uint32_t key = i / (HD / 8u), u = i % (HD / 8u);
     const uint32_t b = scales[0][key * (HD / 32u) + u / 4u];
     *reinterpret_cast<uint4*>(out + k_place(key, u)) =
@@ -175,6 +177,7 @@ __global__ void __launch_bounds__(256)
   out += k_bytes(HD);
   for (uint32_t i = threadIdx.x; i < (kKeys / 8u) * (HD / 8u); i += 256u) {
     const uint32_t kg = i % (kKeys / 8u), dg = i / (kKeys / 8u);
+    if (8u * kg >= span) continue;
     uint32_t w[8], sb[8], h[8][4];
 #pragma unroll
     for (uint32_t r = 0; r < 8u; ++r) {
