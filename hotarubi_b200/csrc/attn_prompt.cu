@@ -261,45 +261,51 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// A row's raw scores to softcap log2(e) tanh(factor s / softcap).  Where all
-// of a warp's arguments are under 1/2, tanh is its power series up to x^11
-// (the next term is under 4.4e-7 there) on the FMA pipe; else 1 - 2 / (1 +
-// e^2x).
-__device__ __forceinline__ void cap_scores(const AttnJob& j, float factor, uint32_t (&s)[4][32]) {
-  const float f = factor * j.cap_inv;
-  const uint64_t f2 = pack2(f, f);
-  float top[4];
+// A row's raw scores to softcap log2(e) tanh(factor s / softcap).  Where a
+// warp's arguments are all small, tanh is its power series on the FMA pipe: up
+// to x^7 under 1/4 and x^11 under 1/2 (the next terms are under 9e-8 and 4.4e-7
+// there); else 1 - 2 / (1 + e^2x).
+template <uint32_t TERMS>
+__device__ __forceinline__ void tanh_series(uint32_t (&s)[4][32], float f, float b) {
+  constexpr float kSeries[6] = {1.f, -1.f / 3.f, 2.f / 15.f, -17.f / 315.f, 62.f / 2835.f, -1382.f / 155925.f};
+  uint64_t a[TERMS];
 #pragma unroll
-  for (uint32_t c = 0; c < 4u; ++c) {
-    top[c] = 0.f;
+  for (uint32_t t = 0; t < TERMS; ++t) a[t] = pack2(b * kSeries[t], b * kSeries[t]);
+  const uint64_t f2 = pack2(f, f);
+#pragma unroll
+  for (uint32_t c = 0; c < 4u; ++c)
 #pragma unroll
     for (uint32_t i = 0; i < 32u; i += 2u) {
-      top[c] = fmaxf(fmaxf(top[c], fabsf(__uint_as_float(s[c][i]))), fabsf(__uint_as_float(s[c][i + 1u])));
+      const uint64_t x = mul_2(pack2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1u])), f2);
+      const uint64_t u = mul_2(x, x);
+      uint64_t r = a[TERMS - 1u];
+#pragma unroll
+      for (uint32_t t = TERMS - 1u; t > 0u; --t) r = fma_2(r, u, a[t - 1u]);
+      const float2 y = unpack2(mul_2(r, x));
+      s[c][i] = __float_as_uint(y.x);
+      s[c][i + 1u] = __float_as_uint(y.y);
     }
-  }
-  const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+}
+
+__device__ __forceinline__ void cap_scores(const AttnJob& j, float factor, uint32_t (&s)[4][32]) {
+  const float f = factor * j.cap_inv;
+  float top[8];
+#pragma unroll
+  for (uint32_t c = 0; c < 8u; ++c) top[c] = 0.f;
+#pragma unroll
+  for (uint32_t i = 0; i < 16u; i += 2u)
+#pragma unroll
+    for (uint32_t c = 0; c < 8u; ++c) {
+      const uint32_t at = 16u * (c & 1u) + i;
+      top[c] = max3(top[c], fabsf(__uint_as_float(s[c >> 1][at])), fabsf(__uint_as_float(s[c >> 1][at + 1u])));
+    }
+  const float high = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]),
+                          fmaxf(top[6], top[7])) * f;
   const float b = j.cap_out;
-  if (__all_sync(0xFFFFFFFFu, high < 0.5f)) {
-    const uint64_t a1 = pack2(b, b), a3 = pack2(b * (-1.f / 3.f), b * (-1.f / 3.f));
-    const uint64_t a5 = pack2(b * (2.f / 15.f), b * (2.f / 15.f));
-    const uint64_t a7 = pack2(b * (-17.f / 315.f), b * (-17.f / 315.f));
-    const uint64_t a9 = pack2(b * (62.f / 2835.f), b * (62.f / 2835.f));
-    const uint64_t a11 = pack2(b * (-1382.f / 155925.f), b * (-1382.f / 155925.f));
-#pragma unroll
-    for (uint32_t c = 0; c < 4u; ++c)
-#pragma unroll
-      for (uint32_t i = 0; i < 32u; i += 2u) {
-        const uint64_t x = mul_2(pack2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1u])), f2);
-        const uint64_t u = mul_2(x, x);
-        uint64_t r = fma_2(u, a11, a9);
-        r = fma_2(r, u, a7);
-        r = fma_2(r, u, a5);
-        r = fma_2(r, u, a3);
-        r = fma_2(r, u, a1);
-        const float2 y = unpack2(mul_2(r, x));
-        s[c][i] = __float_as_uint(y.x);
-        s[c][i + 1u] = __float_as_uint(y.y);
-      }
+  if (__all_sync(0xFFFFFFFFu, high < 0.25f)) {
+    tanh_series<4>(s, f, b);
+  } else if (__all_sync(0xFFFFFFFFu, high < 0.5f)) {
+    tanh_series<6>(s, f, b);
   } else {
 #pragma unroll
     for (uint32_t c = 0; c < 4u; ++c)
