@@ -111,7 +111,10 @@ __global__ void __launch_bounds__(256)
   constexpr uint32_t kLd = HD / 2u + 4u;  // padded row of codes in shared memory
   __shared__ __align__(16) uint8_t codes[2][kKeys * kLd];
   __shared__ uint8_t scales[2][kKeys * (HD / 32u)];
-  griddep_launch_dependents();  // k_attn_prompt may set up meanwhile
+  // First what comes before in the stream is done; then k_attn_prompt may set
+  // up, and load Q, while this runs.
+  griddep_wait();
+  griddep_launch_dependents();
   const uint32_t n = blockIdx.z, head = blockIdx.y, k0 = blockIdx.x * kKeys;
   int32_t q0, q_len, kv;
   if (!attn_request(j, n, &q0, &q_len, &kv)) {
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
 
   // The tiles that some row of the block sees: numbers 0 .. gap - 1 and
   // resume .. of the chunk's, `count` in all.
-  const int32_t pre = j.prefix != nullptr ? ld(j.prefix + n) : 0;
+  const int32_t pre = j.prefix != nullptr ? __ldcg(j.prefix + n) : 0;
   const int32_t group = static_cast<int32_t>(j.group);
   const Seen first = attn_seen(j, kv - q_len + r0 / group, kv, pre);
   const Seen last = attn_seen(j, kv - q_len + (r1 - 1) / group, kv, pre);
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   uint4 q_row[HD / 8u];
 #pragma unroll
   for (uint32_t i = 0; i < HD / 8u; ++i) {
-    q_row[i] = mine ? ld(reinterpret_cast<const uint4*>(j.q + row * j.ldq + static_cast<uint64_t>(qh) * HD) + i)
+    q_row[i] = mine ? __ldcg(reinterpret_cast<const uint4*>(j.q + row * j.ldq + static_cast<uint64_t>(qh) * HD) + i)
                     : make_uint4(0, 0, 0, 0);
   }
 
@@ -709,10 +712,13 @@ int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stre
   const uint32_t q_tiles = (job.max_q * job.group + HV * kHalf - 1u) / (HV * kHalf);
   const bool expand = key_tiles != 0u;
   if (expand) {
-    k_kv_expand<HD><<<dim3(key_tiles, job.cache.kv_heads, job.seqs), 256, 0, stream>>>(job, err);
+    if (launch_early(k_kv_expand<HD>, dim3(key_tiles, job.cache.kv_heads, job.seqs), 256, 0, stream, job,
+                     err) != cudaSuccess) {
+      return -1;
+    }
   }
   // Its blocks may start, load Q and set up while k_kv_expand still runs: that
-  // is launched when all before it is done, so Q and the lists are there.
+  // lets them when all before it is done, so Q and the lists are there.
   const dim3 grid(chunks * job.cache.kv_heads, q_tiles, job.seqs);
   if (expand) {
     if (launch_early(k_attn_prompt<HD, HV, SHAPED>, grid, S::kThreads, S::kBytes, stream, job, err) !=

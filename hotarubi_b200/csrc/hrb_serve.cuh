@@ -106,9 +106,10 @@ struct AttnJob {
 // says there are; false (and no rows) where the lists contradict it.
 __device__ __forceinline__ bool attn_request(const AttnJob& j, uint32_t n, int32_t* q0,
                                              int32_t* q_len, int32_t* kv) {
-  *q0 = ld(j.q_start + n);
-  *q_len = ld(j.q_start + n + 1u) - *q0;
-  const int32_t len = ld(j.kv_len + n);
+  // From L2: k_attn_prompt asks before it waits.
+  *q0 = __ldcg(j.q_start + n);
+  *q_len = __ldcg(j.q_start + n + 1u) - *q0;
+  const int32_t len = __ldcg(j.kv_len + n);
   *kv = min(max(len, 0), static_cast<int32_t>(j.max_kv));
   if (*q0 >= 0 && *q_len >= 0 && *q_len <= static_cast<int32_t>(j.max_q) &&
       *q0 <= static_cast<int32_t>(j.total_q) - *q_len && len <= static_cast<int32_t>(j.max_kv)) {
