@@ -149,9 +149,7 @@ __device__ __forceinline__ uint16_t attn_bf16(float x) {
   return r;
 }
 
-// Requests of at most kDecodeRows rows of q times query heads a key/value
-// head.  Returns the launches, or -1.
-constexpr uint32_t kDecodeRows = 32u;
+// Any number of rows; few (serve.cu).  Returns the launches, or -1.
 uint32_t attn_decode_chunk(const AttnJob& job, uint64_t total_kv, int sm_count);
 int launch_attn_decode(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream);
 

@@ -160,11 +160,17 @@ hrb::AttnJob attn_job(const hrb_ctx* ctx, const hrb_attn_desc* d) {
 
 uint64_t up256(uint64_t x) { return (x + 255u) / 256u * 256u; }
 
-// Few rows a request stream its keys once through mma.sync; more go to the
-// prompt kernel.  Measured at the border, rows 48 of 15/5 heads of 64: 64
-// requests of 2000 keys 187 us there (in two blocks of rows) and 199 us here,
-// one of 30000 keys 53 and 45 us.
-bool decoding(const hrb::AttnJob& j) { return j.max_q * j.group <= hrb::kDecodeRows; }
+// Whether a call takes the decoding kernel, in blocks of 32 rows, or the
+// prompt kernel.  Measured, 32/8 heads of 128 unless said (decoding, prompt):
+//   28 rows (28/4 heads), 64 requests of 2000 keys         49 and 177 us
+//   64 rows, one request of 200, 2000, 30000 keys          14 and 12, 19 and 23, 49 and 73 us
+//   64 rows, 64 requests of 500, 4000 keys                 81 and 96, 340 and 536 us
+//   96 rows, one of 2000, 30000; 64 of 500, 4000 keys      22 and 24, 64 and 75, 121 and 99, 505 and 540 us
+//   128 rows, one of 30000; 64 of 4000 keys                81 and 63, 599 and 439 us
+bool decoding(const hrb::AttnJob& j) {
+  const uint32_t rows = j.max_q * j.group;
+  return rows <= 32u || (rows <= 64u && j.max_kv > 256u) || (rows <= 96u && j.max_kv > 1024u);
+}
 
 // Fills in how the call is split and where its scratch lies from `base`
 // (null: to learn the size).  Returns the scratch bytes.
