@@ -481,7 +481,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     for (uint32_t hf = 0; hf < 2u; ++hf) {
       const uint8_t* vc = tile + Geo::kV + hf * Geo::kCodeHalf;
       const uint8_t* vs = tile + Geo::kVs + hf * Geo::kScaleHalf;
-      constexpr uint32_t kWords = (HD + 63u) / 64u;  // words of codes a lane and key (the last half used at hd 96 and 32)
+      // Words of codes a lane and key (the last half used at hd 96 and 32).
+      constexpr uint32_t kWords = (HD + 63u) / 64u;
       uint32_t w[4][kWords], sc[2][2];
 #pragma unroll
       for (uint32_t r = 0; r < 4u; ++r) {  // keys 2t, 2t + 1, 2t + 8, 2t + 9

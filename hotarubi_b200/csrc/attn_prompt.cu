@@ -421,84 +421,84 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     }
-  if (warp == 4u * HV + 1u) {
-    if (lane == 0u) {
-      griddep_wait();  // k_kv_expand's tiles
-      const uint8_t* src = j.tiles + (static_cast<uint64_t>(head) * j.tiles_cap + base +
-                                      static_cast<uint32_t>(c0) / kKeys) * tile_bytes(HD);
-      int32_t it = 0;
-      for (; it < count; ++it) {
-        const uint32_t st = static_cast<uint32_t>(it) % kNs, ph = (static_cast<uint32_t>(it) / kNs) & 1u;
-        const bool wait = it >= static_cast<int32_t>(kNs);
-        const uint8_t* tile = src + static_cast<uint64_t>(tile_at(it)) * tile_bytes(HD);
-        if (wait && !mbar_wait(k_empty + st, ph ^ 1u, error_flag)) break;
-        mbar_arrive_expect_tx(k_full + st, k_bytes(HD));
-        bulk_g2s(smem + S::kK + st * k_bytes(HD), tile, k_bytes(HD), k_full + st);
-        if (wait && !mbar_wait(v_empty + st, ph ^ 1u, error_flag)) break;
-        mbar_arrive_expect_tx(v_full + st, v_bytes(HD));
-        bulk_g2s(smem + S::kV + st * v_bytes(HD), tile + k_bytes(HD), v_bytes(HD), v_full + st);
-      }
-      // Nothing of this block's may still be arriving when it ends.
-      for (int32_t w = max(it - static_cast<int32_t>(kNs), 0); w < min(it + 1, count); ++w) {
-        const uint32_t st = static_cast<uint32_t>(w) % kNs, ph = (static_cast<uint32_t>(w) / kNs) & 1u;
-        if (w < it && !mbar_wait(v_full + st, ph, error_flag)) break;
-        if (w == it && !mbar_wait(k_full + st, ph, error_flag, 1000u)) break;
-      }
-    }
-  } else if (warp == 4u * HV) {
-    if (lane == 0u && count > 0) {
-      const uint32_t q_at = desc_low(smem_addr(smem)), k_at = desc_low(smem_addr(smem + S::kK));
-      const uint32_t v_at = desc_low(smem_addr(smem + S::kV));
-      auto scores = [&](uint32_t h, uint32_t st) {
-        const uint32_t a = here(q_at + h * (k_bytes(HD) / 16u));
-        const uint32_t b = here(k_at + st * (k_bytes(HD) / 16u));
-#pragma unroll
-        for (uint32_t k = 0; k < HD / 16u; ++k) {
-          const uint32_t off = ((k >> 2) * (kKeys * kRowB) + 32u * (k & 3u)) / 16u;
-          mma_ss(tmem + 128u * h, a + off, b + off, idesc_f16(128, 128), k != 0u);
+    if (warp == 4u * HV + 1u) {
+      if (lane == 0u) {
+        griddep_wait();  // k_kv_expand's tiles
+        const uint8_t* src = j.tiles + (static_cast<uint64_t>(head) * j.tiles_cap + base +
+                                        static_cast<uint32_t>(c0) / kKeys) * tile_bytes(HD);
+        int32_t it = 0;
+        for (; it < count; ++it) {
+          const uint32_t st = static_cast<uint32_t>(it) % kNs, ph = (static_cast<uint32_t>(it) / kNs) & 1u;
+          const bool wait = it >= static_cast<int32_t>(kNs);
+          const uint8_t* tile = src + static_cast<uint64_t>(tile_at(it)) * tile_bytes(HD);
+          if (wait && !mbar_wait(k_empty + st, ph ^ 1u, error_flag)) break;
+          mbar_arrive_expect_tx(k_full + st, k_bytes(HD));
+          bulk_g2s(smem + S::kK + st * k_bytes(HD), tile, k_bytes(HD), k_full + st);
+          if (wait && !mbar_wait(v_empty + st, ph ^ 1u, error_flag)) break;
+          mbar_arrive_expect_tx(v_full + st, v_bytes(HD));
+          bulk_g2s(smem + S::kV + st * v_bytes(HD), tile + k_bytes(HD), v_bytes(HD), v_full + st);
         }
-        mma_commit(s_full + h);
-      };
-      bool ok = mbar_wait(q_full, 0, error_flag) && mbar_wait(k_full, 0, error_flag);
-      if (ok) {
-        tc_fence_after();
-        for (uint32_t h = 0; h < halves; ++h) scores(h, 0);
-        mma_commit(k_empty);
+        // Nothing of this block's may still be arriving when it ends.
+        for (int32_t w = max(it - static_cast<int32_t>(kNs), 0); w < min(it + 1, count); ++w) {
+          const uint32_t st = static_cast<uint32_t>(w) % kNs, ph = (static_cast<uint32_t>(w) / kNs) & 1u;
+          if (w < it && !mbar_wait(v_full + st, ph, error_flag)) break;
+          if (w == it && !mbar_wait(k_full + st, ph, error_flag, 1000u)) break;
+        }
       }
-      for (int32_t it = 0; it < count && ok; ++it) {
-        const uint32_t st = static_cast<uint32_t>(it) % kNs, ph = (static_cast<uint32_t>(it) / kNs) & 1u;
-        const uint32_t nst = static_cast<uint32_t>(it + 1) % kNs;
-        const bool more = it + 1 < count;
-        // Both tiles' arrivals first: the softmax's are then the only waits
-        // between the products.
-        ok = mbar_wait(v_full + st, ph, error_flag) &&
-             (!more || mbar_wait(k_full + nst, (static_cast<uint32_t>(it + 1) / kNs) & 1u, error_flag));
-        for (uint32_t h = 0; h < halves && ok; ++h) {
-          const uint32_t a = here(tmem + 128u * h), b = here(v_at + st * (v_bytes(HD) / 16u));
-          const uint32_t d = tmem + S::kO + 128u * h;
+    } else if (warp == 4u * HV) {
+      if (lane == 0u && count > 0) {
+        const uint32_t q_at = desc_low(smem_addr(smem)), k_at = desc_low(smem_addr(smem + S::kK));
+        const uint32_t v_at = desc_low(smem_addr(smem + S::kV));
+        auto scores = [&](uint32_t h, uint32_t st) {
+          const uint32_t a = here(q_at + h * (k_bytes(HD) / 16u));
+          const uint32_t b = here(k_at + st * (k_bytes(HD) / 16u));
 #pragma unroll
-          for (uint32_t k = 0; k < kKeys / 16u; ++k) {
-            if (k == 4u && last_half && !more) break;
-            if ((k & 3u) == 0u) {  // 64 keys' weights
-              ok = mbar_wait(p_full + 2u * h + (k >> 2), static_cast<uint32_t>(it) & 1u, error_flag);
-              if (!ok) break;
-              tc_fence_after();
+          for (uint32_t k = 0; k < HD / 16u; ++k) {
+            const uint32_t off = ((k >> 2) * (kKeys * kRowB) + 32u * (k & 3u)) / 16u;
+            mma_ss(tmem + 128u * h, a + off, b + off, idesc_f16(128, 128), k != 0u);
+          }
+          mma_commit(s_full + h);
+        };
+        bool ok = mbar_wait(q_full, 0, error_flag) && mbar_wait(k_full, 0, error_flag);
+        if (ok) {
+          tc_fence_after();
+          for (uint32_t h = 0; h < halves; ++h) scores(h, 0);
+          mma_commit(k_empty);
+        }
+        for (int32_t it = 0; it < count && ok; ++it) {
+          const uint32_t st = static_cast<uint32_t>(it) % kNs, ph = (static_cast<uint32_t>(it) / kNs) & 1u;
+          const uint32_t nst = static_cast<uint32_t>(it + 1) % kNs;
+          const bool more = it + 1 < count;
+          // Both tiles' arrivals first: the softmax's are then the only waits
+          // between the products.
+          ok = mbar_wait(v_full + st, ph, error_flag) &&
+               (!more || mbar_wait(k_full + nst, (static_cast<uint32_t>(it + 1) / kNs) & 1u, error_flag));
+          for (uint32_t h = 0; h < halves && ok; ++h) {
+            const uint32_t a = here(tmem + 128u * h), b = here(v_at + st * (v_bytes(HD) / 16u));
+            const uint32_t d = tmem + S::kO + 128u * h;
+#pragma unroll
+            for (uint32_t k = 0; k < kKeys / 16u; ++k) {
+              if (k == 4u && last_half && !more) break;
+              if ((k & 3u) == 0u) {  // 64 keys' weights
+                ok = mbar_wait(p_full + 2u * h + (k >> 2), static_cast<uint32_t>(it) & 1u, error_flag);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              mma_ts(d, a + 8u * k, b + ((k >> 2) * (HD * kRowB) + 32u * (k & 3u)) / 16u, idesc_f16(128, HD),
+                     it != 0 || k != 0u);
             }
-            mma_ts(d, a + 8u * k, b + ((k >> 2) * (HD * kRowB) + 32u * (k & 3u)) / 16u, idesc_f16(128, HD),
-                   it != 0 || k != 0u);
+            if (!ok) break;
+            if (more) {
+              scores(h, nst);
+            } else {
+              mma_commit(o_full + h);
+            }
           }
-          if (!ok) break;
-          if (more) {
-            scores(h, nst);
-          } else {
-            mma_commit(o_full + h);
-          }
+          mma_commit(v_empty + st);
+          if (more) mma_commit(k_empty + nst);
         }
-        mma_commit(v_empty + st);
-        if (more) mma_commit(k_empty + nst);
       }
     }
-  }
   } else {
     if constexpr (HV == 2u) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");

@@ -45,12 +45,10 @@ __device__ __forceinline__ uint8_t* kv_record(const KvCache& c, uint32_t page, u
   return c.data + static_cast<uint64_t>(page) * c.page_stride +
          static_cast<uint64_t>(head) * c.record;
 }
-// Offsets in a record: K codes at 0, then K scales, V codes, V scales.
+// Offsets in a record: K codes at 0, then K scales, V codes; V scales are as far
+// from the V codes as K scales from the K codes.
 __device__ __forceinline__ uint32_t kv_kscales(const KvCache& c) { return c.page * (c.hd / 2u); }
 __device__ __forceinline__ uint32_t kv_vcodes(const KvCache& c) { return c.record / 2u; }
-__device__ __forceinline__ uint32_t kv_vscales(const KvCache& c) {
-  return c.record / 2u + c.page * (c.hd / 2u);
-}
 
 // The exponent of a block whose largest magnitude has these FP32 bits.
 __device__ __forceinline__ int32_t kv_block_exp(uint32_t top_bits) {
@@ -70,21 +68,10 @@ __device__ __forceinline__ uint32_t e2m1_pair(float lo, float hi) {
   return r;
 }
 
-// A byte of two E2M1 codes as two FP16 values, the low nibble's in the low
-// half.
-__device__ __forceinline__ uint32_t e2m1_to_f16x2(uint32_t byte) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 b;\n\t"
-      "cvt.u8.u32 b, %1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
-      : "=r"(r)
-      : "r"(byte));
-  return r;
-}
-
-// The same for the four bytes of a word: one conversion a byte, no shifts
-// (measured: 152 values a ns and SM, against 74 for shifts, masks and a
-// multiplication that place the code's bits in an FP16).
+// The four bytes of a word, two E2M1 codes each, as pairs of FP16 values, a
+// byte's low nibble in the low half: one conversion a byte, no shifts (measured:
+// 152 values a ns and SM, against 74 for shifts, masks and a multiplication that
+// place the code's bits in an FP16).
 __device__ __forceinline__ void e2m1x8_to_f16x2(uint32_t word, uint32_t (&r)[4]) {
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
@@ -94,14 +81,6 @@ __device__ __forceinline__ void e2m1x8_to_f16x2(uint32_t word, uint32_t (&r)[4])
       "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
       : "r"(word));
-}
-
-// A scale byte as the FP32 power of two it stands for, held to the cache's
-// range of exponents.
-__device__ __forceinline__ float kv_scale(uint32_t byte) {
-  const uint32_t b = min(max(byte, static_cast<uint32_t>(127 + kKvExpMin)),
-                         static_cast<uint32_t>(127 + kKvExpMax));
-  return __uint_as_float(b << 23);
 }
 
 }  // namespace hrb
