@@ -228,6 +228,10 @@ constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_low(uint32_t smem_byte_addr) {
   return static_cast<uint32_t>(desc_sw128(smem_byte_addr));
 }
+// The lowest n bits (none for n below 0, all from 32).
+__device__ __forceinline__ uint32_t low_bits(int32_t n) {
+  return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1u;
+}
 // Keeps a value where it is: what is added to it is not computed ahead for a
 // whole loop, in registers the issuing thread does not have.
 __device__ __forceinline__ uint32_t here(uint32_t x) {
@@ -543,7 +547,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
     }
     const int32_t pos = kv - q_len + (mine ? r : r0) / group;
     Seen seen = attn_seen(j, pos, kv, pre);
-    if (!mine) seen.lo = seen.hi = seen.pre = 0;
+    const bool idle = !__any_sync(0xFFFFFFFFu, mine);  // a warp without rows
     const float slope = SHAPED && j.slopes != nullptr ? ld(j.slopes + qh) * kLog2e : 0.f;
     const uint32_t lanes = ((warp & 3u) * 32u) << 16;
     const uint32_t t_s = tmem + lanes + 128u * h, t_o = tmem + lanes + S::kO + 128u * h;
@@ -553,9 +557,14 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
       for (int32_t it = 0; it < count; ++it) {
         ok = mbar_wait(s_full + h, static_cast<uint32_t>(it) & 1u, error_flag);
         if (!__all_sync(0xFFFFFFFFu, ok)) break;
+        const bool both = !(last_half && it == count - 1);  // 64s of keys
+        if (idle) {  // what its rows of P and O hold does not matter
+          mbar_arrive(p_full + 2u * h);
+          if (both) mbar_arrive(p_full + 2u * h + 1u);
+          continue;
+        }
         tc_fence_after();
         uint32_t s[4][32];
-        const bool both = !(last_half && it == count - 1);  // 64s of keys
         tmem_ld32(t_s, s[0]);
         tmem_ld32(t_s + 32u, s[1]);
         if (both) {
@@ -587,17 +596,18 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
             }
           scale = 1.0f;
         }
-        const bool clear = (k0 >= seen.lo && k1 <= seen.hi) || k1 <= seen.pre;
+        const bool clear = !mine || (k0 >= seen.lo && k1 <= seen.hi) || k1 <= seen.pre;
         if (!__all_sync(0xFFFFFFFFu, clear)) {
-          // Keys [a, b) and [0, c) of the tile.
-          const int32_t a = seen.lo - k0, b = seen.hi - k0, cc = seen.pre - k0;
+          // Keys [lo, hi) and [0, pre) of the tile, a bit each.
 #pragma unroll
-          for (uint32_t c = 0; c < 4u; ++c)
+          for (uint32_t c = 0; c < 4u; ++c) {
+            const int32_t k = k0 + static_cast<int32_t>(32u * c);
+            const uint32_t see = (low_bits(seen.hi - k) & ~low_bits(seen.lo - k)) | low_bits(seen.pre - k);
 #pragma unroll
             for (uint32_t i = 0; i < 32u; ++i) {
-              const int32_t k = static_cast<int32_t>(32u * c + i);
-              if (!((k >= a && k < b) || k < cc)) s[c][i] = 0xFF800000u;
+              if (((see >> i) & 1u) == 0u) s[c][i] = 0xFF800000u;
             }
+          }
         }
         float top[8];
 #pragma unroll
@@ -655,8 +665,8 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
         const float2 all = unpack2(add_2(add_2(sum[0], sum[1]), add_2(sum[2], sum[3])));
         l += all.x + all.y;
       }
-      if (count > 0 && ok) ok = mbar_wait(o_full + h, 0, error_flag);
-      if (__all_sync(0xFFFFFFFFu, ok)) {
+      if (count > 0 && ok && !idle) ok = mbar_wait(o_full + h, 0, error_flag);
+      if (__all_sync(0xFFFFFFFFu, ok && !idle)) {
         tc_fence_after();
         if (odd && (seen.lo < seen.hi || seen.pre > 0)) l = NAN;
         const float inv = l != 0.f ? 1.0f / l : 0.f;
