@@ -24,8 +24,8 @@
 // (attn_decode.cu) joins the rows' (m, l, O).
 //
 // Its floor is the tensor cores: 4 hd FLOP a pair of query and key that see
-// each other.  Measured: a prompt of 8191 tokens, 32/8 heads of 128, 481 us,
-// 1143 TFLOP/s, 69 % of a large BF16 product's rate.  A tile takes about 3600
+// each other.  Measured: a prompt of 8191 tokens, 32/8 heads of 128, 478 us,
+// 1148 TFLOP/s, 69 % of a large BF16 product's rate.  A tile takes about 3600
 // clocks for both halves, the tensor cores work 2048 of them: a half's softmax
 // (2200) and its products (1200 with the waits) follow each other.  Two S of
 // 64 keys a half, which would let a softmax run ahead, measured slower: a
@@ -416,12 +416,13 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // A softmax thread holds a row's 128 scores (split 224/56: 482 us for the
-  // 8191 prompt, 232/40 499, 216/72 481).  Registers at launch: 384 x
-  // 168 = 256 x 216 + 128 x 72 (HV 2), 256 x 128 = 128 x 200 + 128 x 56.
+  // A softmax thread holds a row's 128 scores (split 224/56: 475 us for the
+  // 8191 prompt but 124.5 for 512 tokens over 8703 keys, 216/72 481 and 119.5,
+  // 208/88 478 and 119.6).  Registers at launch: 384 x 168 = 256 x 208 +
+  // 128 x 88 (HV 2), 256 x 128 = 128 x 200 + 128 x 56.
   if (warp >= 4u * HV) {
     if constexpr (HV == 2u) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     }
@@ -505,7 +506,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
     }
   } else {
     if constexpr (HV == 2u) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     }
@@ -743,16 +744,14 @@ int launch(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stre
 
 template <uint32_t HD>
 int launch_hd(const AttnJob& job, uint32_t chunks, uint32_t* err, cudaStream_t stream) {
-  // Short histories of small heads: 32 prompts of 141 tokens (15/5 heads of
-  // 64) 42.7 us with two halves a block, 35.2 with one; one of 512 20.9 and
-  // 16.9.  At hd 128 one half a block is slower throughout (98.6 and 103.2 us
-  // for 32 of 141 with 32/8 heads), as is a long history (43.4 and 47.1 us for
-  // 200 rows over 8000 keys at hd 64).
-  constexpr uint32_t kOne = HD <= 64u ? 1u : 2u;
+  // One half a block for short histories, two for long ones: 32 prompts of 141
+  // tokens 23.7 and 28.9 us (15/5 heads of 64), 70.9 and 72.6 us (32/8 of 128);
+  // one of 512 12.1 and 15.1 us (64); 80 rows over 500 keys, 32 requests, 36.7
+  // and 43.9 us (128); but 600 rows over 3000 keys 58.2 and 54.7 us (64).
   const bool shaped = job.softcap != 0.f || job.slopes != nullptr;
   if (job.max_kv <= 1024u) {
-    return shaped ? launch<HD, kOne, true>(job, chunks, err, stream)
-                  : launch<HD, kOne, false>(job, chunks, err, stream);
+    return shaped ? launch<HD, 1, true>(job, chunks, err, stream)
+                  : launch<HD, 1, false>(job, chunks, err, stream);
   }
   return shaped ? launch<HD, 2, true>(job, chunks, err, stream)
                 : launch<HD, 2, false>(job, chunks, err, stream);

@@ -162,14 +162,18 @@ uint64_t up256(uint64_t x) { return (x + 255u) / 256u * 256u; }
 
 // Whether a call takes the decoding kernel, in blocks of 32 rows, or the
 // prompt kernel.  Measured, 32/8 heads of 128 unless said (decoding, prompt):
-//   28 rows (28/4 heads), 64 requests of 2000 keys         49 and 177 us
-//   64 rows, one request of 200, 2000, 30000 keys          14 and 12, 19 and 23, 49 and 73 us
-//   64 rows, 64 requests of 500, 4000 keys                 81 and 96, 340 and 536 us
-//   96 rows, one of 2000, 30000; 64 of 500, 4000 keys      22 and 24, 64 and 75, 121 and 99, 505 and 540 us
-//   128 rows, one of 30000; 64 of 4000 keys                81 and 63, 599 and 439 us
+//   12 rows, one request of 100, 64 of 100 and 500   7 and 9, 16 and 25, 25 and 66 us
+//   28 rows, the same                                12 and 9, 27 and 25, 41 and 67 us
+//   27 rows, the same, 15/5 heads of 64              9 and 7, 19 and 16, 27 and 34 us
+//   64 rows, one request of 200, 2000, 30000 keys    15 and 12, 20 and 20, 49 and 60 us
+//   64 rows, 64 of 500; 16 of 2000; 64 of 4000       82 and 72, 50 and 93, 340 and 439 us
+//   96 rows, the same three                          121 and 87, 96 and 92, 505 and 441 us
+//   96 rows, the same three, 15/5 heads of 64        55 and 35, 33 and 52, 214 and 224 us
+//   126 rows, the same three, 15/5 heads of 64       69 and 35, 61 and 49, 267 and 226 us
 bool decoding(const hrb::AttnJob& j) {
   const uint32_t rows = j.max_q * j.group;
-  return rows <= 32u || (rows <= 64u && j.max_kv > 256u) || (rows <= 96u && j.max_kv > 1024u);
+  return rows <= 16u || (rows <= 32u && j.max_kv > 128u) ||
+         (rows <= (j.cache.hd <= 64u ? 96u : 64u) && j.max_kv > 1024u);
 }
 
 // Fills in how the call is split and where its scratch lies from `base`
