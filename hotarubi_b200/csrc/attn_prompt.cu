@@ -16,8 +16,9 @@
 //   warp 8          issues S_A, S_B and O_A += P_A V, O_B += P_B V
 //                   (tcgen05.mma kind::f16, P from TMEM)
 //   warp 9          bulk copies of K and V^T tiles, two stages each
-// (with one half a block, 0-3, 4 and 5).  While one half's softmax runs, the
-// other half's products do.  m moves only when a row's scores pass it by 2^8,
+// (with one half a block, 0-3, 4 and 5, and one stage at hd 96 and 128).  While
+// one half's softmax runs, the other half's products do; with one half, another
+// block's.  m moves only when a row's scores pass it by 2^8,
 // so O is rarely scaled.
 //
 // Few blocks (a short chunk over a long cache) split the keys; k_attn_join
