@@ -129,18 +129,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
 
   const int32_t* table = j.table + static_cast<uint64_t>(n) * j.table_ld;
   const uint32_t copies = P16 ? 2u : j.cache.page == 32u ? 1u : 4u;
-  // Lane l holds the pages of the warp's tile number base + l.
+  // Lane l holds the pages of the warp's tile number base + l: -2 past the
+  // request's keys, -1 for any negative entry of the table.
   int32_t page_a = -1, page_b = -1, base = 0;
   auto load_pages = [&](int32_t at) {  // tiles number at .. at + 31 of this warp
     base = at;
     const int32_t i = static_cast<int32_t>(warp) + (at + static_cast<int32_t>(lane)) * static_cast<int32_t>(kWarps);
     const int32_t k = c0 + i * static_cast<int32_t>(kTile);
-    page_a = k < kv ? ld(table + (k >> j.cache.page_log2)) : -2;
+    page_a = k < kv ? max(ld(table + (k >> j.cache.page_log2)), -1) : -2;
     page_b = page_a;
-    if (P16) page_b = k + 16 < kv ? ld(table + ((k + 16) >> 4)) : -2;
+    if (P16) page_b = k + 16 < kv ? max(ld(table + ((k + 16) >> 4)), -1) : -2;
   };
   const uint8_t* const head_data = j.cache.data + static_cast<uint64_t>(head) * j.cache.record;
-  // -2: no keys there; other values outside the cache read as zeros.
+  // Pages outside the cache read as zeros.
   auto issue = [&](int32_t number, uint32_t stage) {
     const int32_t i = static_cast<int32_t>(warp) + number * static_cast<int32_t>(kWarps);
     const uint32_t k = static_cast<uint32_t>(c0 + i * static_cast<int32_t>(kTile));

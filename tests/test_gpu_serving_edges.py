@@ -1,0 +1,37 @@
+"""Edges of the serving calls on the GPU: data and arguments outside what the
+calls name, scores and weights near the ends of their types.  Against the
+plain 64-bit forms of serving_ref.py, with test_gpu_serving.py's tolerances
+unless a test says otherwise."""
+import numpy as np
+import pytest
+
+import serving_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from hotarubi_b200 import capi  # noqa: E402
+from test_gpu_serving import Step, check_codes, close, dev, ready, run_qkv  # noqa: E402
+
+
+def rows_of(s):
+    """What a Step's call has written, after an error too."""
+    torch.cuda.synchronize()
+    return s.out.double().cpu().numpy().reshape(s.rows, s.heads, s.hd)
+
+
+@pytest.mark.parametrize("entry", ["pages", -1, -2, -(1 << 31)])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("lens", [[(1, 90), (1, 200)], [(100, 150), (30, 400)]], ids=["one", "prompt"])
+def test_attention_any_entry_outside_the_cache_reads_as_zeros(hrb, lens, page, entry):
+    rng = np.random.default_rng(21)
+    s = Step(rng, lens, 4, 2, 64, page)
+    table = s.table.copy()
+    table[1, 1] = s.pages if entry == "pages" else entry
+    for k in (s.keys, s.values):
+        k[1][page:2 * page] = 0
+    with pytest.raises(capi.HrbError) as e:
+        s.run(hrb, table=table)
+    assert e.value.status == capi.HRB_EDATA
+    close(rows_of(s), *s.want())
