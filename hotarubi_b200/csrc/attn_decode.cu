@@ -646,6 +646,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   const uint64_t row = static_cast<uint64_t>(q0) + r, unit = row * j.heads + h;
   const uint32_t chunks = (static_cast<uint32_t>(kv) + j.chunk - 1u) / j.chunk;
   if (chunks <= 1u) return;
+  // k_attn_prompt left the request out: there is nothing to join.
+  if (j.tiles != nullptr && !attn_tiles_fit(j, attn_first_tile(j, blockIdx.y), kv)) return;
   const uint64_t stride = static_cast<uint64_t>(j.total_q) * j.heads;
   float top = -INFINITY;
   for (uint32_t c = lane; c < chunks; c += 32u) top = fmaxf(top, j.part_ml[c * stride + unit].x);

@@ -45,7 +45,7 @@ namespace {
 
 using namespace sm100;
 
-constexpr uint32_t kKeys = 128;      // keys a tile
+constexpr uint32_t kKeys = kAttnTileKeys;
 constexpr uint32_t kHalf = 128;      // rows a half
 constexpr uint32_t kRowB = 128;      // bytes of a swizzled row
 
@@ -53,22 +53,6 @@ constexpr uint32_t kRowB = 128;      // bytes of a swizzled row
 __host__ __device__ constexpr uint32_t k_bytes(uint32_t hd) { return (hd + 63u) / 64u * kKeys * kRowB; }
 __host__ __device__ constexpr uint32_t v_bytes(uint32_t hd) { return 2u * hd * kRowB; }
 __host__ __device__ constexpr uint32_t tile_bytes(uint32_t hd) { return k_bytes(hd) + v_bytes(hd); }
-
-// First tile in scratch of request n (a whole warp; the same in all lanes):
-// n times the most tiles of a request where the scratch has room for that
-// (tile_stride), else the requests' tiles one after another, which every
-// block adds up from their lengths.
-__device__ __forceinline__ uint32_t first_tile(const AttnJob& j, uint32_t n) {
-  if (j.tile_stride != 0u) return n * j.tile_stride;
-  uint32_t sum = 0;
-  for (uint32_t i = threadIdx.x & 31u; i < n; i += 32u) {
-    int32_t q0, q_len, kv;
-    if (attn_request(j, i, &q0, &q_len, &kv) && q_len > 0) {
-      sum += (static_cast<uint32_t>(kv) + kKeys - 1u) / kKeys;
-    }
-  }
-  return __reduce_add_sync(0xFFFFFFFFu, sum);
-}
 
 // Eight dims of a key (a word of codes) as FP16.
 __device__ __forceinline__ uint4 key_dims(uint32_t word, uint32_t scale) {
@@ -123,7 +107,7 @@ __global__ void __launch_bounds__(256)
     return;
   }
   if (q_len == 0 || k0 >= static_cast<uint32_t>(kv)) return;
-  const uint32_t tile = first_tile(j, n) + blockIdx.x;
+  const uint32_t tile = attn_first_tile(j, n) + blockIdx.x;
   if (tile >= j.tiles_cap) {  // more keys than total_kv said
     if (threadIdx.x == 0u) atomicOr(error_flag, kErrKvSlot);
     return;
@@ -356,8 +340,8 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   const bool whole = kv <= static_cast<int32_t>(j.chunk);
   if (c0 >= kv && c0 > 0) return;
   const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
-  const uint32_t base = first_tile(j, n);
-  if (base + (static_cast<uint32_t>(kv) + kKeys - 1u) / kKeys > j.tiles_cap) {  // reported too
+  const uint32_t base = attn_first_tile(j, n);
+  if (!attn_tiles_fit(j, base, kv)) {  // reported too
     griddep_wait();  // what follows in the stream must find k_kv_expand done
     return;
   }

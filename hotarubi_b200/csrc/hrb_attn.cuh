@@ -14,6 +14,28 @@ namespace hrb {
 constexpr float kLazy = 8.0f;    // log2 of the most a weight may pass 1 before m moves
 constexpr float kLog2e = 1.4426950408889634f;
 
+constexpr uint32_t kAttnTileKeys = 128;  // keys a tile of the prompt kernel
+
+// First tile in scratch of request n (a whole warp; the same in all lanes):
+// n times the most tiles of a request where the scratch has room for that
+// (tile_stride), else the requests' tiles one after another, which every
+// block adds up from their lengths.
+__device__ __forceinline__ uint32_t attn_first_tile(const AttnJob& j, uint32_t n) {
+  if (j.tile_stride != 0u) return n * j.tile_stride;
+  uint32_t sum = 0;
+  for (uint32_t i = threadIdx.x & 31u; i < n; i += 32u) {
+    int32_t q0, q_len, kv;
+    if (attn_request(j, i, &q0, &q_len, &kv) && q_len > 0) {
+      sum += (static_cast<uint32_t>(kv) + kAttnTileKeys - 1u) / kAttnTileKeys;
+    }
+  }
+  return __reduce_add_sync(0xFFFFFFFFu, sum);
+}
+// Whether a request's tiles are in the scratch: total_kv may have said less.
+__device__ __forceinline__ bool attn_tiles_fit(const AttnJob& j, uint32_t first, int32_t kv) {
+  return first + (static_cast<uint32_t>(kv) + kAttnTileKeys - 1u) / kAttnTileKeys <= j.tiles_cap;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -778,9 +778,11 @@ HRB_API hrb_status hrb_kv_read(hrb_ctx* ctx, const hrb_kv_cache* cache, const in
  * and has an Inf or NaN in q gives NaN.  Scores,
  * softmax statistics and sums are FP32; q and the softmax weights enter the
  * tensor cores as FP16 (q after a power-of-two scaling of its row).
- * Rows of q past q_start[seqs] are left alone.  A negative length is no keys.  A table entry outside the cache reads as a
- * page of zeros; a request whose rows or keys pass the descriptor's bounds
- * (total_q, max_q, max_kv) is left out: both are HRB_EDATA from hrb_sync. */
+ * Rows of q past q_start[seqs] are left alone.  A negative length is no keys.
+ * A table entry outside the cache reads as a page of zeros; a request whose
+ * rows or keys pass the descriptor's bounds (total_q, max_q, max_kv, or the
+ * scratch that total_kv gives) is left out, its rows of out left alone: both
+ * are HRB_EDATA from hrb_sync. */
 typedef struct hrb_attn_desc {
   hrb_kv_cache cache;
   uint32_t seqs, heads;

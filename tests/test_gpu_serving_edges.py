@@ -35,3 +35,19 @@ def test_attention_any_entry_outside_the_cache_reads_as_zeros(hrb, lens, page, e
         s.run(hrb, table=table)
     assert e.value.status == capi.HRB_EDATA
     close(rows_of(s), *s.want())
+
+
+def test_attention_more_keys_than_total_kv_says_in_a_split_call(hrb):
+    """Scratch for two tiles: the second request's 24, in six chunks, are left
+    out, and so are its rows, whatever the chunks' scratch held before."""
+    rng = np.random.default_rng(22)
+    s = Step(rng, [(40, 100), (200, 3000)], 4, 2, 64, 16)
+    want, mass = s.want()
+    close(s.run(hrb, total_kv=3100, oq=True), want, mass)   # fills the scratch
+    with pytest.raises(capi.HrbError) as e:
+        s.run(hrb, total_kv=100, oq=True)
+    assert e.value.status == capi.HRB_EDATA
+    got = rows_of(s)
+    close(got[:40], want[:40], mass[:40])
+    assert (got[40:] == 5.0).all()
+    assert (s.codes[40:] == 99).all() and (s.scales[40:] == 99).all()
