@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kWarps * 32, BF16 ? 7 : 6)
 #pragma unroll
             for (uint32_t i = 0; i < 4u; ++i) odd = fmaf(y[c][i], 0.f, odd);
           if (odd != odd) {  // rare: NaN counts as zero, Inf saturates
-            non_finite = true;
+            non_finite |= mine && cached;  // rows that pad a step may hold anything
 #pragma unroll
             for (uint32_t c = 0; c < 2u; ++c)
 #pragma unroll

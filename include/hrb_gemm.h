@@ -738,8 +738,9 @@ HRB_API hrb_status hrb_block_tables(hrb_ctx* ctx, const hrb_blocks_desc* desc, v
  * e = -23.  Arithmetic is FP32, each of the two roundings once.
  * A negative slot caches nothing (q_out is still written).  hrb_sync reports
  * HRB_EDATA for a slot or position outside the cache or the table (nothing is
- * cached; the row is not rotated) and for Inf or NaN in k or v (NaN is cached
- * as 0, Inf saturates).  Two tokens of one call must not share a slot. */
+ * cached; the row is not rotated) and for Inf or NaN in a k or v that is
+ * cached (NaN as 0, Inf saturates).  Two tokens of one call must not share a
+ * slot. */
 typedef struct hrb_qkv_desc {
   hrb_kv_cache cache;
   uint32_t tokens, heads;

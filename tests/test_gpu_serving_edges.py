@@ -51,3 +51,20 @@ def test_attention_more_keys_than_total_kv_says_in_a_split_call(hrb):
     close(got[:40], want[:40], mass[:40])
     assert (got[40:] == 5.0).all()
     assert (s.codes[40:] == 99).all() and (s.scales[40:] == 99).all()
+
+
+@pytest.mark.parametrize("odd", [float("nan"), float("inf")])
+def test_qkv_append_reports_only_what_it_caches(hrb, odd):
+    """Rows that pad a step (slot -1) may hold anything."""
+    rng = np.random.default_rng(23)
+    c = ref.Cache(4, 16, 2, 64)
+    x = [rng.standard_normal((9, h, 64)).astype(np.float32) for h in (4, 2, 2)]
+    slots = np.array([3, 40, 9, 22, 63, 1, -1, -1, -1])
+    for part in x:
+        part[6:] = odd
+    q, got, used, err = run_qkv(hrb, c, x, 4, slots=slots)
+    assert err is None
+    for t in range(6):
+        assert np.array_equal(got.read(slots[t])[1], ref.decode(*ref.encode(x[2][t].astype(np.float64))))
+    x[1][2, 0, 7] = odd
+    assert run_qkv(hrb, c, x, 4, slots=slots)[3].status == capi.HRB_EDATA
