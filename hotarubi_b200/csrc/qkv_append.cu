@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kWarps * 32, BF16 ? 7 : 6)
   const uint32_t t = unit / st.runs;
   const uint32_t begin = (unit - t * st.runs) * st.run;
   const uint32_t end = min(begin + st.run, st.all);
-  bool bad_slot = false, non_finite = false;
+  bool non_finite = false;
   sm100::griddep_wait();
 
   // The lane's cos and sin, of its dims 4l + i (c = 0) and hd / 2 further
@@ -114,12 +114,18 @@ __global__ void __launch_bounds__(kWarps * 32, BF16 ? 7 : 6)
     co[0][i] = co[1][i] = 1.f;
     si[0][i] = si[1][i] = 0.f;
   }
-  if (j.rope != nullptr && begin < st.k) {
-    const int32_t p0 = ld(j.pos + t);
-    const int32_t p1 = j.cut[0] < j.half ? ld(j.pos + j.tokens + t) : 0;
+  // A token with a position outside the table, on an axis that has pairs, is
+  // neither rotated nor cached.
+  bool bad_pos = false;
+  if (j.rope != nullptr) {
+    const int32_t p0 = j.cut[0] > 0u ? ld(j.pos + t) : 0;
+    const int32_t p1 = j.cut[0] < j.cut[1] ? ld(j.pos + j.tokens + t) : 0;
     const int32_t p2 = j.cut[1] < j.half ? ld(j.pos + 2ull * j.tokens + t) : 0;
+    bad_pos = max(max(static_cast<uint32_t>(p0), static_cast<uint32_t>(p1)),
+                  static_cast<uint32_t>(p2)) >= j.max_pos;
 #pragma unroll
     for (uint32_t c = 0; c < 2u; ++c) {
+      if (bad_pos || begin >= st.k) break;
       if (c == 1u && paired) {
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
@@ -139,20 +145,17 @@ __global__ void __launch_bounds__(kWarps * 32, BF16 ? 7 : 6)
         }
         const uint32_t p = j.interleaved ? d / 2u : d < j.half ? d : d - j.half;
         const int32_t pos = p < j.cut[0] ? p0 : p < j.cut[1] ? p1 : p2;
-        if (pos >= 0 && static_cast<uint32_t>(pos) < j.max_pos) {
-          const float2 v = ld(j.rope + static_cast<uint64_t>(pos) * j.half + p);
-          co[c][i] = v.x;
-          si[c][i] = v.y;
-        } else {
-          bad_slot = true;
-        }
+        const float2 v = ld(j.rope + static_cast<uint64_t>(static_cast<uint32_t>(pos)) * j.half + p);
+        co[c][i] = v.x;
+        si[c][i] = v.y;
       }
     }
   }
   const int32_t slot = ld(j.slots + t);
-  const bool cached = slot >= 0 &&
-                      (static_cast<uint32_t>(slot) >> j.cache.page_log2) < j.cache.pages;
-  bad_slot |= slot >= 0 && !cached;
+  const bool in_cache = slot >= 0 &&
+                        (static_cast<uint32_t>(slot) >> j.cache.page_log2) < j.cache.pages;
+  const bool cached = in_cache && !bad_pos;
+  const bool bad_slot = bad_pos || (slot >= 0 && !in_cache);
 
   // Steps [begin, end) of q (W = 0), k (1) or v (2): numbers a .. b of its own.
   auto phase = [&](auto which, uint32_t a, uint32_t b) {

@@ -737,8 +737,9 @@ HRB_API hrb_status hrb_block_tables(hrb_ctx* ctx, const hrb_blocks_desc* desc, v
  * E2M1 nearest x / 2^e, ties to even, saturating at 6; a block of zeros has
  * e = -23.  Arithmetic is FP32, each of the two roundings once.
  * A negative slot caches nothing (q_out is still written).  hrb_sync reports
- * HRB_EDATA for a slot or position outside the cache or the table (nothing is
- * cached; the row is not rotated) and for Inf or NaN in a k or v that is
+ * HRB_EDATA for a slot outside the cache (nothing is cached), for a position
+ * outside the table on an axis that has pairs (nothing is cached; the token's
+ * rows are not rotated, on no axis) and for Inf or NaN in a k or v that is
  * cached (NaN as 0, Inf saturates).  Two tokens of one call must not share a
  * slot. */
 typedef struct hrb_qkv_desc {

@@ -68,3 +68,40 @@ def test_qkv_append_reports_only_what_it_caches(hrb, odd):
         assert np.array_equal(got.read(slots[t])[1], ref.decode(*ref.encode(x[2][t].astype(np.float64))))
     x[1][2, 0, 7] = odd
     assert run_qkv(hrb, c, x, 4, slots=slots)[3].status == capi.HRB_EDATA
+
+
+@pytest.mark.parametrize("sections,bad", [((32,), 0), ((10, 6, 16), 0), ((10, 6, 16), 1),
+                                          ((10, 6, 16), 2), ((0, 12, 20), 1), ((32, 0, 0), 0)])
+def test_qkv_append_a_position_outside_the_table(hrb, sections, bad):
+    """The row keeps its norm, is not rotated on any axis, and nothing is
+    cached; positions of axes without pairs do not matter."""
+    rng = np.random.default_rng(28)
+    tokens = 7
+    c = ref.Cache(4, 16, 2, 64)
+    x = [rng.standard_normal((tokens, h, 64)).astype(np.float32) for h in (20, 2, 2)]
+    w = [(0.5 + rng.random(64)).astype(np.float32) for _ in range(2)]
+    table = capi.rope_table(16, 64)
+    pos = rng.integers(0, 16, (len(sections), tokens))
+    for axis, pairs in enumerate(sections):
+        if pairs == 0:
+            pos[axis] = 1 << 20
+    pos[bad, 3], pos[bad, 5] = 16, -1
+    slots = rng.permutation(64)[:tokens]
+    q, got, used, err = run_qkv(hrb, c, x, 20, w=w, table=table, pos=pos, rot=64, sections=sections,
+                                slots=slots)
+    assert err is not None and err.status == capi.HRB_EDATA
+    good = np.array([t not in (3, 5) for t in range(tokens)])
+    want = ref.norm_rotate(x[0], w[0], 1e-6, None, None, 0, False, ())
+    k = ref.norm_rotate(x[1], w[1], 1e-6, None, None, 0, False, ())
+    spread = np.abs(want) + np.abs(want).max(-1, keepdims=True)
+    inside = np.where((pos >= 0) & (pos < 16), pos, 0)
+    want[good] = ref.norm_rotate(x[0], w[0], 1e-6, table, inside, 64, False, sections)[good]
+    k[good] = ref.norm_rotate(x[1], w[1], 1e-6, table, inside, 64, False, sections)[good]
+    assert (np.abs(q - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -19 * spread).all()
+    for t in range(tokens):
+        gk, gv = got.read(slots[t])
+        if good[t]:
+            check_codes(gk, k[t], exact=False)
+            check_codes(gv, x[2][t].astype(np.float64), exact=True)
+        else:
+            assert not gk.any() and not gv.any()
