@@ -558,9 +558,9 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
           tmem_ld32(t_s + 96u, s[3]);
         }
         tmem_wait_ld();
-        if (!both) {
+        if (!both) {  // masked below, no row sees them; zeros leave a cap's series open
 #pragma unroll
-          for (uint32_t i = 0; i < 32u; ++i) s[2][i] = s[3][i] = 0xFF800000u;
+          for (uint32_t i = 0; i < 32u; ++i) s[2][i] = s[3][i] = 0;
         }
         const int32_t k0 = c0 + tile_at(it) * static_cast<int32_t>(kKeys);
         const int32_t k1 = k0 + static_cast<int32_t>(kKeys);

@@ -105,3 +105,15 @@ def test_qkv_append_a_position_outside_the_table(hrb, sections, bad):
             check_codes(gv, x[2][t].astype(np.float64), exact=True)
         else:
             assert not gk.any() and not gv.any()
+
+
+CAPS = [1.0, 30.0, 1e4, 1e6, 1e9, 1e30]
+
+
+@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_caps_of_any_size_on_every_last_tile(hrb, cap, hd):
+    """Prompts whose last tile of 128 keys holds 1, 64, 65 and 128."""
+    rng = np.random.default_rng(24)
+    s = Step(rng, [(90, 129), (90, 192), (90, 193), (90, 256), (90, 1)], 4, 2, hd, 16)
+    close(s.run(hrb, softcap=cap), *s.want(softcap=cap))
