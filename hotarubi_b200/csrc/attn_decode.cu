@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
   float factor[NT][2], m[NT][2], l[NT][2], slope[NT][2];
   Seen seen[NT][2];
   int32_t pos[NT][2];
-  const bool capped = j.softcap != 0.f;
+  const bool capped = j.softcap != 0.f, wide = j.softcap > kWideCap;
 #pragma unroll
   for (uint32_t nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -393,19 +393,31 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     const int32_t k1 = k0 + static_cast<int32_t>(kTile);
     const bool clear = (k0 >= last.lo && k1 <= first.hi) || k1 <= first.pre;
     const bool shaped = capped || j.slopes != nullptr;
-    if (shaped) {
-      // cap tanh(x / cap) = cap (1 - 2 / (1 + e^(2x / cap)))
+    if (wide) {  // a branch of its own: the others' arithmetic is not doubled
 #pragma unroll
       for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (uint32_t c = 0; c < 8u; ++c) {
-          float x = s[nt][c / 4u][c & 3u] * factor[nt][c & 1u];
-          if (capped) x = j.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(x * j.cap_in)));
+          float& x = s[nt][c / 4u][c & 3u];
+          x = cap_score<true>(j, x * factor[nt][c & 1u]);
+        }
+    } else if (shaped) {
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) {
+          float& x = s[nt][c / 4u][c & 3u];
+          x *= factor[nt][c & 1u];
+          if (capped) x = cap_score<false>(j, x);
+        }
+    }
+    if (j.slopes != nullptr) {
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (uint32_t c = 0; c < 8u; ++c) {
           const int32_t k = k0 + static_cast<int32_t>(16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g);
-          if (j.slopes != nullptr) {
-            x -= slope[nt][c & 1u] * fabsf(static_cast<float>(pos[nt][c & 1u] - k));
-          }
-          s[nt][c / 4u][c & 3u] = x;
+          s[nt][c / 4u][c & 3u] -= slope[nt][c & 1u] * fabsf(static_cast<float>(pos[nt][c & 1u] - k));
         }
     }
     if (!clear) {

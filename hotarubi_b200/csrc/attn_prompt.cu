@@ -256,7 +256,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // A row's raw scores to softcap log2(e) tanh(factor s / softcap).  Where a
 // warp's arguments are all small, tanh is its power series on the FMA pipe: up
 // to x^7 under 1/4 and x^11 under 1/2 (the next terms are under 9e-8 and 4.4e-7
-// there); else 1 - 2 / (1 + e^2x).
+// there); else cap_score, a score at a time.
 template <uint32_t TERMS>
 __device__ __forceinline__ void tanh_series(uint32_t (&s)[4][32], float f, float b) {
   constexpr float kSeries[6] = {1.f, -1.f / 3.f, 2.f / 15.f, -17.f / 315.f, 62.f / 2835.f, -1382.f / 155925.f};
@@ -298,13 +298,19 @@ __device__ __forceinline__ void cap_scores(const AttnJob& j, float factor, uint3
     tanh_series<4>(s, f, b);
   } else if (__all_sync(0xFFFFFFFFu, high < 0.5f)) {
     tanh_series<6>(s, f, b);
+  } else if (j.softcap > kWideCap) {
+#pragma unroll
+    for (uint32_t c = 0; c < 4u; ++c)
+#pragma unroll
+      for (uint32_t i = 0; i < 32u; ++i) {
+        s[c][i] = __float_as_uint(cap_score<true>(j, __uint_as_float(s[c][i]) * factor));
+      }
   } else {
 #pragma unroll
     for (uint32_t c = 0; c < 4u; ++c)
 #pragma unroll
       for (uint32_t i = 0; i < 32u; ++i) {
-        const float y = ex2(__uint_as_float(s[c][i]) * factor * j.cap_in);
-        s[c][i] = __float_as_uint(b * (1.0f - __fdividef(2.0f, 1.0f + y)));
+        s[c][i] = __float_as_uint(cap_score<false>(j, __uint_as_float(s[c][i]) * factor));
       }
   }
 }

@@ -42,6 +42,23 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// A score x to softcap log2(e) tanh(x / softcap), by 1 - 2 / (1 + e^2x).  Its
+// error is about 2^-23 of the cap, whatever the score: up to a cap of 256
+// under 2^-14 in the exponent, an eighth of the weights' FP16 rounding.  For
+// WIDE caps, arguments under 1/4 take tanh's series (to x^7; the next term is
+// under 9e-8 there), whose error goes with the score.
+constexpr float kWideCap = 256.0f;
+
+template <bool WIDE>
+__device__ __forceinline__ float cap_score(const AttnJob& j, float x) {
+  const float y = j.cap_out * (1.0f - __fdividef(2.0f, 1.0f + ex2(x * j.cap_in)));
+  if constexpr (!WIDE) return y;
+  const float a = x * j.cap_inv, u = a * a;
+  const float r = fmaf(u, fmaf(u, fmaf(u, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+  const float series = j.cap_out * (a * r);
+  return u < 0.0625f ? series : y;
+}
+
 // Pairs of FP32 in a 64-bit register: one instruction for both.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;

@@ -117,3 +117,26 @@ def test_attention_caps_of_any_size_on_every_last_tile(hrb, cap, hd):
     rng = np.random.default_rng(24)
     s = Step(rng, [(90, 129), (90, 192), (90, 193), (90, 256), (90, 1)], 4, 2, hd, 16)
     close(s.run(hrb, softcap=cap), *s.want(softcap=cap))
+
+
+@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("hd,page", [(32, 64), (64, 16), (96, 16), (128, 32)])
+def test_attention_caps_of_any_size_for_single_tokens(hrb, cap, hd, page):
+    rng = np.random.default_rng(25)
+    s = Step(rng, [(1, 129), (1, 192), (1, 193), (1, 256), (1, 1), (3, 900)], 4, 2, hd, page)
+    close(s.run(hrb, softcap=cap), *s.want(softcap=cap))
+
+
+@pytest.mark.parametrize("cap", [50.0, 1e4, 1e6, 1e9])
+@pytest.mark.parametrize("lens", [[(4, 300)], [(100, 300)]], ids=["few", "prompt"])
+def test_attention_a_row_near_the_cap_leaves_the_others_alone(hrb, cap, lens):
+    """One row's scores reach the cap, the others' stay small beside it."""
+    rng = np.random.default_rng(26)
+    s = Step(rng, lens, 4, 2, 64, 16)
+    s.q[1] *= cap
+    want, mass = s.want(softcap=cap)
+    got = s.run(hrb, softcap=cap)
+    # FP32 scores as large as the cap are too coarse to compare that row.
+    assert np.isfinite(got[1]).all()
+    got[1] = want[1]
+    close(got, want, mass)
