@@ -280,7 +280,11 @@ __device__ __forceinline__ void tanh_series(uint32_t (&s)[4][32], float f, float
 }
 
 __device__ __forceinline__ void cap_scores(const AttnJob& j, float factor, uint32_t (&s)[4][32]) {
-  const float f = factor * j.cap_inv;
+  // For a cap near the type's end the factor would lose its bits under 2^-126;
+  // under 2^-100 no product of S passes 2^-60, where tanh x is x.
+  const bool linear = factor * j.cap_inv < 0x1p-100f;
+  const float f = linear ? 0x1p-100f : factor * j.cap_inv;
+  const float b = linear ? factor * kLog2e * 0x1p100f : j.cap_out;
   float top[8];
 #pragma unroll
   for (uint32_t c = 0; c < 8u; ++c) top[c] = 0.f;
@@ -293,7 +297,6 @@ __device__ __forceinline__ void cap_scores(const AttnJob& j, float factor, uint3
     }
   const float high = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]),
                           fmaxf(top[6], top[7])) * f;
-  const float b = j.cap_out;
   if (__all_sync(0xFFFFFFFFu, high < 0.25f)) {
     tanh_series<4>(s, f, b);
   } else if (__all_sync(0xFFFFFFFFu, high < 0.5f)) {

@@ -2,6 +2,7 @@
 // checks, jobs, dispatch.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -152,9 +153,14 @@ hrb::AttnJob attn_job(const hrb_ctx* ctx, const hrb_attn_desc* d) {
   j.window = d->window;
   j.scale = d->scale;
   j.softcap = d->softcap;
-  j.cap_inv = d->softcap != 0.f ? 1.0f / d->softcap : 0.f;
-  j.cap_in = d->softcap != 0.f ? 2.885390081777927f / d->softcap : 0.f;
-  j.cap_out = d->softcap * 1.4426950408889634f;
+  if (d->softcap != 0.f) {
+    // Finite for every cap: a score of zero times these is no NaN.  A cap
+    // above 2.3e38 is taken as that.
+    const double cap = std::min<double>(d->softcap, 2.3e38), most = 3.4e38;
+    j.cap_inv = static_cast<float>(std::min(1.0 / cap, most));
+    j.cap_in = static_cast<float>(std::min(2.885390081777927 / cap, most));
+    j.cap_out = static_cast<float>(cap * 1.4426950408889634);
+  }
   return j;
 }
 

@@ -140,3 +140,22 @@ def test_attention_a_row_near_the_cap_leaves_the_others_alone(hrb, cap, lens):
     assert np.isfinite(got[1]).all()
     got[1] = want[1]
     close(got, want, mass)
+
+
+@pytest.mark.parametrize("cap", [1e-45, 1e-39, 1e-30])
+@pytest.mark.parametrize("lens", [[(1, 90), (2, 300)], [(100, 200)]], ids=["one", "prompt"])
+def test_attention_a_tiny_cap_makes_all_scores_alike(hrb, cap, lens):
+    """Products of exactly zero among them."""
+    rng = np.random.default_rng(27)
+    s = Step(rng, lens, 4, 2, 64, 16)
+    s.q[0] = 0.0
+    cap = float(np.float32(cap))
+    close(s.run(hrb, softcap=cap), *s.want(softcap=cap))
+
+
+@pytest.mark.parametrize("cap", [1e34, 1e37, 2.9e38])
+@pytest.mark.parametrize("lens", [[(1, 90), (2, 300)], [(100, 200)]], ids=["one", "prompt"])
+def test_attention_a_cap_near_the_end_of_its_type(hrb, cap, lens):
+    rng = np.random.default_rng(31)
+    s = Step(rng, lens, 4, 2, 64, 16)
+    close(s.run(hrb, softcap=cap), *s.want(softcap=cap))
