@@ -43,9 +43,12 @@ struct hrb_ctx {
   // The int8 weight chunks of the tensor-core exact GEMM (launch_x_translate).
   void* xscratch = nullptr;
   size_t xscratch_bytes = 0;
-  // Scratch of the serving calls (serve.cu).
+  // Scratch of the serving calls (serve.cu).  A block that a captured call
+  // uses stays for the graph's replays when a larger one takes its place.
   void* serve = nullptr;
   size_t serve_bytes = 0;
+  bool serve_captured = false;
+  std::vector<void*> serve_kept;
   // Bit 0: the encoder met Inf/NaN; bit 1: a tensor-core kernel gave up
   // waiting (it then leaves its outputs unwritten).
   uint32_t* d_error = nullptr;
@@ -802,10 +805,24 @@ cudaStream_t ctx_stream(const hrb_ctx* ctx, void* stream) {
 uint32_t* ctx_error_word(const hrb_ctx* ctx) { return ctx->d_error; }
 int ctx_sm_count(const hrb_ctx* ctx) { return ctx->sm_count; }
 void ctx_count_launches(hrb_ctx* ctx, uint32_t n) { ctx->launches += n; }
-hrb_status ctx_serve_scratch(hrb_ctx* ctx, size_t bytes, void** out) {
+hrb_status ctx_serve_scratch(hrb_ctx* ctx, size_t bytes, cudaStream_t stream, void** out) {
+  if (ctx->serve_bytes < bytes && ctx->serve_captured) {
+    try {
+      ctx->serve_kept.push_back(ctx->serve);
+    } catch (const std::bad_alloc&) {
+      return fail(ctx, HRB_ENOMEM, "no host memory");
+    }
+    ctx->serve = nullptr;
+    ctx->serve_bytes = 0;
+    ctx->serve_captured = false;
+  }
   const hrb_status st = grow(ctx, &ctx->serve, &ctx->serve_bytes, bytes);
+  if (st != HRB_OK) return st;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  HRB_CUDA(ctx, cudaStreamIsCapturing(stream, &capture));
+  if (capture != cudaStreamCaptureStatusNone) ctx->serve_captured = true;
   *out = ctx->serve;
-  return st;
+  return HRB_OK;
 }
 
 hrb_status ctx_fail(hrb_ctx* ctx, hrb_status status, const char* message) {
@@ -877,6 +894,7 @@ hrb_status hrb_destroy(hrb_ctx* ctx) {
   cudaFree(ctx->staging);
   cudaFree(ctx->xscratch);
   cudaFree(ctx->serve);
+  for (void* p : ctx->serve_kept) cudaFree(p);
   cudaFree(ctx->d_error);
   if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
   delete ctx;

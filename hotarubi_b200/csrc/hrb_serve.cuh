@@ -44,8 +44,9 @@ cudaStream_t ctx_stream(const hrb_ctx* ctx, void* stream);
 uint32_t* ctx_error_word(const hrb_ctx* ctx);
 int ctx_sm_count(const hrb_ctx* ctx);
 void ctx_count_launches(hrb_ctx* ctx, uint32_t n);
-// The context's scratch of the serving calls, grown to `bytes`.
-hrb_status ctx_serve_scratch(hrb_ctx* ctx, size_t bytes, void** out);
+// The context's scratch of the serving calls, grown to `bytes`, for a call on
+// `stream`.
+hrb_status ctx_serve_scratch(hrb_ctx* ctx, size_t bytes, cudaStream_t stream, void** out);
 
 struct BlocksJob {
   const int32_t *cached, *fresh, *free_pages, *head_in;

@@ -370,12 +370,13 @@ hrb_status hrb_attention(hrb_ctx* ctx, const hrb_attn_desc* d, void* stream) {
   if (cudaSetDevice(hrb::ctx_device(ctx)) != cudaSuccess) {
     return refuse(ctx, HRB_ECUDA, "cudaSetDevice");
   }
+  cudaStream_t s = hrb::ctx_stream(ctx, stream);
   hrb::AttnJob j = attn_job(ctx, d);
   const uint64_t need = attn_plan(ctx, d, &j, nullptr);
   if (need != 0u) {
     void* base = d->workspace;
     if (base == nullptr) {
-      st = hrb::ctx_serve_scratch(ctx, need, &base);
+      st = hrb::ctx_serve_scratch(ctx, need, s, &base);
       if (st != HRB_OK) return st;
     } else if (d->workspace_bytes < need) {
       return refuse(ctx, HRB_EINVAL, "workspace of %llu bytes, %llu needed",
@@ -384,7 +385,6 @@ hrb_status hrb_attention(hrb_ctx* ctx, const hrb_attn_desc* d, void* stream) {
     }
     attn_plan(ctx, d, &j, static_cast<uint8_t*>(base));
   }
-  cudaStream_t s = hrb::ctx_stream(ctx, stream);
   const int n = decoding(j)
                     ? hrb::launch_attn_decode(j, hrb::ctx_error_word(ctx), s)
                     : hrb::launch_attn_prompt(j, hrb::ctx_error_word(ctx), s);

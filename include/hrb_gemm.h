@@ -654,8 +654,10 @@ HRB_API hrb_status hrb_gemm_rows(hrb_ctx* ctx, const hrb_gemm_desc* desc, const 
  *      hrb_attention     attention of the new tokens over the cache.
  *    All pointers are device pointers unless said otherwise; every call is
  *    asynchronous on `stream` and reads request lengths, tables and slots on
- *    the device, so a step can be captured into a CUDA graph (with a
- *    workspace of the caller's, or after one call of the same size).
+ *    the device, so a step can be captured into a CUDA graph: with a
+ *    workspace of the caller's, or after one call of the same size in the
+ *    context's scratch, which then stays as it is until hrb_destroy (a later
+ *    call that needs more gets another block).
  * ------------------------------------------------------------------- */
 
 /* Keys and values in MXFP4 (E2M1 codes, one E8M0 scale byte per 32 dims, the

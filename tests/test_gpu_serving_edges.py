@@ -159,3 +159,40 @@ def test_attention_a_cap_near_the_end_of_its_type(hrb, cap, lens):
     rng = np.random.default_rng(31)
     s = Step(rng, lens, 4, 2, 64, 16)
     close(s.run(hrb, softcap=cap), *s.want(softcap=cap))
+
+
+@pytest.mark.parametrize("lens", [[(1, 3000), (1, 40)], [(60, 200), (9, 70)]], ids=["one", "prompt"])
+def test_attention_captured_on_the_contexts_scratch_outlives_larger_calls(hrb, lens):
+    """A step captured after a call of its size, a larger call that makes the
+    scratch grow, other allocations, and the step's replays."""
+    lib = capi.Library()
+    rng = np.random.default_rng(32)
+    s = Step(rng, lens, 4, 2, 64, 16)
+    want = s.want()
+    close(s.run(lib), *want)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    lists = [dev(np.asarray(x, np.int32)) for x in (s.start, [kv for _, kv in lens], s.table)]
+    out = torch.empty(s.rows, 4 * 64, dtype=torch.bfloat16, device="cuda")
+    d = capi.attn_desc(capi.kv_cache(s.dd, s.pages, 16, 2, 64), len(lens), 4, q=s.dq, ldq=s.ldq,
+                       q_start=lists[0], total_q=s.rows, max_q=max(q for q, _ in lens),
+                       kv_len=lists[1], max_kv=max(kv for _, kv in lens), table=lists[2],
+                       table_ld=s.ld, scale=s.scale, out=out)
+    ready()
+    with torch.cuda.graph(graph, stream=side):
+        lib.attention(d, stream=torch.cuda.current_stream().cuda_stream)
+    big = Step(rng, [(300, 4000)], 4, 2, 64, 16)
+    more = [big]
+    for q in (600, 900):   # each larger than all before
+        more.append(Step(rng, [(q, 2500 + 10 * q)], 4, 2, 64, 16))
+    for b in more:
+        close(b.run(lib), *b.want())
+        filler = torch.full((1 << 26,), 0xFF, dtype=torch.uint8, device="cuda")
+        out.zero_()
+        ready()
+        graph.replay()
+        torch.cuda.synchronize()
+        close(out.double().cpu().numpy().reshape(s.rows, 4, 64), *want)
+        del filler
+    lib.sync()
+    del graph
+    lib.close()
