@@ -25,36 +25,51 @@ namespace {
 
 constexpr uint32_t kThreads = 256;  // and tokens a block
 
-// Inclusive sums of two values over the block's threads; `total` receives
-// the block's sums.
+constexpr uint32_t kMost = 0x80000000u;  // sums are held to this: more than any max_tokens or nfree
+
+__device__ __forceinline__ uint32_t held_add(uint32_t a, uint32_t b) {
+  const uint32_t s = a + b;
+  return s < a ? kMost : min(s, kMost);
+}
+
+// Sums of two values over the threads before each one; `total` receives the
+// block's sums.  HELD: for values whose sums may pass kMost.
+template <bool HELD>
 __device__ __forceinline__ uint2 block_scan(uint2 v, uint2* total, uint2* warp_sums) {
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+  auto add = [](uint2 a, uint2 b) {
+    return HELD ? make_uint2(held_add(a.x, b.x), held_add(a.y, b.y)) : make_uint2(a.x + b.x, a.y + b.y);
+  };
+  const uint2 own = v;
 #pragma unroll
   for (uint32_t d = 1; d < 32; d *= 2) {
-    const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, v.x, d);
-    const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, v.y, d);
-    if (lane >= d) {
-      v.x += x;
-      v.y += y;
-    }
+    const uint2 u = make_uint2(__shfl_up_sync(0xFFFFFFFFu, v.x, d), __shfl_up_sync(0xFFFFFFFFu, v.y, d));
+    if (lane >= d) v = add(v, u);
   }
   if (lane == 31u) warp_sums[warp] = v;
+  if constexpr (HELD) {
+    v = make_uint2(__shfl_up_sync(0xFFFFFFFFu, v.x, 1), __shfl_up_sync(0xFFFFFFFFu, v.y, 1));
+    if (lane == 0u) v = make_uint2(0, 0);
+  } else {
+    v = make_uint2(v.x - own.x, v.y - own.y);
+  }
   __syncthreads();
   uint2 before = make_uint2(0, 0), all = make_uint2(0, 0);
 #pragma unroll
   for (uint32_t w = 0; w < kThreads / 32u; ++w) {
     const uint2 s = warp_sums[w];
-    if (w < warp) {
-      before.x += s.x;
-      before.y += s.y;
-    }
-    all.x += s.x;
-    all.y += s.y;
+    if (w < warp) before = add(before, s);
+    all = add(all, s);
   }
   __syncthreads();
   *total = all;
-  return make_uint2(v.x + before.x, v.y + before.y);
+  return add(v, before);
 }
+
+template <bool H>
+struct Held {
+  static constexpr bool value = H;
+};
 
 struct Request {
   uint32_t seq, first, cached, have, base;  // first token, cached tokens, old pages, free entry
@@ -73,42 +88,60 @@ __global__ void __launch_bounds__(kThreads)
   bool bad = false, short_of = false;
   uint2 carry = make_uint2(0, 0);
   uint32_t listed = 0;  // requests listed so far
-  for (uint32_t c = 0; c < j.seqs; c += kThreads) {
-    const uint32_t i = c + threadIdx.x;
-    int32_t cached = 0, fresh = 0;
-    if (i < j.seqs) {
-      cached = ld(j.cached + i);
-      fresh = ld(j.fresh + i);
-      bad |= cached < 0 || fresh < 0;
-      cached = max(cached, 0);
-      fresh = max(fresh, 0);
+  // Scans the requests.  Held<false> takes lengths and sums as they are, and
+  // gives false where some are out of range: Held<true> then does it again.
+  auto scan = [&](auto which) -> bool {
+    constexpr bool kHeld = decltype(which)::value;
+    bool fits = true;
+    carry = make_uint2(0, 0);
+    listed = 0;
+    for (uint32_t c = 0; c < j.seqs; c += kThreads) {
+      const uint32_t i = c + threadIdx.x;
+      int32_t cached = 0, fresh = 0;
+      if (i < j.seqs) {
+        cached = ld(j.cached + i);
+        fresh = ld(j.fresh + i);
+      }
+      const bool odd = (cached | fresh | static_cast<int32_t>(
+                            static_cast<uint32_t>(cached) + static_cast<uint32_t>(fresh))) < 0;
+      if constexpr (kHeld) {
+        bad |= odd;
+        cached = max(cached, 0);
+        fresh = min(max(fresh, 0), 0x7FFFFFFF - cached);
+      }
+      const uint32_t have = (static_cast<uint32_t>(cached) + mask) >> j.page_log2;
+      const uint32_t need =
+          ((static_cast<uint32_t>(cached) + static_cast<uint32_t>(fresh) + mask) >> j.page_log2) -
+          have;
+      // kThreads lengths under 2^18, of pages under 2^15 each, have sums under
+      // 2^26 and 2^23; a longer or odd one counts 2^23 pages here, and shows.
+      const uint32_t pages = !kHeld && (odd || fresh >= 1 << 18) ? 1u << 23 : need;
+      uint2 total;
+      const uint2 sum =
+          block_scan<kHeld>(make_uint2(static_cast<uint32_t>(fresh), pages), &total, warp_sums);
+      const uint32_t first = kHeld ? held_add(carry.x, sum.x) : carry.x + sum.x;
+      const uint32_t base = kHeld ? held_add(carry.y, sum.y) : carry.y + sum.y;
+      carry.x = kHeld ? held_add(carry.x, total.x) : carry.x + total.x;
+      carry.y = kHeld ? held_add(carry.y, total.y) : carry.y + total.y;
+      fits = fits && (kHeld || (total.y < 1u << 23 && carry.x < kMost));
+      if (i < j.seqs && i >= s0 && i < s1) {
+        j.q_start[i] = static_cast<int32_t>(kHeld ? min(first, 0x7FFFFFFFu) : first);
+        j.kv_len[i] = cached + fresh;
+      }
+      // At most one request a token: the range holds kThreads tokens, and a sum
+      // that was held starts past all ranges.
+      const bool mine = fits && fresh > 0 && first < t1 && first + static_cast<uint32_t>(fresh) > t0;
+      uint2 in_chunk;
+      const uint2 rank = block_scan<false>(make_uint2(mine ? 1u : 0u, 0u), &in_chunk, warp_sums);
+      if (mine) list[listed + rank.x] = Request{i, first, static_cast<uint32_t>(cached), have, base};
+      listed += in_chunk.x;
     }
-    const uint32_t have = (static_cast<uint32_t>(cached) + mask) >> j.page_log2;
-    const uint32_t need =
-        ((static_cast<uint32_t>(cached) + static_cast<uint32_t>(fresh) + mask) >> j.page_log2) -
-        have;
-    uint2 total;
-    const uint2 sum = block_scan(make_uint2(static_cast<uint32_t>(fresh), need), &total, warp_sums);
-    const uint32_t first = carry.x + sum.x - static_cast<uint32_t>(fresh);
-    if (i < j.seqs && i >= s0 && i < s1) {
-      j.q_start[i] = static_cast<int32_t>(first);
-      j.kv_len[i] = cached + fresh;
-    }
-    // At most one request a token: the range holds kThreads tokens.
-    const bool mine = fresh > 0 && first < t1 && first + static_cast<uint32_t>(fresh) > t0;
-    uint2 in_chunk;
-    const uint2 rank = block_scan(make_uint2(mine ? 1u : 0u, 0u), &in_chunk, warp_sums);
-    if (mine) {
-      list[listed + rank.x - 1u] = Request{i, first, static_cast<uint32_t>(cached), have,
-                                           carry.y + sum.y - need};
-    }
-    listed += in_chunk.x;
-    carry.x += total.x;
-    carry.y += total.y;
-  }
+    return fits;
+  };
+  if (!scan(Held<false>{})) scan(Held<true>{});
   __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    j.q_start[j.seqs] = static_cast<int32_t>(carry.x);
+    j.q_start[j.seqs] = static_cast<int32_t>(min(carry.x, 0x7FFFFFFFu));
     if (j.head_out != nullptr) *j.head_out = static_cast<int32_t>(head + carry.y);
     short_of |= carry.x > j.max_tokens;
   }

@@ -704,8 +704,8 @@ typedef enum hrb_dtype {
  * the row is full, or the table's own entry is negative) get slot -1, a table
  * entry without a page becomes -1, tokens past max_tokens are dropped (with
  * the table entries of pages that only they use), a negative length counts as
- * 0: hrb_sync then reports HRB_EDATA.  The step's tokens together, and each
- * request's, are fewer than 2^31. */
+ * 0, and lengths and sums past 2^31 - 1 as that: hrb_sync then reports
+ * HRB_EDATA. */
 typedef struct hrb_blocks_desc {
   uint32_t seqs;               /* at most 65536 */
   uint32_t page;               /* tokens a page, as hrb_kv_cache's */

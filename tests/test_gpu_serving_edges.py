@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from hotarubi_b200 import capi  # noqa: E402
-from test_gpu_serving import Step, check_codes, close, dev, ready, run_qkv  # noqa: E402
+from test_gpu_serving import Step, check_codes, close, dev, ready, run_qkv, run_tables  # noqa: E402
 
 
 def rows_of(s):
@@ -196,3 +196,53 @@ def test_attention_captured_on_the_contexts_scratch_outlives_larger_calls(hrb, l
     lib.sync()
     del graph
     lib.close()
+
+
+def test_block_tables_lengths_whose_sums_pass_31_bits(hrb):
+    """1200 requests of 2^30 new tokens: the step's slots are the first
+    request's, and the sums are held to 2^31 - 1."""
+    n, tokens = 1200, 1000
+    free = np.random.default_rng(33).permutation(70).astype(np.int32)
+    table = np.full((n, 64), -7, np.int32)
+    got, err = run_tables(hrb, np.zeros(n), np.full(n, 1 << 30), free, 2, table, 16, tokens)
+    assert err is not None and err.status == capi.HRB_EDATA
+    t = np.arange(tokens)
+    assert np.array_equal(got[1], free[2 + t // 16] * 16 + t % 16) and np.array_equal(got[2], t)
+    assert np.array_equal(got[3], np.minimum(np.arange(n + 1) * (1 << 30), 0x7FFFFFFF))
+    assert (got[4] == 1 << 30).all()
+    table[0, :63] = free[2:65]
+    assert np.array_equal(got[0], table)
+
+
+def test_block_tables_a_length_past_31_bits(hrb):
+    table = np.full((3, 4), 5, np.int32)
+    got, err = run_tables(hrb, [0, 0x7FFFFFFB, 3], [2, 10, 1], [8, 9], 0, table, 16, 8)
+    assert err is not None and err.status == capi.HRB_EDATA
+    assert np.array_equal(got[4], [2, 0x7FFFFFFF, 4]) and np.array_equal(got[3], [0, 2, 6, 7])
+    assert np.array_equal(got[1], [128, 129, -1, -1, -1, -1, 83, -1])
+
+
+@pytest.mark.parametrize("long", [(1 << 18) - 1, 1 << 18, 3000000])
+def test_block_tables_long_prompts_among_short_ones(hrb, long):
+    rng = np.random.default_rng(long)
+    fresh = rng.integers(0, 40, 600)
+    cached = rng.integers(0, 500, 600)
+    fresh[[3, 255, 256, 420]] = long
+    table = np.full((600, (long + 500) // 64 + 2), -1, np.int32)
+    table[:, :8] = rng.integers(0, 10000, (600, 8))
+    need = -(-(cached + fresh) // 64) - -(-cached // 64)
+    free = rng.permutation(int(need.sum()) + 9).astype(np.int32)
+    start = np.concatenate(([0], np.cumsum(fresh)))
+    tokens = int(start[-1]) + 5
+    got, err = run_tables(hrb, cached, fresh, free, 4, table, 64, tokens)
+    assert err is None
+    seq = np.repeat(np.arange(600), fresh)
+    pos = np.arange(tokens - 5) - start[seq] + cached[seq]
+    base = 4 + np.cumsum(need) - need
+    have = -(-cached // 64)
+    for i in range(600):
+        table[i, have[i]:have[i] + need[i]] = free[base[i]:base[i] + need[i]]
+    assert np.array_equal(got[0], table) and np.array_equal(got[3], start)
+    assert np.array_equal(got[2], np.concatenate((pos, np.zeros(5, int))))
+    assert np.array_equal(got[1], np.concatenate((table[seq, pos // 64] * 64 + pos % 64, [-1] * 5)))
+    assert got[5][0] == 4 + need.sum()
