@@ -228,14 +228,20 @@ hrb_status hrb_block_tables(hrb_ctx* ctx, const hrb_blocks_desc* d, void* stream
       (d->max_tokens != 0u && d->slots == nullptr) || (d->nfree != 0u && d->free_pages == nullptr)) {
     return refuse(ctx, HRB_EINVAL, "null buffer");
   }
-  if (d->head_in != nullptr && d->head_in == d->head_out) {
-    return refuse(ctx, HRB_EINVAL, "head_out is head_in: blocks still read the one while the other "
-                                   "is written");
-  }
   if (!on(d->cached, 4) || !on(d->fresh, 4) || !on(d->free_pages, 4) || !on(d->head_in, 4) ||
       !on(d->head_out, 4) || !on(d->table, 4) || !on(d->q_start, 4) || !on(d->kv_len, 4) ||
       !on(d->slots, 4) || !on(d->pos, 4)) {
     return refuse(ctx, HRB_EINVAL, "a list is not 4-byte aligned");
+  }
+  const int32_t* const in[] = {d->cached, d->fresh, d->free_pages, d->head_in};
+  const int32_t* const out[] = {d->table, d->q_start, d->kv_len, d->slots, d->pos, d->head_out};
+  for (const int32_t* a : in) {
+    for (const int32_t* b : out) {
+      if (a != nullptr && a == b) {
+        return refuse(ctx, HRB_EINVAL, "an output list is an input: blocks still read the one while "
+                                       "the other is written");
+      }
+    }
   }
   if (cudaSetDevice(hrb::ctx_device(ctx)) != cudaSuccess) {
     return refuse(ctx, HRB_ECUDA, "cudaSetDevice");

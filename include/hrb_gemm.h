@@ -705,7 +705,8 @@ typedef enum hrb_dtype {
  * entry without a page becomes -1, tokens past max_tokens are dropped (with
  * the table entries of pages that only they use), a negative length counts as
  * 0, and lengths and sums past 2^31 - 1 as that: hrb_sync then reports
- * HRB_EDATA. */
+ * HRB_EDATA.  The lists written (table, q_start, kv_len, slots, pos, head_out)
+ * are none of those read: kv_len is copied to cached after the call. */
 typedef struct hrb_blocks_desc {
   uint32_t seqs;               /* at most 65536 */
   uint32_t page;               /* tokens a page, as hrb_kv_cache's */
@@ -714,8 +715,7 @@ typedef struct hrb_blocks_desc {
   const int32_t* free_pages;   /* [nfree] */
   uint32_t nfree;
   const int32_t* head_in;      /* [1] first unused entry of free_pages, or NULL: 0 */
-  int32_t* head_out;           /* [1] head + pages asked for, or NULL.  Another
-                                  address than head_in */
+  int32_t* head_out;           /* [1] head + pages asked for, or NULL */
   int32_t* table;              /* [seqs][table_ld], in and out */
   uint32_t table_ld;
   int32_t* q_start;            /* [seqs + 1] */

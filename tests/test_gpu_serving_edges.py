@@ -246,3 +246,20 @@ def test_block_tables_long_prompts_among_short_ones(hrb, long):
     assert np.array_equal(got[2], np.concatenate((pos, np.zeros(5, int))))
     assert np.array_equal(got[1], np.concatenate((table[seq, pos // 64] * 64 + pos % 64, [-1] * 5)))
     assert got[5][0] == 4 + need.sum()
+
+
+def test_block_tables_refuse_an_output_that_is_an_input(hrb):
+    """Blocks still read the lists that others would be writing."""
+    buf = torch.zeros(16, 64, dtype=torch.int32, device="cuda")
+    at = {name: buf[i].data_ptr() for i, name in enumerate(
+        ("cached", "fresh", "free_pages", "head_in", "head_out", "table", "q_start", "kv_len", "slots", "pos"))}
+    ready()
+    for out in ("table", "q_start", "kv_len", "slots", "pos", "head_out"):
+        for into in ("cached", "fresh", "free_pages", "head_in"):
+            d = capi.blocks_desc(2, 16, nfree=4, table_ld=4, max_tokens=4, **at)
+            hrb.block_tables(d)
+            setattr(d, out, at[into])
+            with pytest.raises(capi.HrbError) as e:
+                hrb.block_tables(d)
+            assert e.value.status == capi.HRB_EINVAL, (out, into)
+    hrb.sync()
