@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
   const int32_t rows = min(q_len * group - r0, static_cast<int32_t>(kRows));
   const int32_t c0 = static_cast<int32_t>(chunk * j.chunk);
   if (rows <= 0 || (c0 >= kv && c0 > 0)) return;
-  const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
+  const int32_t c1 = c0 + min(kv - c0, static_cast<int32_t>(j.chunk));
   const bool whole = kv <= static_cast<int32_t>(j.chunk);  // no other chunk of this request
 
   // The keys that the rows see, and the tiles of this warp among them.
@@ -134,11 +134,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
   int32_t page_a = -1, page_b = -1, base = 0;
   auto load_pages = [&](int32_t at) {  // tiles number at .. at + 31 of this warp
     base = at;
-    const int32_t i = static_cast<int32_t>(warp) + (at + static_cast<int32_t>(lane)) * static_cast<int32_t>(kWarps);
-    const int32_t k = c0 + i * static_cast<int32_t>(kTile);
-    page_a = k < kv ? max(ld(table + (k >> j.cache.page_log2)), -1) : -2;
+    // Unsigned: the last tiles' numbers run up to 2^12 keys past kv.
+    const uint32_t i = warp + (static_cast<uint32_t>(at) + lane) * kWarps, end = static_cast<uint32_t>(kv);
+    const uint32_t k = static_cast<uint32_t>(c0) + i * kTile;
+    page_a = k < end ? max(ld(table + (k >> j.cache.page_log2)), -1) : -2;
     page_b = page_a;
-    if (P16) page_b = k + 16 < kv ? max(ld(table + ((k + 16) >> 4)), -1) : -2;
+    if (P16) page_b = k + 16u < end ? max(ld(table + ((k + 16u) >> 4)), -1) : -2;
   };
   const uint8_t* const head_data = j.cache.data + static_cast<uint64_t>(head) * j.cache.record;
   // Pages outside the cache read as zeros.
@@ -390,8 +391,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     }
     // Scores to the exponent of two.  Tiles that all rows see whole (all but
     // a request's last for single tokens) skip the masks.
-    const int32_t k1 = k0 + static_cast<int32_t>(kTile);
-    const bool clear = (k0 >= last.lo && k1 <= first.hi) || k1 <= first.pre;
+    const bool clear = (k0 >= last.lo && first.hi - k0 >= static_cast<int32_t>(kTile)) ||
+                       first.pre - k0 >= static_cast<int32_t>(kTile);
     const bool shaped = capped || j.slopes != nullptr;
     if (wide) {  // a branch of its own: the others' arithmetic is not doubled
 #pragma unroll
@@ -416,8 +417,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
       for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (uint32_t c = 0; c < 8u; ++c) {
-          const int32_t k = k0 + static_cast<int32_t>(16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g);
-          s[nt][c / 4u][c & 3u] -= slope[nt][c & 1u] * fabsf(static_cast<float>(pos[nt][c & 1u] - k));
+          const uint32_t k = static_cast<uint32_t>(k0) + 16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g;
+          const int32_t away = static_cast<int32_t>(static_cast<uint32_t>(pos[nt][c & 1u]) - k);
+          s[nt][c / 4u][c & 3u] -= slope[nt][c & 1u] * fabsf(static_cast<float>(away));
         }
     }
     if (!clear) {
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
       for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (uint32_t c = 0; c < 8u; ++c) {
-          const int32_t k = k0 + static_cast<int32_t>(16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g);
+          const uint32_t k = static_cast<uint32_t>(k0) + 16u * (c / 4u) + 8u * ((c >> 1) & 1u) + g;
           if (!attn_sees(seen[nt][c & 1u], k)) s[nt][c / 4u][c & 3u] = -INFINITY;
         }
     }

@@ -135,12 +135,14 @@ __device__ __forceinline__ Seen attn_seen(const AttnJob& j, int32_t i, int32_t k
     s.hi = min(max(i + 1, 0), kv);
     s.lo = j.window != 0 && i >= static_cast<int32_t>(j.window)
                ? i + 1 - static_cast<int32_t>(j.window) : 0;
-    s.pre = min(pre, kv);
+    s.pre = min(max(pre, 0), kv);
   }
   return s;
 }
-__device__ __forceinline__ bool attn_sees(const Seen& s, int32_t k) {
-  return (k >= s.lo && k < s.hi) || k < s.pre;
+// A tile's last keys may pass 2^31 where the request's do not.
+__device__ __forceinline__ bool attn_sees(const Seen& s, uint32_t k) {
+  return (k >= static_cast<uint32_t>(s.lo) && k < static_cast<uint32_t>(s.hi)) ||
+         k < static_cast<uint32_t>(s.pre);
 }
 
 // FP32 to BF16 bits, to nearest even.

@@ -263,3 +263,34 @@ def test_block_tables_refuse_an_output_that_is_an_input(hrb):
                 hrb.block_tables(d)
             assert e.value.status == capi.HRB_EINVAL, (out, into)
     hrb.sync()
+
+
+def test_attention_single_tokens_over_close_to_2_to_the_31_keys(hrb):
+    """One page, seen 2^23 - 2 times, and a last one whose keys' scores stand
+    40 over the others': it takes all but 2^-20 of the weights."""
+    rng = np.random.default_rng(34)
+    page, heads, hd = 256, 4, 32
+    kv = (1 << 31) - page
+    c = ref.Cache(3, page, 1, hd)
+    keys, values = np.zeros((2, page, 1, hd)), rng.standard_normal((2, page, 1, hd))
+    keys[:, :, 0, 1:] = rng.standard_normal((2, page, hd - 1))
+    keys[1, :, 0, 0] = 6.0
+    for p in range(2):
+        for t in range(page):
+            c.write(p * page + t, keys[p, t], values[p, t])
+    read = [c.read(page + t) for t in range(page)]
+    q = torch.from_numpy(0.1 * rng.standard_normal((1, heads, hd)).astype(np.float32)).to(torch.bfloat16)
+    q[..., 0] = 7.0
+    table = torch.zeros(1, kv // page, dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    data, dq, start = dev(c.data), q.cuda(), dev(np.array([0, 1], np.int32))
+    lens = dev(np.array([kv], np.int32))
+    out = torch.empty(1, heads * hd, dtype=torch.bfloat16, device="cuda")
+    ready()
+    hrb.attention(capi.attn_desc(capi.kv_cache(data, 3, page, 1, hd), 1, heads, q=dq, q_start=start,
+                                 total_q=1, max_q=1, kv_len=lens, max_kv=kv, table=table,
+                                 table_ld=kv // page, scale=1.0, out=out))
+    hrb.sync()
+    want, mass = ref.attention(q.double().numpy(), [0, 1], [page], [np.stack([k for k, _ in read])],
+                               [np.stack([v for _, v in read])], 1.0)
+    close(out.double().cpu().numpy().reshape(1, heads, hd), want, mass)
