@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   const int32_t c0 = static_cast<int32_t>(chunk * j.chunk);
   const bool whole = kv <= static_cast<int32_t>(j.chunk);
   if (c0 >= kv && c0 > 0) return;
-  const int32_t c1 = min(kv, c0 + static_cast<int32_t>(j.chunk));
+  const int32_t c1 = c0 + min(kv - c0, static_cast<int32_t>(j.chunk));
   const uint32_t base = attn_first_tile(j, n);
   if (!attn_tiles_fit(j, base, kv)) {  // reported too
     griddep_wait();  // what follows in the stream must find k_kv_expand done
@@ -775,7 +775,8 @@ uint32_t attn_prompt_chunk(const AttnJob& job, int sm_count) {
   uint64_t chunk = job.max_kv;
   if (split > 1u) chunk = (job.max_kv + split - 1u) / split;
   if (chunk < 512u) chunk = 512u;
-  return static_cast<uint32_t>((chunk + kKeys - 1u) / kKeys * kKeys);
+  chunk = (chunk + kKeys - 1u) / kKeys * kKeys;
+  return static_cast<uint32_t>(chunk < 0x40000000u ? chunk : 0x40000000u);  // 31 bits
 }
 
 int launch_attn_prompt(const AttnJob& job, uint32_t* error_flag, cudaStream_t stream) {

@@ -294,3 +294,13 @@ def test_attention_single_tokens_over_close_to_2_to_the_31_keys(hrb):
     want, mass = ref.attention(q.double().numpy(), [0, 1], [page], [np.stack([k for k, _ in read])],
                                [np.stack([v for _, v in read])], 1.0)
     close(out.double().cpu().numpy().reshape(1, heads, hd), want, mass)
+
+
+def test_attention_prompt_with_the_largest_bound_on_keys(hrb):
+    """max_kv says 2^31 - 1; the request has 300 keys."""
+    rng = np.random.default_rng(35)
+    s = Step(rng, [(100, 300)], 2, 1, 32, 256)
+    s.ld = 1 << 23
+    table = np.full((1, s.ld), -1, np.int32)
+    table[0, :2] = s.table[0, :2]
+    close(s.run(hrb, table=table, max_kv=0x7FFFFFFF, total_kv=300), *s.want())
