@@ -26,7 +26,8 @@ __device__ __forceinline__ uint32_t attn_first_tile(const AttnJob& j, uint32_t n
   for (uint32_t i = threadIdx.x & 31u; i < n; i += 32u) {
     int32_t q0, q_len, kv;
     if (attn_request(j, i, &q0, &q_len, &kv) && q_len > 0) {
-      sum += (static_cast<uint32_t>(kv) + kAttnTileKeys - 1u) / kAttnTileKeys;
+      // Held to what no scratch has (2^26 tiles), so that no sum wraps.
+      sum = min(sum + (static_cast<uint32_t>(kv) + kAttnTileKeys - 1u) / kAttnTileKeys, 1u << 26);
     }
   }
   return __reduce_add_sync(0xFFFFFFFFu, sum);

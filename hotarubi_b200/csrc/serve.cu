@@ -182,26 +182,44 @@ bool decoding(const hrb::AttnJob& j) {
          (rows <= (j.cache.hd <= 64u ? 96u : 64u) && j.max_kv > 1024u);
 }
 
+// More tiles or partial rows than any GPU's memory holds (2^26 tiles of 24 KB
+// at least, 2^36 rows of 136 bytes at least): their bytes fit 64 bits.
+constexpr uint64_t kMostTiles = uint64_t{1} << 26, kMostCells = uint64_t{1} << 36;
+
 // Fills in how the call is split and where its scratch lies from `base`
-// (null: to learn the size).  Returns the scratch bytes.
-uint64_t attn_plan(const hrb_ctx* ctx, const hrb_attn_desc* d, hrb::AttnJob* j, uint8_t* base) {
-  const uint64_t total_kv = d->total_kv != 0u ? d->total_kv : uint64_t{d->seqs} * d->max_kv;
+// (null: to learn the size).  False where the scratch passes all memory, else
+// its bytes in `bytes`.
+bool attn_plan(const hrb_ctx* ctx, const hrb_attn_desc* d, hrb::AttnJob* j, uint8_t* base,
+               uint64_t* bytes) {
+  // Requests with more than max_kv keys are left out.
+  const uint64_t most_kv = uint64_t{d->seqs} * d->max_kv;
+  const uint64_t total_kv = d->total_kv != 0u && d->total_kv < most_kv ? d->total_kv : most_kv;
   uint64_t at = 0;
   if (decoding(*j)) {
     j->chunk = hrb::attn_decode_chunk(*j, total_kv, hrb::ctx_sm_count(ctx));
   } else {
     const uint64_t tiles = hrb::attn_prompt_tiles(*j, total_kv, &j->tile_stride);
-    j->tiles_cap = static_cast<uint32_t>(tiles < 0xFFFFFFFFull ? tiles : 0xFFFFFFFFull);
+    if (tiles > kMostTiles) return false;
+    j->tiles_cap = static_cast<uint32_t>(tiles);
     j->tiles = base;
     at = up256(tiles * j->cache.kv_heads * hrb::attn_prompt_tile_bytes(*j));
     j->chunk = hrb::attn_prompt_chunk(*j, hrb::ctx_sm_count(ctx));
   }
-  if (j->max_kv <= j->chunk) return at;
-  const uint64_t cells = (uint64_t{j->max_kv} + j->chunk - 1u) / j->chunk * j->total_q * j->heads;
-  j->part_ml = reinterpret_cast<float2*>(base + at);
-  at += up256(cells * 8u);
-  j->part_o = reinterpret_cast<float*>(base + at);
-  return at + cells * j->cache.hd * 4u;
+  if (j->max_kv > j->chunk) {
+    const uint64_t cells = (uint64_t{j->max_kv} + j->chunk - 1u) / j->chunk * j->total_q * j->heads;
+    if (cells > kMostCells) return false;
+    j->part_ml = reinterpret_cast<float2*>(base + at);
+    at += up256(cells * 8u);
+    j->part_o = reinterpret_cast<float*>(base + at);
+    at += cells * j->cache.hd * 4u;
+  }
+  *bytes = at;
+  return true;
+}
+
+hrb_status too_large(hrb_ctx* ctx, const hrb_attn_desc* d) {
+  return refuse(ctx, HRB_ENOMEM, "hrb_attention: no scratch for %u requests of up to %u keys, %llu together",
+                d->seqs, d->max_kv, static_cast<unsigned long long>(d->total_kv));
 }
 
 }  // namespace
@@ -364,8 +382,7 @@ hrb_status hrb_attention_workspace(hrb_ctx* ctx, const hrb_attn_desc* d, uint64_
   const hrb_status st = check_attn(ctx, d);
   if (st != HRB_OK || d->total_q == 0u) return st;
   hrb::AttnJob j = attn_job(ctx, d);
-  *bytes = attn_plan(ctx, d, &j, nullptr);
-  return HRB_OK;
+  return attn_plan(ctx, d, &j, nullptr, bytes) ? HRB_OK : too_large(ctx, d);
 }
 
 hrb_status hrb_attention(hrb_ctx* ctx, const hrb_attn_desc* d, void* stream) {
@@ -378,7 +395,8 @@ hrb_status hrb_attention(hrb_ctx* ctx, const hrb_attn_desc* d, void* stream) {
   }
   cudaStream_t s = hrb::ctx_stream(ctx, stream);
   hrb::AttnJob j = attn_job(ctx, d);
-  const uint64_t need = attn_plan(ctx, d, &j, nullptr);
+  uint64_t need = 0;
+  if (!attn_plan(ctx, d, &j, nullptr, &need)) return too_large(ctx, d);
   if (need != 0u) {
     void* base = d->workspace;
     if (base == nullptr) {
@@ -389,7 +407,7 @@ hrb_status hrb_attention(hrb_ctx* ctx, const hrb_attn_desc* d, void* stream) {
                     static_cast<unsigned long long>(d->workspace_bytes),
                     static_cast<unsigned long long>(need));
     }
-    attn_plan(ctx, d, &j, static_cast<uint8_t*>(base));
+    attn_plan(ctx, d, &j, static_cast<uint8_t*>(base), &need);
   }
   const int n = decoding(j)
                     ? hrb::launch_attn_decode(j, hrb::ctx_error_word(ctx), s)

@@ -304,3 +304,26 @@ def test_attention_prompt_with_the_largest_bound_on_keys(hrb):
     table = np.full((1, s.ld), -1, np.int32)
     table[0, :2] = s.table[0, :2]
     close(s.run(hrb, table=table, max_kv=0x7FFFFFFF, total_kv=300), *s.want())
+
+
+@pytest.mark.parametrize("lens", [[(1, 700), (1, 3000)], [(60, 700), (9, 3000)]], ids=["one", "prompt"])
+def test_attention_total_kv_past_all_requests_together(hrb, lens):
+    rng = np.random.default_rng(36)
+    s = Step(rng, lens, 4, 2, 64, 16)
+    for total in (6001, 1 << 60, (1 << 64) - 1):
+        close(s.run(hrb, total_kv=total, workspace=True), *s.want())
+
+
+@pytest.mark.parametrize("total", [0, 1 << 40, 1 << 60, (1 << 64) - 1])
+def test_attention_refuses_scratch_past_all_memory(hrb, total):
+    """300 requests of up to 2^31 - 1 keys: bytes that passed 64 bits came out
+    as a few megabytes.  Refused on the host."""
+    buf = torch.zeros(1 << 12, dtype=torch.uint8, device="cuda")
+    p = buf.data_ptr()
+    d = capi.attn_desc(capi.kv_cache(p, 1, 256, 2, 64), 300, 4, q=p, q_start=p, total_q=30000, max_q=100,
+                       kv_len=p, max_kv=0x7FFFFFFF, total_kv=total, table=p, table_ld=1 << 23, scale=0.1,
+                       out=p)
+    for call in (hrb.attention_workspace, hrb.attention):
+        with pytest.raises(capi.HrbError) as e:
+            call(d)
+        assert e.value.status == capi.HRB_ENOMEM and e.value.message
