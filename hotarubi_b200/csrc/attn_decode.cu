@@ -240,12 +240,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
       const int32_t r = static_cast<int32_t>(8u * nt + 2u * t + c);
       const float sc = __shfl_sync(0xFFFFFFFFu, row_scale[nt], (2u * t + c) * 4u);
       factor[nt][c] = fmaxf(fabsf(j.scale) * sc, 1.2e-38f) * (capped ? 1.0f : kLog2e);
-      if (sc != sc) factor[nt][c] = sc;
       m[nt][c] = -INFINITY;
       l[nt][c] = 0.f;
       pos[nt][c] = kv - q_len + (r0 + r) / group;
       seen[nt][c] = attn_seen(j, pos[nt][c], kv, pre);
       if (r >= rows) seen[nt][c].lo = seen[nt][c].hi = seen[nt][c].pre = 0;
+      // Inf or NaN in the row: its scores and outputs are NaN, unless it sees no key.
+      if (sc != sc && (seen[nt][c].lo < seen[nt][c].hi || seen[nt][c].pre > 0)) factor[nt][c] = sc;
       slope[nt][c] = j.slopes != nullptr && r < rows
                          ? ld(j.slopes + head * j.group + static_cast<uint32_t>((r0 + r) % group)) * kLog2e
                          : 0.f;

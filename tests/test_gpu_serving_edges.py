@@ -327,3 +327,14 @@ def test_attention_refuses_scratch_past_all_memory(hrb, total):
         with pytest.raises(capi.HrbError) as e:
             call(d)
         assert e.value.status == capi.HRB_ENOMEM and e.value.message
+
+
+@pytest.mark.parametrize("odd", [float("nan"), float("inf")])
+@pytest.mark.parametrize("lens", [[(3, 1), (1, 40)], [(100, 60), (30, 400)]], ids=["few", "prompt"])
+def test_attention_nan_in_a_row_without_keys_gives_zeros(hrb, lens, odd):
+    rng = np.random.default_rng(30)
+    s = Step(rng, lens, 4, 2, 64, 16)
+    want, mass = s.want()
+    s.q[0, 5] = odd
+    assert not mass[0].any()
+    close(s.run(hrb), want, mass)
