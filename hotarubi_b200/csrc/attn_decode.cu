@@ -9,7 +9,7 @@
 // (cvt.e2m1x2, times the block scale: both exact) straight in the layout of
 // an mma.sync operand, and with the running maximum m and sum l of a row
 //   S^T = K Q^T           (keys x rows; m16n8k16, the keys as the 16)
-//   p = 2^(s - m)         (FP16 for the product, FP32 for l)
+//   p = 2^(s - m + 7)     (FP16 for the product, FP32 for l)
 //   O^T += V^T P^T        (dims x rows; the dims as the 16)
 // Keys and dims, not rows, fill the 16 of the instruction, so 8 rows or
 // fewer waste nothing; tcgen05 would need the decoded keys written to shared
@@ -469,8 +469,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     uint32_t p[NT][2][2];
 #pragma unroll
     for (uint32_t nt = 0; nt < NT; ++nt) {
-      const float m0 = m[nt][0] == -INFINITY ? 0.f : -m[nt][0];
-      const float m1 = m[nt][1] == -INFINITY ? 0.f : -m[nt][1];
+      const float m0 = m[nt][0] == -INFINITY ? 0.f : kLift - m[nt][0];
+      const float m1 = m[nt][1] == -INFINITY ? 0.f : kLift - m[nt][1];
       const float f0 = shaped ? 1.0f : factor[nt][0], f1 = shaped ? 1.0f : factor[nt][1];
 #pragma unroll
       for (uint32_t hf = 0; hf < 2u; ++hf) {

@@ -11,7 +11,7 @@
 // k_attn_prompt: a block takes 256 rows (query token x query head of one
 // key/value head), two halves of 128 that alternate on the tensor cores:
 //   warps 0-3, 4-7  softmax of half A, B: a thread a row.  S = Q K^T from
-//                   TMEM, running maximum and sum, P = 2^(s - m) as FP16
+//                   TMEM, running maximum and sum, P = 2^(s - m + 7) as FP16
 //                   back to TMEM over S, O scaled there when m moves
 //   warp 8          issues S_A, S_B and O_A += P_A V, O_B += P_B V
 //                   (tcgen05.mma kind::f16, P from TMEM)
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
             }
           }
         }
-        const float shift = m == -INFINITY ? 0.f : -m;
+        const float shift = m == -INFINITY ? 0.f : kLift - m;
         const uint64_t scale2x = pack2(scale, scale), shift2x = pack2(shift, shift);
         uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll

@@ -11,7 +11,10 @@
 
 namespace hrb {
 
-constexpr float kLazy = 8.0f;    // log2 of the most a weight may pass 1 before m moves
+constexpr float kLazy = 8.0f;    // log2 of the most a score may pass m before m moves
+// Weights are 2^(s - m + kLift), up to 2^15: FP16 keeps what lies down to 2^-31
+// of the largest (2^-24 without it), and the factor cancels in O / l.
+constexpr float kLift = 7.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 constexpr uint32_t kAttnTileKeys = 128;  // keys a tile of the prompt kernel

@@ -338,3 +338,28 @@ def test_attention_nan_in_a_row_without_keys_gives_zeros(hrb, lens, odd):
     s.q[0, 5] = odd
     assert not mass[0].any()
     close(s.run(hrb), want, mass)
+
+
+@pytest.mark.parametrize("q", [1, 60])
+@pytest.mark.parametrize("drop", [20, 26, 30])
+def test_attention_small_weights_beside_a_large_one(hrb, q, drop):
+    """One key's score stands `drop` powers of two over all others', whose
+    weights are all there is to see: its value is zero, theirs are one.  A
+    weight of 2^-30 is still an FP16 number of one significant bit after the
+    factor of 2^7 that all weights carry, and the score's FP32 error (30 ln 2
+    of 2^-23 each for scale, product and exponent) moves it by 2^-17, so what is
+    left is the output's BF16 rounding, 2^-8."""
+    rng = np.random.default_rng(29)
+    kv = 700
+    s = Step(rng, [(q, kv)], 2, 1, 32, 16)
+    zero, one = np.zeros((1, 32)), np.ones((1, 32))
+    for j in range(kv):
+        k = zero.copy()
+        k[0, 0] = 4.0 if j == 3 else 0.0
+        s.cache.write(int(s.table[0, j // 16]) * 16 + j % 16, k, zero if j == 3 else one)
+    s.q[:] = 0.0
+    s.q[:, 0] = s.q[:, 32] = 8.0
+    s.scale = drop * np.log(2.0) / 32.0
+    got = s.run(hrb, causal=False)
+    want = (kv - 1) * 2.0 ** -drop / (1 + (kv - 1) * 2.0 ** -drop)
+    assert (np.abs(got - want) <= 2.0 ** -8 * want).all()
