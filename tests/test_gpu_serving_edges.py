@@ -363,3 +363,126 @@ def test_attention_small_weights_beside_a_large_one(hrb, q, drop):
     got = s.run(hrb, causal=False)
     want = (kv - 1) * 2.0 ** -drop / (1 + (kv - 1) * 2.0 ** -drop)
     assert (np.abs(got - want) <= 2.0 ** -8 * want).all()
+
+
+# ---------------------------------------------------------------------------
+# kernels and forms that the dispatch takes by size
+
+
+def again(s, n):
+    """n more requests like a Step's first: its rows, its pages."""
+    q = s.lens[0][0]
+    s.lens = s.lens + [s.lens[0]] * n
+    s.table = np.concatenate((s.table, np.repeat(s.table[:1], n, 0)))
+    s.q = torch.cat((s.q, s.q[:q].repeat(n, 1)))
+    s.start = np.concatenate((s.start, s.start[-1] + q * np.arange(1, n + 1))).astype(np.int32)
+    s.rows = int(s.start[-1])
+
+
+LONG = {   # requests of more than 1024 keys: two halves of 128 rows a block
+    "plain": {}, "open": dict(causal=False), "window": dict(window=300),
+    "prefix": dict(window=200, prefix=(300, 0, 2000)), "cap": dict(softcap=4.0),
+    "bias": dict(slopes=True), "all": dict(softcap=20.0, slopes=True, window=700, prefix=(130, 1, 0)),
+}
+
+
+@pytest.mark.parametrize("hd,page", [(32, 16), (64, 64), (96, 32), (128, 16)])
+@pytest.mark.parametrize("option", LONG)
+def test_attention_prompts_over_long_histories(hrb, option, hd, page):
+    """Blocks of one and of two halves, several requests, one tile's end."""
+    rng = np.random.default_rng(40 + hd)
+    s = Step(rng, [(150, 1500), (70, 1153), (129, 129)], 6, 3, hd, page)
+    kw = dict(LONG[option])
+    if "slopes" in kw:
+        kw["slopes"] = (0.05 * rng.random(6)).astype(np.float32)
+    ref_kw = dict(kw)
+    if "prefix" in kw:
+        ref_kw["prefix"] = np.minimum(kw["prefix"], [kv for _, kv in s.lens])
+    got = s.run(hrb, **kw)
+    close(got, *s.want(**ref_kw))
+    assert np.array_equal(got, s.run(hrb, **kw))
+
+
+@pytest.mark.parametrize("hd,page", [(32, 32), (64, 16), (96, 16), (128, 64)])
+@pytest.mark.parametrize("option", LONG)
+def test_attention_prompts_over_long_histories_unsplit(hrb, option, hd, page):
+    """Enough rows for every SM: a block takes all keys."""
+    rng = np.random.default_rng(45 + hd)
+    s = Step(rng, [(160, 1100), (90, 1300), (20, 1037)], 16, 8, hd, page)
+    kw = dict(LONG[option])
+    if "slopes" in kw:
+        kw["slopes"] = (0.05 * rng.random(16)).astype(np.float32)
+    ref_kw = dict(kw)
+    if "prefix" in kw:
+        ref_kw["prefix"] = np.minimum(kw["prefix"], [kv for _, kv in s.lens])
+        kw["prefix"] = tuple(kw["prefix"]) + (kw["prefix"][0],) * 7
+    want, mass = s.want(**ref_kw)
+    again(s, 7)
+    got = s.run(hrb, **kw)
+    close(got[:270], want, mass)
+    for i in range(7):
+        assert np.array_equal(got[270 + 160 * i:430 + 160 * i], got[:160])
+
+
+@pytest.mark.parametrize("lens,heads,kvh,hd", [
+    ([(5, 1100), (2, 1300)], 8, 1, 128),                 # 40 rows, in chunks of keys
+    ([(4, 1200), (4, 1025), (3, 40)], 16, 1, 64),        # 64 rows
+    ([(6, 1100), (1, 1500)], 16, 1, 64),                 # 96 rows
+    ([(24, 1030), (20, 1200)], 8, 2, 32),                # 96 rows of two heads
+    ([(16, 1040), (9, 1028)], 6, 2, 96),                 # 48 rows
+    ([(8, 1030)] * 90, 32, 8, 32),                       # 32 rows, one chunk
+    ([(16, 1030)] * 48, 32, 8, 32),                      # 64 rows, one chunk
+])
+@pytest.mark.parametrize("option", ["plain", "all"])
+def test_attention_rows_in_blocks_over_long_histories(hrb, lens, heads, kvh, hd, option):
+    rng = np.random.default_rng(len(lens) + hd)
+    few = lens[:3]
+    s = Step(rng, few, heads, kvh, hd, 16)
+    kw = {}
+    if option == "all":
+        kw = dict(softcap=20.0, slopes=(0.05 * rng.random(heads)).astype(np.float32), window=700,
+                  prefix=(130, 1, 0)[:len(few)])
+    ref_kw = dict(kw)
+    if "prefix" in kw:
+        ref_kw["prefix"] = np.minimum(kw["prefix"], [kv for _, kv in few])
+    want, mass = s.want(**ref_kw)
+    n, q = len(lens) - len(few), few[0][0]
+    again(s, n)
+    if "prefix" in kw:
+        kw["prefix"] = tuple(kw["prefix"]) + (kw["prefix"][0],) * n
+    got = s.run(hrb, **kw)
+    rows = len(want)
+    close(got[:rows], want, mass)
+    for i in range(n):
+        close(got[rows + i * q:rows + (i + 1) * q], want[:q], mass[:q])
+
+
+@pytest.mark.parametrize("hd,page", [(32, 64), (96, 64), (128, 64), (128, 16)])
+@pytest.mark.parametrize("lens", [[(1, 90), (1, 700)], [(3, 130), (2, 300)], [(90, 200), (33, 257)]],
+                         ids=["one", "few", "prompt"])
+@pytest.mark.parametrize("option", [dict(softcap=3.0), dict(slopes=True),
+                                    dict(softcap=300.0, slopes=True, window=50)], ids=str)
+def test_attention_shaped_scores_at_every_head_size(hrb, option, lens, hd, page):
+    rng = np.random.default_rng(50 + hd)
+    s = Step(rng, lens, 6, 2, hd, page)
+    kw = dict(option)
+    if "slopes" in kw:
+        kw["slopes"] = (0.1 * rng.random(6)).astype(np.float32)
+    close(s.run(hrb, **kw), *s.want(**kw))
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+def test_attention_mxint8_copy_of_joined_and_two_half_rows(hrb, hd):
+    """The MXINT8 copy alone and beside BF16 rows, within half a step of the
+    64-bit value."""
+    rng = np.random.default_rng(60 + hd)
+    for lens in ([(1, 3000), (1, 2049)], [(140, 1500), (100, 1100)]):
+        s = Step(rng, lens, 4, 2, hd, 16)
+        want, mass = s.want()
+        for out in (True, False):
+            s.run(hrb, oq=True, out=out)
+            codes, scales = s.codes.cpu().numpy()[:, :4 * hd], s.scales.cpu().numpy()[:, :hd // 8]
+            step = np.repeat(np.exp2(scales.astype(np.float64) - 133), 32, 1).reshape(want.shape)
+            value = codes.reshape(want.shape) * step
+            tol = 0.5 * step + 2.0 ** -9 * mass + np.where(np.abs(codes.reshape(want.shape)) == 127, step, 0)
+            assert (np.abs(value - want) <= tol).all()
