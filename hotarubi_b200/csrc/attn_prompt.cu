@@ -195,7 +195,7 @@ struct Cfg {
   static constexpr uint32_t kK = kQ;
   static constexpr uint32_t kV = kK + kStages * k_bytes(HD);
   static constexpr uint32_t kBars = kV + kStages * v_bytes(HD);
-  static constexpr uint32_t kUsed = kBars + 144u;
+  static constexpr uint32_t kUsed = kBars + 160u;
   // No more blocks an SM than its 512 columns of TMEM hold.
   static constexpr uint32_t kLeast = (HV == 2u ? 120u : 78u) * 1024u;
   static constexpr uint32_t kBytes = (kUsed > kLeast ? kUsed : kLeast) + 1024u;
@@ -331,8 +331,9 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5,
            *v_empty = bars + 7, *s_full = bars + 9, *o_full = bars + 11,
-           *p_full = bars + 13;  // [half][first or second 64 keys]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+           *p_full = bars + 13,  // [half][first or second 64 keys]
+           *done = bars + 17;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
 
   const uint32_t head = blockIdx.x % j.cache.kv_heads, n = blockIdx.z;
@@ -389,6 +390,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
 
   if (threadIdx.x == 0u) {
     mbar_init(q_full, HV * 128u);
+    mbar_init(done, 1);
     for (uint32_t i = 0; i < 2u; ++i) {
       mbar_init(k_full + i, 1);
       mbar_init(k_empty + i, 1);
@@ -496,6 +498,10 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
           mma_commit(v_empty + st);
           if (more) mma_commit(k_empty + nst);
         }
+        // The block keeps its barriers and TMEM until all products, and their
+        // arrivals that nothing else waits for, are in (also after a timeout).
+        mma_commit(done);
+        mbar_wait(done, 0, error_flag);
       }
     }
   } else {
