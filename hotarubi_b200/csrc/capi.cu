@@ -919,7 +919,8 @@ hrb_status hrb_sync(hrb_ctx* ctx) {
                                   "(use HRB_MODE_EXACT)");
     }
     if (flag & hrb::kErrKvSlot) {
-      return fail(ctx, HRB_EDATA, "a slot, position or block table entry is out of range");
+      return fail(ctx, HRB_EDATA, "a slot, position or block table entry is out of range, or a request "
+                                  "passes its call's bounds");
     }
     if (flag & hrb::kErrKvNonFinite) {
       return fail(ctx, HRB_EDATA, "a key or value to cache is infinite or NaN");

@@ -753,7 +753,7 @@ typedef struct hrb_qkv_desc {
   const float *q_norm, *k_norm;    /* [hd], or NULL */
   float eps;
   const float* rope;               /* [max_pos][rot / 2][2] (cos, sin), or NULL: no rotation */
-  uint32_t max_pos, rot;           /* rot even, at most hd */
+  uint32_t max_pos, rot;           /* rot a multiple of 8, at most hd */
   uint32_t interleaved;
   const int32_t* pos;              /* [axes][tokens] */
   uint32_t axes, sections[3];      /* 1..3; sections sum to rot / 2 (ignored for one axis) */
