@@ -16,17 +16,18 @@
 // memory first (2 bytes a code against half a byte read).  The order of the
 // reduced index is free, so a lane reads consecutive dims of a key: its 32
 // nibbles are one 16-byte load at hd = 128.
-// m only moves when a score passes it by 2^8 (a vote, no shuffles), which
-// FP16 weights allow.
+// m only moves when a score passes it by 2^8 (a vote, no shuffles): weights
+// reach 2^15, which FP16 allows.
 //
 // Chunks of one request are joined by k_attn_join from the rows' (m, l, O)
 // in FP32.
 //
 // Its floor is HBM: hd + hd / 16 bytes a key and head.  Measured (32/8 heads of
-// 128): 64 requests of up to 16384 keys 177 us, 4.1 TB/s, 63 % of a copy's
-// rate; one request of 131071 keys 43 us; one of 241 keys (15/5 heads of 64)
-// 4.4 us.  Bound by the lanes' work: with all pages in L2 it takes as long, 64 %
-// of the issue slots and 54 % of the ALU pipe (the conversions) are used.
+// 128; ranges over several boxes): 64 requests of up to 16384 keys 180 to
+// 184 us, 4.0 TB/s, 60 to 62 % of a copy's rate; one request of 131071 keys 43 to
+// 44 us; one of 241 keys (15/5 heads of 64) 4.4 to 4.7 us.  Bound by the lanes'
+// work: with all pages in L2 it takes as long, 63 % of the issue slots and 54 %
+// of the ALU pipe (the conversions) are used.
 #include <cuda_fp16.h>
 
 #include <atomic>

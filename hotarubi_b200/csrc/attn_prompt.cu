@@ -25,13 +25,12 @@
 // (attn_decode.cu) joins the rows' (m, l, O).
 //
 // Its floor is the tensor cores: 4 hd FLOP a pair of query and key that see
-// each other.  Measured: a prompt of 8191 tokens, 32/8 heads of 128, 478 us,
-// 1148 TFLOP/s, 69 % of a large BF16 product's rate.  A tile takes about 3600
-// clocks for both halves, the tensor cores work 2048 of them: a half's softmax
-// (2200) and its products (1200 with the waits) follow each other.  Two S of
-// 64 keys a half, which would let a softmax run ahead, measured slower: a
-// product of N = 64 with both operands in shared memory takes the time of
-// N = 128.
+// each other.  Measured: a prompt of 8191 tokens, 32/8 heads of 128, 507 to
+// 516 us, 1065 to 1085 TFLOP/s, 64 to 65 % of a large BF16 product's rate.  A tile
+// takes about 3600 clocks for both halves, the tensor cores work 2048 of them: a
+// half's softmax (2200) and its products (1200 with the waits) follow each
+// other.  Two S of 64 keys a half, which would let a softmax run ahead, measured
+// 660 us where this stood at 555.
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -256,7 +255,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // A row's raw scores to softcap log2(e) tanh(factor s / softcap).  Where a
 // warp's arguments are all small, tanh is its power series on the FMA pipe: up
 // to x^7 under 1/4 and x^11 under 1/2 (the next terms are under 9e-8 and 4.4e-7
-// there); else cap_score, a score at a time.
+// there); else cap_score, a score at a time.  A chunk of 512 tokens over 8703
+// keys, 32/8 heads of 128, a pass alone with cold L2: 128 us with small scores,
+// 196 with scores near a cap of 30 (two MUFU operations a score more).
 template <uint32_t TERMS>
 __device__ __forceinline__ void tanh_series(uint32_t (&s)[4][32], float f, float b) {
   constexpr float kSeries[6] = {1.f, -1.f / 3.f, 2.f / 15.f, -17.f / 315.f, 62.f / 2835.f, -1382.f / 155925.f};
@@ -412,10 +413,10 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // A softmax thread holds a row's 128 scores (split 224/56: 475 us for the
-  // 8191 prompt but 124.5 for 512 tokens over 8703 keys, 216/72 481 and 119.5,
-  // 208/88 478 and 119.6).  Registers at launch: 384 x 168 = 256 x 208 +
-  // 128 x 88 (HV 2), 256 x 128 = 128 x 200 + 128 x 56.
+  // A softmax thread holds a row's 128 scores (measured on one box, split 224/56:
+  // 475 us for the 8191 prompt but 124.5 for 512 tokens over 8703 keys, 216/72
+  // 481 and 119.5, 208/88 478 and 119.6).  Registers at launch: 384 x 168 =
+  // 256 x 208 + 128 x 88 (HV 2), 256 x 128 = 128 x 200 + 128 x 56.
   if (warp >= 4u * HV) {
     if constexpr (HV == 2u) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");

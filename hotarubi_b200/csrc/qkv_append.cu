@@ -17,8 +17,8 @@
 // Memory bound: each input is read once (FP32: 4 bytes a value, BF16: 2),
 // and per token heads * hd BF16 values and kv_heads * (hd + hd / 16) bytes
 // are written.  Measured: 16387 tokens of 32/8 heads of 128 (BF16, three
-// axes) 81 us with the read-back, 4.9 TB/s, 74 % of a copy's rate; the issue
-// slots are used to 57 %.  With rsqrtf where the norm divides by a square root
+// axes) 81 to 83 us with the read-back, 4.8 to 4.9 TB/s, 73 to 75 % of a copy's
+// rate; k_qkv alone uses DRAM to 53 % and the issue slots to 57 %.  With rsqrtf where the norm divides by a square root
 // (two units in the last place), packed FP32 pairs, and rows in phases of q,
 // k and v it takes 43 M warp instructions, against 199 M for a lane of four
 // dims with one code path for all three.
