@@ -16,8 +16,8 @@
 // memory first (2 bytes a code against half a byte read).  The order of the
 // reduced index is free, so a lane reads consecutive dims of a key: its 32
 // nibbles are one 16-byte load at hd = 128.
-// m only moves when a score passes it by 2^8 (a vote, no shuffles): weights
-// reach 2^15, which FP16 allows.
+// m only moves when a score passes it by 2^6 (a vote, no shuffles): weights
+// reach 2^14, which FP16 allows.
 //
 // Chunks of one request are joined by k_attn_join from the rows' (m, l, O)
 // in FP32.
@@ -288,6 +288,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
   }
   uint32_t stage = 0, parity = 0;
   bool ok = true, bad_page = false;
+  // Scores take their factor before the maximum: a cap, a bias, or an m that
+  // has been far (kFar).
+  bool shaped = capped || j.slopes != nullptr;
   while (at < mine) {
     if (in_flight == 0u) {  // the loaded pages are used up
       load_pages(at);
@@ -395,7 +398,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
     // a request's last for single tokens) skip the masks.
     const bool clear = (k0 >= last.lo && first.hi - k0 >= static_cast<int32_t>(kTile)) ||
                        first.pre - k0 >= static_cast<int32_t>(kTile);
-    const bool shaped = capped || j.slopes != nullptr;
     if (wide) {  // a branch of its own: the others' arithmetic is not doubled
 #pragma unroll
       for (uint32_t nt = 0; nt < NT; ++nt)
@@ -442,10 +444,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
       for (uint32_t c = 0; c < 2u; ++c) {
         top[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][c + 2u]), fmaxf(s[nt][1][c], s[nt][1][c + 2u])) *
                      (shaped ? 1.0f : factor[nt][c]);
-        moves |= top[nt][c] > m[nt][c] + kLazy;
+        moves |= top[nt][c] - m[nt][c] > kLazy;
       }
     }
     if (__any_sync(0xFFFFFFFFu, moves)) {
+      bool large = false;
 #pragma unroll
       for (uint32_t nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -457,6 +460,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
           const float to = fmaxf(m[nt][c], x);
           const float keep = to == -INFINITY ? 1.0f : ex2(m[nt][c] - to);
           m[nt][c] = to;
+          large |= attn_far(to);
           l[nt][c] *= keep;
 #pragma unroll
           for (uint32_t i = 0; i < kSteps; ++i) {
@@ -464,6 +468,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1u ? 4 : 2)
             o[nt][i][c + 2u] *= keep;
           }
         }
+      }
+      if (!shaped && __any_sync(0xFFFFFFFFu, large)) {
+        shaped = true;
+#pragma unroll
+        for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (uint32_t c = 0; c < 8u; ++c) s[nt][c / 4u][c & 3u] *= factor[nt][c & 1u];
       }
     }
     // P^T as the B operand: pairs of keys in a lane, rows across lanes.

@@ -18,7 +18,7 @@
 //   warp 9          bulk copies of K and V^T tiles, two stages each
 // (with one half a block, 0-3, 4 and 5, and one stage at hd 96 and 128).  While
 // one half's softmax runs, the other half's products do; with one half, another
-// block's.  m moves only when a row's scores pass it by 2^8,
+// block's.  m moves only when a row's scores pass it by 2^6,
 // so O is rarely scaled.
 //
 // Few blocks (a short chunk over a long cache) split the keys; k_attn_join
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
     const uint32_t lanes = ((warp & 3u) * 32u) << 16;
     const uint32_t t_s = tmem + lanes + 128u * h, t_o = tmem + lanes + S::kO + 128u * h;
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
+    bool ok = true, far = false;  // far: some row's m of the warp has been (kFar)
     if (h < halves) {
       for (int32_t it = 0; it < count; ++it) {
         ok = mbar_wait(s_full + h, static_cast<uint32_t>(it) & 1u, error_flag);
@@ -628,10 +628,20 @@ __global__ void __launch_bounds__(Cfg<HD, HV>::kThreads, HV == 2u ? 1 : 2)
         for (uint32_t c = 0; c < 8u; ++c) top[c] = fmaxf(top[c], at(c >> 1, 16u * (c & 1u) + 15u));
         const float high = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]),
                                 fmaxf(top[6], top[7])) * scale;
-        const bool moves = high > m + kLazy;
-        if (__any_sync(0xFFFFFFFFu, moves)) {
+        const bool moves = high - m > kLazy;
+        if (__any_sync(0xFFFFFFFFu, moves || far)) {
           const float keep = moves ? ex2(m - high) : 1.0f;
           if (moves) m = high;
+          if constexpr (!SHAPED) {
+            far = far || __any_sync(0xFFFFFFFFu, attn_far(m));
+            if (far) {
+#pragma unroll
+              for (uint32_t c = 0; c < 4u; ++c)
+#pragma unroll
+                for (uint32_t i = 0; i < 32u; ++i) s[c][i] = __float_as_uint(__fmul_rn(at(c, i), scale));
+              scale = 1.0f;
+            }
+          }
           l *= keep;
           if (it != 0) {
 #pragma unroll 1

@@ -11,11 +11,17 @@
 
 namespace hrb {
 
-constexpr float kLazy = 8.0f;    // log2 of the most a score may pass m before m moves
-// Weights are 2^(s - m + kLift), up to 2^15: FP16 keeps what lies down to 2^-31
-// of the largest (2^-24 without it), and the factor cancels in O / l.
-constexpr float kLift = 7.0f;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 6.0f;    // log2 of the most a score may pass m before m moves
+// Weights are 2^(s - m + kLift), up to 2^14 (kLift may round to 8 where m is
+// large): FP16 keeps what lies down to 2^-31 of the largest (2^-24 without it),
+// and the factor cancels in O / l.
+constexpr float kLift = 7.0f;
+// From here on the rounding of a maximum (the score's product with its factor,
+// half a unit of 2^-23) is no longer small beside kLazy, and a fused s factor - m
+// would be off by it: the products are rounded first, as the maximum was.
+constexpr float kFar = 0x1p20f;
+__device__ __forceinline__ bool attn_far(float m) { return fabsf(m) >= kFar && fabsf(m) < INFINITY; }
 
 constexpr uint32_t kAttnTileKeys = 128;  // keys a tile of the prompt kernel
 

@@ -486,3 +486,29 @@ def test_attention_mxint8_copy_of_joined_and_two_half_rows(hrb, hd):
             value = codes.reshape(want.shape) * step
             tol = 0.5 * step + 2.0 ** -9 * mass + np.where(np.abs(codes.reshape(want.shape)) == 127, step, 0)
             assert (np.abs(value - want) <= tol).all()
+
+
+@pytest.mark.parametrize("power", [10, 19, 20, 24, 27, 28, 30, 40, 100])
+@pytest.mark.parametrize("lens", [[(1, 300), (3, 700)], [(90, 300)], [(70, 1200)]], ids=["few", "prompt", "long"])
+@pytest.mark.parametrize("form", ["plain", "cap", "bias"])
+def test_attention_equal_scores_of_any_size(hrb, lens, power, form):
+    """Scores are 0, 4 or 6 times 2^power, without rounding: the keys of 6
+    share all the weight (the others' is under 2^-1000).  Left is the output's
+    BF16 rounding, 2^-8, and the weights' FP16 rounding, 2^-11 of the values."""
+    rng = np.random.default_rng(70)
+    s = Step(rng, lens, 2, 1, 32, 16)
+    s.q[:] = 0.0
+    s.q[:, 0] = s.q[:, 32] = 2.0 ** power
+    s.scale = 1.0
+    for n, (_, kv) in enumerate(lens):
+        big = rng.random(kv)
+        for j in range(kv):
+            key = np.zeros((1, 32))
+            key[0, 0] = 6.0 if big[j] < 0.1 or j == kv // 2 else rng.choice((0.0, 4.0))
+            s.cache.write(int(s.table[n, j // 16]) * 16 + j % 16, key, s.values[n][j])
+            s.keys[n][j] = key
+    want, mass = s.want(causal=False)
+    kw = {"plain": {}, "cap": dict(softcap=2e38), "bias": dict(slopes=np.zeros(2, np.float32))}[form]
+    got = s.run(hrb, causal=False, **kw)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -11 * mass).all()
