@@ -23,9 +23,9 @@
 // in FP32.
 //
 // Its floor is HBM: hd + hd / 16 bytes a key and head.  Measured (32/8 heads of
-// 128; ranges over several boxes): 64 requests of up to 16384 keys 180 to
-// 184 us, 4.0 TB/s, 60 to 62 % of a copy's rate; one request of 131071 keys 43 to
-// 44 us; one of 241 keys (15/5 heads of 64) 4.4 to 4.7 us.  Bound by the lanes'
+// 128; ranges over several boxes): 64 requests of up to 16384 keys 181 to
+// 187 us, 3.9 to 4.0 TB/s, 59 to 61 % of a copy's rate; one request of 131071 keys
+// 44 us; one of 241 keys (15/5 heads of 64) 4.6 to 4.8 us.  Bound by the lanes'
 // work: with all pages in L2 it takes as long, 63 % of the issue slots and 54 %
 // of the ALU pipe (the conversions) are used.
 #include <cuda_fp16.h>

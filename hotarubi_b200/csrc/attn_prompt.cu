@@ -25,8 +25,8 @@
 // (attn_decode.cu) joins the rows' (m, l, O).
 //
 // Its floor is the tensor cores: 4 hd FLOP a pair of query and key that see
-// each other.  Measured: a prompt of 8191 tokens, 32/8 heads of 128, 507 to
-// 516 us, 1065 to 1085 TFLOP/s, 64 to 65 % of a large BF16 product's rate.  A tile
+// each other.  Measured: a prompt of 8191 tokens, 32/8 heads of 128, 508 to
+// 520 us, 1057 to 1083 TFLOP/s, 64 to 65 % of a large BF16 product's rate.  A tile
 // takes about 3600 clocks for both halves, the tensor cores work 2048 of them: a
 // half's softmax (2200) and its products (1200 with the waits) follow each
 // other.  Two S of 64 keys a half, which would let a softmax run ahead, measured
